@@ -233,6 +233,150 @@ imi_cuda_status imi_cuda_bench_matvec(int device, int rows, int cols, int ncol, 
 imi_cuda_status imi_cuda_q4_matvec_static(int device, const uint8_t *q4, int rows, int cols, const int8_t *xq,
                                           const float *xd, const float *xs, int ncol, float *out, void *stream);
 
+/* ---- serving operators on device buffers ----
+ *
+ * No counterpart in the reference (imi serves a handful of conversations, each with its own contiguous memory, and picks
+ * greedily): what a server of many conversations on one GPU needs beside the step, as operators a caller runs on buffers
+ * of its own: pages instead of one n_ctx-sized cache per conversation, attention that reads a prompt all conversations
+ * share once for all of them, and sampling.
+ *
+ * In common: every pointer in the argument blocks is device memory of `device` (checked; IMI_E_ARG otherwise), unless it
+ * is said to be optional and is NULL. A call checks its arguments on the host, enqueues its kernels on `stream` (a
+ * cudaStream_t of that device; NULL: the default stream) and returns without waiting; it allocates nothing and may be
+ * captured into a CUDA graph, which then replays with the same pointers and sizes and whatever the buffers hold. The
+ * current device of the calling thread is left as it was. Calls from several threads or on several streams are
+ * independent as long as they write different buffers (outputs, workspaces and status words included).
+ * What only the device can see (lengths, page numbers, slots) is checked there: nothing outside the buffers is read or
+ * written, and the largest IMI_DEV_* code met is left in the call's status word (atomic maximum; a call never clears
+ * it: the caller zeroes it when it has read it). */
+typedef enum { IMI_F32 = 0, IMI_F16 = 1, IMI_BF16 = 2 } imi_cuda_type;
+enum {
+    IMI_DEV_PAGE = 1,    /* a page number outside 0..n_pages-1, or a slot beyond the last page */
+    IMI_DEV_TABLE = 2,   /* a request longer than its block table's row holds */
+    IMI_DEV_CAP = 3,     /* the step's new positions exceed the slot arrays */
+    IMI_DEV_POOL = 4,    /* not enough free pages (or a free count outside the list) */
+    IMI_DEV_LENGTH = 5   /* a negative number of new positions */
+};
+
+/* Block tables and slot maps from the requests' lengths.
+ * Request i holds held[i] positions and adds add[i]; its pages are table[i * table_stride + c], c counting pages of
+ * `page` positions (a power of two, 16..256). Pages it lacks are taken from the end of the free list (a stack: page
+ * k-th taken is free_pages[n_free - 1 - k]), request by request, and entered into its row; nothing else of the table
+ * is written. held[i] < 0 marks a row that is not in use (add ignored, length -1).
+ *   start[n + 1]   exclusive sums of add: request i's new positions are rows start[i]..start[i+1]-1 of the step
+ *   length[n]      held + add
+ *   slots[cap]     per new row: page number * page + offset in the page; -1 behind the last
+ *   pos[cap]       per new row: its position, pos0 + (position within the request's own pages); -1 behind the last
+ *   n_free_out[1]  free pages left (the list itself is not written)
+ * length may be held's buffer, n_free_out may be n_free's (the next step's inputs in place). When a request passes
+ * its table row (IMI_DEV_TABLE), the new rows exceed cap, the pool is short or a length is negative, the step maps
+ * nothing: slots and pos are -1 throughout, start 0, length = held, n_free_out = n_free, the table as it was. A page
+ * number outside the pool (IMI_DEV_PAGE) makes its slots -1. status[2]: the status word, then a counter that must be 0
+ * before the first call and is 0 after every call; calls that share status run one after the other. n <= 4096. */
+typedef struct {
+    const int32_t *held, *add;
+    int n;
+    int32_t *table;
+    int64_t table_stride;
+    int width;                      /* pages per table row */
+    const int32_t *free_pages;
+    int free_cap;                   /* entries of free_pages (0: none) */
+    const int32_t *n_free;
+    int page, n_pages, pos0, cap;
+    int32_t *start, *length, *slots, *pos, *n_free_out, *status;
+} imi_cuda_page_map_args;
+imi_cuda_status imi_cuda_page_map(int device, const imi_cuda_page_map_args *a, void *stream);
+
+/* K and V rows into pages: row r, head h of k (k + r * row_stride + h * head_stride, in elements; v alike) goes to
+ * offset slots[r] % page of page slots[r] / page of k_pages, [n_pages][n_head_kv][page][head_dim] (v_pages alike),
+ * rounded to nearest even where the pages' type is narrower. slots[r] < 0: row r is skipped. head_dim a multiple of 8,
+ * at most 256; pages IMI_F16 or IMI_BF16, rows those of the pages' type or IMI_F32; pages 16-byte aligned (rows of any
+ * alignment; 16-byte aligned ones with strides of whole 16 bytes are read in 16-byte pieces). Slots of one call are
+ * distinct, as imi_cuda_page_map makes them: of rows with the same slot each element is one of theirs. status optional. */
+typedef struct {
+    const void *k, *v;
+    int type;                       /* imi_cuda_type of the rows */
+    int64_t row_stride, head_stride;
+    int rows;
+    const int32_t *slots;
+    int n_head_kv, head_dim;
+    void *k_pages, *v_pages;
+    int page_type, page, n_pages;
+    int32_t *status;
+} imi_cuda_page_write_args;
+imi_cuda_status imi_cuda_page_write(int device, const imi_cuda_page_write_args *a, void *stream);
+
+/* Attention of one new token per conversation over a prompt that all of them share and the conversation's own pages.
+ * Conversation i sees the prompt's prefix_len positions (the pages prefix[0..], in order, the last one possibly in part)
+ * and then its own length[i] positions (pages table[i * table_stride + c]); with window > 0 only the last `window` of
+ * these prefix_len + length[i] positions (the engine's sliding-window layers: the query's own position included).
+ *   out[i][h] = sum_j p_j V_j,  p = softmax(scale * q[i][h] . K_j),  lse[i][h] = log sum_j exp(scale * q . K_j)
+ * Head h reads kv head h / (n_head / n_head_kv). The prompt's pages are read once for the whole batch. A conversation
+ * that sees nothing gets out 0 and lse -infinity. length[i] < 0: the row is not in use, its out and lse stay as they
+ * were. Positions beyond a length may hold anything, NaN included; a NaN or infinity in V at a prompt position that some
+ * conversation's window includes may reach the others' outputs too.
+ * type: IMI_F16 or IMI_BF16, of q and the pages; products, softmax and sums are held in 32 bits, the probabilities
+ * rounded to `type` for their product with V. out_type: any imi_cuda_type. head_dim 64 or 128; n_head / n_head_kv at
+ * most 16; rows at most 4096; page a power of two, 16..256; q and pages 16-byte aligned, q's and out's rows
+ * q_stride / out_stride elements apart (multiples of 8), heads head_dim apart. A length beyond its table row
+ * (IMI_DEV_TABLE) counts as the row's positions; a page number outside the pool (IMI_DEV_PAGE) hides its positions.
+ * work: imi_cuda_prefix_attn_work(...) bytes, 16-byte aligned, nothing expected in it; calls that may overlap need one
+ * each. lse and status optional. */
+typedef struct {
+    const void *q;
+    int type;
+    int64_t q_stride;
+    int rows, n_head, n_head_kv, head_dim;
+    const void *k_pages, *v_pages;
+    int page, n_pages;
+    const int32_t *prefix;
+    int prefix_len;
+    const int32_t *table;
+    int64_t table_stride;
+    int width;                      /* pages per table row (0: no own pages) */
+    const int32_t *length;
+    float scale;
+    int window;
+    void *out;
+    int out_type;
+    int64_t out_stride;
+    float *lse;
+    void *work;
+    size_t work_bytes;
+    int32_t *status;
+} imi_cuda_prefix_attn_args;
+/* workspace bytes of a call of at most these sizes (smaller ones of the same heads fit) */
+size_t imi_cuda_prefix_attn_work(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len, int width, int page);
+imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefix_attn_args *a, void *stream);
+
+/* A word per row of scores[n][vocab] (rows `stride` elements apart, any imi_cuda_type) from a given uniform number u[i]
+ * in [0, 1). With x the row's scores, w_j = exp((x_j - max x) / temperature), words ordered by score, equal scores by id:
+ *   top-k  the first top_k words (0 or less: all)
+ *   top-p  of those, the words before which less than top_p of their total weight lies (1 or more, or NaN: all); the
+ *          first always
+ *   min-p  of those, the words of w_j >= min_p (0 or less, or NaN: all); the first always
+ * ids[i] is the first word, by id, at which the running sum of the kept weights exceeds u[i] times their total;
+ * logprob[i] = log(its weight / that total); kept[i] the number of words kept. temperature 0 (or negative, or NaN):
+ * the greedy pick (highest score, lowest id), logprob 0, kept 1, as imi_cuda_get_argmax. Words of score -infinity or NaN are
+ * never kept; a row of nothing else gives id -1, logprob -infinity, kept 0. Scores of +infinity share the row evenly.
+ * Weights are exact to 2^-44 of the largest word's and summed as integers: the word does not depend on the order of
+ * the sums. Per-row settings (temperature, top_k, top_p, min_p) are optional; without them 1, 0, 1, 0.
+ * vocab at most IMI_CUDA_SAMPLE_VOCAB. logprob and kept optional. */
+#define IMI_CUDA_SAMPLE_VOCAB 262144
+typedef struct {
+    const void *scores;
+    int type;
+    int64_t stride;
+    int n, vocab;
+    const float *u, *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    int32_t *ids;
+    float *logprob;
+    int32_t *kept;
+} imi_cuda_sample_args;
+imi_cuda_status imi_cuda_sample(int device, const imi_cuda_sample_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

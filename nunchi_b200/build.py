@@ -18,7 +18,7 @@ OUT = os.path.join(HERE, "libimi_cuda.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 HOST = "-O3,-fPIC,-ffp-contract=off,-fno-math-errno"
-SOURCES = ["kernels.cu", "engine.cpp", "gguf_file.cpp", "rope_host.cpp"]
+SOURCES = ["kernels.cu", "serve_sample.cu", "serve_attn.cu", "serve_pages.cu", "engine.cpp", "gguf_file.cpp", "rope_host.cpp"]
 
 
 def _stale() -> bool:
@@ -34,8 +34,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return OUT
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
-    objs = []
-    for s in SOURCES:
+    objs, running = [], []
+    for s in SOURCES:   # compiled beside one another
         o = os.path.join(objdir, os.path.splitext(s)[0] + ".o")
         cmd = [NVCC, "-c", os.path.join(SRC, s), "-o", o, "-std=c++17", "-O3", "-lineinfo", "--fmad=false",
                "-Xcompiler", HOST, *ARCH]
@@ -43,8 +43,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
             cmd[1:1] = ["-x", "cu"] if s == "engine.cpp" else []
         if verbose:
             print(" ".join(cmd))
-        subprocess.run(cmd, check=True)
+        running.append(subprocess.Popen(cmd))
         objs.append(o)
+    codes = [(p.wait(), p.args) for p in running]
+    for code, cmd in codes:
+        if code:
+            raise subprocess.CalledProcessError(code, cmd)
     tmp = OUT + f".tmp{os.getpid()}"
     subprocess.run([NVCC, "-shared", "-o", tmp, *objs, *ARCH, "-lcudart"], check=True)
     os.replace(tmp, OUT)

@@ -11,6 +11,7 @@
 #include "../../include/imi_cuda.h"
 #include "gguf_file.h"
 #include "launch.h"
+#include "serve.h"
 
 #include <cudaTypedefs.h>
 
@@ -37,6 +38,8 @@ static imi_cuda_status fail(imi_cuda_status st, const std::string &msg) {
     g_err = msg;
     return st;
 }
+// the same message for the other files of the library (serve.h)
+imi_cuda_status imi::set_error(imi_cuda_status st, const std::string &msg) { return fail(st, msg); }
 #define CK(x)                                                                                                 \
     do {                                                                                                      \
         cudaError_t e_ = (x);                                                                                 \

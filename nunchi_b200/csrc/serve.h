@@ -1,0 +1,97 @@
+// What the serving operators' files (serve_pages.cu, serve_attn.cu, serve_sample.cu) share on the host: the error
+// message of the library, the checks of a call's device and buffers, and the launch with programmatic serialization.
+#pragma once
+#include "../../include/imi_cuda.h"
+
+#include <cuda_runtime.h>
+
+#include <initializer_list>
+#include <mutex>
+#include <string>
+
+namespace imi {
+imi_cuda_status set_error(imi_cuda_status st, const std::string &msg);   // engine.cpp: the text of imi_cuda_error()
+
+// makes `device` current while it lives; ok() false: there is no such device
+class OnDevice {
+    int prev_ = -1;
+    bool ok_ = false;
+
+public:
+    explicit OnDevice(int device) {
+        if (device < 0 || cudaGetDevice(&prev_) != cudaSuccess) {
+            cudaGetLastError();
+            return;
+        }
+        ok_ = prev_ == device || cudaSetDevice(device) == cudaSuccess;
+        if (!ok_) cudaGetLastError();
+    }
+    ~OnDevice() {
+        int now = -1;
+        if (prev_ >= 0 && cudaGetDevice(&now) == cudaSuccess && now != prev_) cudaSetDevice(prev_);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+    bool ok() const { return ok_; }
+};
+
+// every non-null pointer is device memory of `device` (or managed memory)
+inline bool all_on_device(std::initializer_list<const void *> ps, int device) {
+    for (const void *p : ps) {
+        if (!p) continue;
+        cudaPointerAttributes at = {};
+        if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        if (!(at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == device))) return false;
+    }
+    return true;
+}
+
+inline bool aligned(const void *p, size_t n) { return ((uintptr_t) p) % n == 0; }
+inline bool page_ok(int page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0; }
+inline int log2i(int x) {
+    int k = 0;
+    while ((1 << k) < x) k++;
+    return k;
+}
+
+// a launch that may start while its predecessor on the stream drains: the kernel calls pdl_wait() before it reads or
+// writes anything the predecessor may touch
+inline cudaError_t launch_pdl(const void *fn, dim3 grid, int threads, size_t smem, cudaStream_t st, void **args,
+                              int cluster = 1) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+// raises a kernel's shared-memory limit once per device (the attribute belongs to the device that is current)
+constexpr int MAX_DEVICES = 64;
+struct SmemLimit {
+    std::mutex mu;
+    bool done[MAX_DEVICES] = {};
+    cudaError_t raise(int device, std::initializer_list<const void *> fns, int bytes) {
+        std::lock_guard<std::mutex> g(mu);
+        if (device < MAX_DEVICES && done[device]) return cudaSuccess;
+        for (const void *f : fns) {
+            const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (e != cudaSuccess) return e;
+        }
+        if (device < MAX_DEVICES) done[device] = true;
+        return cudaSuccess;
+    }
+};
+}  // namespace imi

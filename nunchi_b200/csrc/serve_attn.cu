@@ -1,0 +1,670 @@
+// Attention of one new token per conversation over a shared prompt and the conversation's own pages
+// (imi_cuda_prefix_attn).
+//
+// For a query row (conversation i, head h) with scores s_j = scale q . K_j over the positions it sees,
+//     out = sum_j 2^(s_j log2 e - m) V_j / l,   l = sum_j 2^(s_j log2 e - m),   lse = (m + log2 l) / log2 e,
+// for any m; a pass keeps m as the running maximum (online softmax), so a list of positions can be cut anywhere: each
+// piece gives (m, l, sum) and pieces join by rescaling to the largest m. The shared prompt is cut into pieces that
+// serve all conversations at once (rows of many conversations against one read of K and V); each conversation's own
+// positions into pieces of equal length; k_join adds them up.
+#include "common.cuh"
+#include "serve.h"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cmath>
+
+namespace imi {
+namespace {
+
+constexpr int PA_ROWS = 4096;             // conversations at most
+constexpr int PA_WARPS = 4;               // warps of a piece's CTA
+constexpr int PA_STEP = 16;               // positions of a warp's step (a page holds whole steps)
+constexpr int PA_MIN_STEPS = 2 * PA_WARPS;   // steps of an own piece at least
+constexpr int PA_OWN_ITEMS = 1184;        // (piece, kv head) items aimed at for the own positions: 148 SMs x 8
+constexpr int PA_PRE_ITEMS = 592;         // (row tile, kv head, piece) items aimed at for the prompt: 148 SMs x 4
+constexpr int PA_DIRECT = 1024;           // positions (prompt and own) up to which one CTA takes a row alone
+constexpr int PA_DWARPS = 8;              // its warps
+
+struct PaArgs {
+    imi_cuda_prefix_attn_args a;
+    int shift, g;               // log2(page); heads per kv head
+    float sl2;                  // scale * log2(e)
+    int pre_splits, pre_len;    // pieces of the prompt and their positions
+    float *po;                  // pieces' sums [slot][head_dim]: prompt slots (row * n_head + head) * pre_splits + piece,
+    float2 *pml;                // then own slots (off[row] + piece) * n_head + head; (m, l) per slot
+    int own_slot0;              // the first own slot
+    int *off;                   // own pieces in front of each row [rows + 1]
+};
+
+template <typename T> struct Half2;
+template <> struct Half2<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *(const uint32_t *) &h;
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <> struct Half2<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *(const uint32_t *) &h;
+    }
+    static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 ldg16(const void *p) { return __ldg((const uint4 *) p); }
+
+template <typename O> __device__ __forceinline__ void put4(O *p, float4 v);
+template <> __device__ __forceinline__ void put4<float>(float *p, float4 v) { *(float4 *) p = v; }
+template <> __device__ __forceinline__ void put4<__half>(__half *p, float4 v) {
+    *(uint2 *) p = make_uint2(Half2<__half>::pack(v.x, v.y), Half2<__half>::pack(v.z, v.w));
+}
+template <> __device__ __forceinline__ void put4<__nv_bfloat16>(__nv_bfloat16 *p, float4 v) {
+    *(uint2 *) p = make_uint2(Half2<__nv_bfloat16>::pack(v.x, v.y), Half2<__nv_bfloat16>::pack(v.z, v.w));
+}
+__device__ __forceinline__ void put_out(const imi_cuda_prefix_attn_args &a, long long at, float4 v) {
+    if (a.out_type == IMI_F32) put4((float *) a.out + at, v);
+    else if (a.out_type == IMI_F16) put4((__half *) a.out + at, v);
+    else put4((__nv_bfloat16 *) a.out + at, v);
+}
+
+// the positions of conversation i that its query sees: the prompt's from `plo`, its own from `olo` to `len`
+struct Seen {
+    int len, plo, olo;
+};
+__device__ __forceinline__ Seen seen_of(const PaArgs &p, int i) {
+    const imi_cuda_prefix_attn_args &a = p.a;
+    int len = a.length[i];
+    const int cap = a.width << p.shift;
+    if (len > cap) {
+        if (a.status) atomicMax(a.status, IMI_DEV_TABLE);
+        len = cap;
+    }
+    const int low = a.window > 0 && len >= 0 ? max(0, a.prefix_len + len - a.window) : 0;
+    return { len, min(low, a.prefix_len), max(0, low - a.prefix_len) };
+}
+
+// ---- a warp's pass over 16 query rows: matrix instructions on registers alone ----
+// m16n8k16 sums over k in any order, so K is read as the lanes can load it: lane (n = lane / 4, t = lane % 4) takes
+// whole 16-byte pieces 8t..8t+7 (+32, ..) of position n's row, and the query's operand uses the same order. V needs two
+// positions of one dimension in a register: lane (w = lane / 4, t) loads the 16 bytes 8w..8w+7 of positions 2t, 2t+1,
+// 2t+8, 2t+9 and pairs them with byte permutes; product j then holds dimension 8n + j at its column n. Nothing passes
+// through shared memory. R8: at most 8 query rows (the fragment's upper rows are zero and not kept).
+template <typename T, int D, bool R8>
+struct Pass {
+    static constexpr int KC = D / 32, NO = D / 8, HV = D / 64, RH = R8 ? 2 : 4;
+    uint32_t q[D / 16][R8 ? 2 : 4];
+    float o[NO][RH];
+    float m0, m1, l0, l1;
+
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int j = 0; j < NO; j++)
+#pragma unroll
+            for (int e = 0; e < RH; e++) o[j][e] = 0.0f;
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.0f;
+    }
+    // the query's operand: qr0, qr1 the rows of this lane (null: zeros)
+    __device__ __forceinline__ void load_q(const T *qr0, const T *qr1) {
+        const int t = threadIdx.x & 3;
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            if (qr0) x = ldg16(qr0 + 32 * c + 8 * t);
+            if (!R8 && qr1) y = ldg16(qr1 + 32 * c + 8 * t);
+            if constexpr (R8) {
+                q[2 * c][0] = x.x; q[2 * c][1] = x.y; q[2 * c + 1][0] = x.z; q[2 * c + 1][1] = x.w;
+            } else {
+                q[2 * c][0] = x.x; q[2 * c][1] = y.x; q[2 * c][2] = x.y; q[2 * c][3] = y.y;
+                q[2 * c + 1][0] = x.z; q[2 * c + 1][1] = y.z; q[2 * c + 1][2] = x.w; q[2 * c + 1][3] = y.w;
+            }
+        }
+    }
+    // positions [lo, hi) of the pages `list`, steps first, first + stride, .. of 16 positions; lo0, lo1: what this
+    // lane's rows see from (>= lo); kb, vb: the kv head's rows in page 0; ps: elements from page to page
+    __device__ void run(const PaArgs &p, const int32_t *list, const T *kb, const T *vb, long long ps, int lo, int hi, int lo0,
+                        int lo1, int first, int stride) {
+        const int lane = threadIdx.x & 31, w = lane >> 2, t = lane & 3, end = (hi + PA_STEP - 1) / PA_STEP;
+        int s = lo / PA_STEP + first;
+        if (s >= end || lo >= hi) return;
+        auto page_at = [&](int step) {
+            const int id = step < end ? __ldg(list + (step * PA_STEP >> p.shift)) : 0;
+            if ((unsigned) id < (unsigned) p.a.n_pages) return id;
+            if (p.a.status) atomicMax(p.a.status, IMI_DEV_PAGE);
+            return -1;
+        };
+        uint4 kr[2][KC];
+        auto load_k = [&](int step, int id) {
+            if (id < 0) id = 0;   // a page that does not exist: page 0 is read and masked
+            const T *r = kb + id * ps + (long long) ((step * PA_STEP & (p.a.page - 1)) + w) * D + 8 * t;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int c = 0; c < KC; c++) kr[i][c] = ldg16(r + 8 * i * D + 32 * c);
+        };
+        int id = page_at(s);
+        load_k(s, id);
+        int id1 = page_at(s + stride);
+        for (; s < end; s += stride) {
+            // this step's V on its way while the scores are made
+            uint4 vr[4][HV];
+            {
+                const T *r = vb + max(id, 0) * ps + (long long) ((s * PA_STEP & (p.a.page - 1)) + 2 * t) * D + 8 * w;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int h = 0; h < HV; h++) vr[i][h] = ldg16(r + ((i & 1) + 8 * (i >> 1)) * D + 64 * h);
+            }
+            float c[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KC; j++) {
+                    const uint4 k = kr[i][j];
+                    uint32_t a0[4], a1[4];
+                    if constexpr (R8) {
+                        a0[0] = q[2 * j][0]; a0[1] = 0; a0[2] = q[2 * j][1]; a0[3] = 0;
+                        a1[0] = q[2 * j + 1][0]; a1[1] = 0; a1[2] = q[2 * j + 1][1]; a1[3] = 0;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) { a0[e] = q[2 * j][e]; a1[e] = q[2 * j + 1][e]; }
+                    }
+                    Half2<T>::mma(c[i], a0, k.x, k.y);
+                    Half2<T>::mma(c[i], a1, k.z, k.w);
+                }
+            }
+            const int base = s * PA_STEP, id_now = id;
+            id = id1;
+            if (s + stride < end) load_k(s + stride, id);
+            id1 = page_at(s + 2 * stride);
+            // the scores in powers of two; positions outside [lo.., hi) masked
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < RH; e++) c[i][e] *= p.sl2;
+            if (base < lo0 || base < lo1 || base + PA_STEP > hi || id_now < 0) {
+                const int from = id_now < 0 ? hi : 0;
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int e = 0; e < RH; e++) {
+                        const int at = base + 8 * i + 2 * t + (e & 1);
+                        if (at >= hi || at < max(from, e < 2 ? lo0 : lo1)) c[i][e] = -INFINITY;
+                    }
+            }
+            if (base < lo || base + PA_STEP > hi || id_now < 0)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {   // what no row sees may be anything: 0 x NaN must not reach the sums
+                    const int at = base + 2 * t + (i & 1) + 8 * (i >> 1);
+                    if (at < lo || at >= hi || id_now < 0)
+#pragma unroll
+                        for (int h = 0; h < HV; h++) vr[i][h] = make_uint4(0, 0, 0, 0);
+                }
+            float x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
+            x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 1));
+            x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 2));
+            const float n0 = fmaxf(m0, x0);
+            float n1 = -INFINITY;
+            if constexpr (!R8) {
+                float x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
+                x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 1));
+                x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 2));
+                n1 = fmaxf(m1, x1);
+            }
+            const float u0 = n0 == -INFINITY ? 0.0f : n0, u1 = n1 == -INFINITY ? 0.0f : n1;
+            if (__any_sync(~0u, n0 != m0 || (!R8 && n1 != m1))) {
+                const float f0 = ex2(m0 - u0), f1 = R8 ? 1.0f : ex2(m1 - u1);
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int j = 0; j < NO; j++) {
+                    o[j][0] *= f0; o[j][1] *= f0;
+                    if constexpr (!R8) { o[j][2] *= f1; o[j][3] *= f1; }
+                }
+                m0 = n0;
+                m1 = n1;
+            }
+            uint32_t pa[4];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float e0 = ex2(c[i][0] - u0), e1 = ex2(c[i][1] - u0);
+                l0 += e0 + e1;
+                pa[2 * i] = Half2<T>::pack(e0, e1);
+                if constexpr (R8) pa[2 * i + 1] = 0;
+                else {
+                    const float e2 = ex2(c[i][2] - u1), e3 = ex2(c[i][3] - u1);
+                    l1 += e2 + e3;
+                    pa[2 * i + 1] = Half2<T>::pack(e2, e3);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < HV; h++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t a = (&vr[0][h].x)[e], b = (&vr[1][h].x)[e], c2 = (&vr[2][h].x)[e], d = (&vr[3][h].x)[e];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const uint32_t sel = k ? 0x7632u : 0x5410u, b0 = __byte_perm(a, b, sel), b1 = __byte_perm(c2, d, sel);
+                        float (&x)[RH] = o[8 * h + 2 * e + k];
+                        if constexpr (R8) {
+                            float y[4] = { x[0], x[1], 0.0f, 0.0f };
+                            Half2<T>::mma(y, pa, b0, b1);
+                            x[0] = y[0];
+                            x[1] = y[1];
+                        } else {
+                            Half2<T>::mma(x, pa, b0, b1);
+                        }
+                    }
+                }
+        }
+    }
+    // the sums of the lanes that share a row
+    __device__ __forceinline__ void finish() {
+        l0 += __shfl_xor_sync(~0u, l0, 1);
+        l0 += __shfl_xor_sync(~0u, l0, 2);
+        if constexpr (!R8) {
+            l1 += __shfl_xor_sync(~0u, l1, 1);
+            l1 += __shfl_xor_sync(~0u, l1, 2);
+        }
+    }
+    // this warp's result into shared memory: rows of D + 4 floats (m, l, and padding that spreads the banks, behind)
+    __device__ __forceinline__ void put(float *sh) const {
+        const int lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int up = 0; up < (R8 ? 1 : 2); up++) {
+            float *row = sh + (r + 8 * up) * (D + 4);
+#pragma unroll
+            for (int h = 0; h < HV; h++)
+#pragma unroll
+                for (int n = 0; n < 2; n++)   // column n of the products: dimensions 64 h + 8 (2t + n) + 0..7
+#pragma unroll
+                    for (int j = 0; j < 8; j += 4)
+                        *(float4 *) (row + 64 * h + 16 * t + 8 * n + j) =
+                            make_float4(o[8 * h + j][2 * up + n], o[8 * h + j + 1][2 * up + n], o[8 * h + j + 2][2 * up + n],
+                                        o[8 * h + j + 3][2 * up + n]);
+            if (t == 0) {
+                row[D] = up ? m1 : m0;
+                row[D + 1] = up ? l1 : l0;
+            }
+        }
+    }
+};
+
+// the NW warps' results of `rows` query rows joined: four dimensions per thread; emit(row, dimension, sum, m, l)
+template <int D, int NW, int ROWS, typename F>
+__device__ __forceinline__ void join_warps(const float *sh, int rows, F emit) {
+    for (int x = threadIdx.x; x < rows * (D / 4); x += NW * 32) {
+        const int r = x / (D / 4), c = x % (D / 4) * 4;
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; k++) m = fmaxf(m, sh[(k * ROWS + r) * (D + 4) + D]);
+        const float u = m == -INFINITY ? 0.0f : m;
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < NW; k++) {
+            const float *row = sh + (k * ROWS + r) * (D + 4);
+            const float f = ex2(row[D] - u);
+            const float4 v = *(const float4 *) (row + c);
+            l = fmaf(f, row[D + 1], l);
+            s.x = fmaf(f, v.x, s.x); s.y = fmaf(f, v.y, s.y); s.z = fmaf(f, v.z, s.z); s.w = fmaf(f, v.w, s.w);
+        }
+        emit(r, c, s, m, l);
+    }
+}
+__device__ __forceinline__ float4 scaled(float4 s, float l) {
+    const float f = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);   // l NaN stays NaN
+    return make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+}
+constexpr float LN2 = 0.693147180559945309f;
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2; }
+
+// ---- few positions: one CTA per (conversation, kv head) takes all of them, its warps step by step in turn ----
+template <typename T, int D, bool R8>
+__global__ void __launch_bounds__(PA_DWARPS * 32) k_pa_direct(const __grid_constant__ PaArgs p) {
+    constexpr int ROWS = R8 ? 8 : 16;
+    extern __shared__ float shf[];
+    const imi_cuda_prefix_attn_args &a = p.a;
+    pdl_wait();
+    pdl_trigger();
+    const int i = blockIdx.x / a.n_head_kv, kvh = blockIdx.x % a.n_head_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Seen v = seen_of(p, i);
+    if (v.len < 0) return;
+    const T *q = (const T *) a.q + i * a.q_stride + (long long) kvh * p.g * D;
+    const int r = lane >> 2;
+    Pass<T, D, R8> f;
+    f.init();
+    f.load_q(r < p.g ? q + r * D : nullptr, r + 8 < p.g ? q + (r + 8) * D : nullptr);
+    const long long ps = (long long) a.n_head_kv * a.page * D, head = (long long) kvh * a.page * D;
+    const T *kb = (const T *) a.k_pages + head, *vb = (const T *) a.v_pages + head;
+    f.run(p, a.prefix, kb, vb, ps, v.plo, a.prefix_len, v.plo, v.plo, warp, PA_DWARPS);
+    f.run(p, a.table + i * a.table_stride, kb, vb, ps, v.olo, v.len, v.olo, v.olo, PA_DWARPS - 1 - warp, PA_DWARPS);
+    f.finish();
+    f.put(shf + warp * ROWS * (D + 4));
+    __syncthreads();
+    join_warps<D, PA_DWARPS, ROWS>(shf, p.g, [&](int row, int c, float4 s, float m, float l) {
+        const int h = kvh * p.g + row;
+        put_out(a, i * a.out_stride + (long long) h * D + c, scaled(s, l));
+        if (c == 0 && a.lse) a.lse[(long long) i * a.n_head + h] = lse_of(m, l);
+    });
+}
+
+// ---- pieces ----
+// own pieces of every row into off[0..rows] (shared memory): steps of 16 positions, `chunk` steps per piece, chosen so
+// that about PA_OWN_ITEMS (piece, kv head) items come out whatever the lengths are. Every CTA works this out from the
+// lengths (4 bytes per row from L2). Returns chunk.
+__device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
+    const imi_cuda_prefix_attn_args &a = p.a;
+    const int tid = threadIdx.x, nt = blockDim.x, per = (a.rows + nt - 1) / nt, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
+    int sum = 0;
+    for (int i = i0; i < i1; i++) {
+        const Seen v = seen_of(p, i);
+        const int steps = v.len > v.olo ? (v.len + PA_STEP - 1) / PA_STEP - v.olo / PA_STEP : 0;
+        off[i + 1] = steps;
+        sum += steps;
+    }
+    auto scan = [&](int x, int &total) {   // exclusive sum over the threads
+        const int lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
+        int y = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(~0u, y, o);
+            if (lane >= o) y += z;
+        }
+        __syncthreads();
+        if (lane == 31) tmp[warp] = y;
+        __syncthreads();
+        int before = 0;
+        total = 0;
+        for (int w = 0; w < nw; w++) {
+            if (w < warp) before += tmp[w];
+            total += tmp[w];
+        }
+        return before + y - x;
+    };
+    int total;
+    scan(sum, total);
+    const long long items = (long long) total * a.n_head_kv;
+    const int chunk = max(PA_MIN_STEPS, (int) ((items + PA_OWN_ITEMS - 1) / PA_OWN_ITEMS));
+    int cnt = 0;
+    for (int i = i0; i < i1; i++) cnt += (off[i + 1] + chunk - 1) / chunk;
+    int at = scan(cnt, total);
+    for (int i = i0; i < i1; i++) {
+        at += (off[i + 1] + chunk - 1) / chunk;
+        off[i + 1] = at;
+    }
+    if (tid == 0) off[0] = 0;
+    __syncthreads();
+    return chunk;
+}
+
+// the pieces: CTA items 0..pre_items-1 are (piece, row tile, kv head) of the prompt, then (piece, kv head) of own positions
+template <typename T, int D, bool R8, bool OWN>
+__global__ void __launch_bounds__(PA_WARPS * 32) k_pa_pieces(const __grid_constant__ PaArgs p) {
+    constexpr int ROWS = R8 ? 8 : 16;
+    extern __shared__ float shf[];
+    __shared__ int tmp[32];
+    const imi_cuda_prefix_attn_args &a = p.a;
+    float *sh = shf;
+    int *off = (int *) (shf + PA_WARPS * ROWS * (D + 4));
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2;
+    const long long ps = (long long) a.n_head_kv * a.page * D;
+    int chunk = 0, items;
+    const int qrows = a.rows * p.g, tiles = (qrows + ROWS - 1) / ROWS;
+    if (OWN) {
+        chunk = own_plan(p, off, tmp);
+        items = off[a.rows] * a.n_head_kv;
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i <= a.rows; i += PA_WARPS * 32) p.off[i] = off[i];
+    } else {
+        items = tiles * a.n_head_kv * p.pre_splits;
+    }
+    for (int it = blockIdx.x; it < items; it += gridDim.x) {
+        Pass<T, D, R8> f;
+        f.init();
+        int fr0, nr, kvh, piece, row = 0;
+        if (OWN) {
+            kvh = it % a.n_head_kv;
+            const int k = it / a.n_head_kv;
+            int lo = 0, hi = a.rows;   // the row whose pieces hold k
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (off[mid] <= k) lo = mid;
+                else hi = mid;
+            }
+            row = lo;
+            piece = k - off[row];
+            fr0 = row * p.g;
+            nr = p.g;
+        } else {
+            kvh = it % a.n_head_kv;
+            const int k = it / a.n_head_kv, tile = k % tiles;
+            piece = k / tiles;
+            fr0 = tile * ROWS;
+            nr = min(ROWS, qrows - fr0);
+        }
+        const T *q = (const T *) a.q + (long long) kvh * p.g * D;
+        auto qrow = [&](int x) -> const T * {
+            if (x >= nr) return nullptr;
+            const int fr = fr0 + x;
+            return q + fr / p.g * a.q_stride + (long long) (fr % p.g) * D;
+        };
+        f.load_q(qrow(r), qrow(r + 8));
+        const long long head = (long long) kvh * a.page * D;
+        const T *kb = (const T *) a.k_pages + head, *vb = (const T *) a.v_pages + head;
+        if (OWN) {
+            const Seen v = seen_of(p, row);
+            const int s0 = v.olo / PA_STEP + piece * chunk, lo = max(v.olo, s0 * PA_STEP), hi = min(v.len, (s0 + chunk) * PA_STEP);
+            f.run(p, a.table + row * a.table_stride, kb, vb, ps, lo, hi, v.olo, v.olo, warp, PA_WARPS);
+        } else {
+            int lo0 = 0, lo1 = 0, lo = piece * p.pre_len;
+            const int hi = min(a.prefix_len, lo + p.pre_len);
+            if (a.window > 0) {
+                if (r < nr) lo0 = seen_of(p, (fr0 + r) / p.g).plo;
+                if (r + 8 < nr) lo1 = seen_of(p, (fr0 + r + 8) / p.g).plo;
+                lo = max(lo, __reduce_min_sync(~0u, min(r < nr ? lo0 : INT32_MAX, r + 8 < nr ? lo1 : INT32_MAX)));
+            }
+            f.run(p, a.prefix, kb, vb, ps, lo, hi, lo0, lo1, warp, PA_WARPS);
+        }
+        f.finish();
+        __syncthreads();   // the item before has been read
+        f.put(sh + warp * ROWS * (D + 4));
+        __syncthreads();
+        join_warps<D, PA_WARPS, ROWS>(sh, nr, [&](int x, int c, float4 s, float m, float l) {
+            const int fr = fr0 + x, i = fr / p.g, h = kvh * p.g + fr % p.g;
+            const long long slot = OWN ? p.own_slot0 + (long long) (off[row] + piece) * a.n_head + h
+                                       : ((long long) i * a.n_head + h) * p.pre_splits + piece;
+            *(float4 *) (p.po + slot * D + c) = s;
+            if (c == 0) p.pml[slot] = make_float2(m, l);
+        });
+    }
+    if (OWN) pdl_wait();
+}
+
+// out and lse of every (row, head) from its pieces: one warp each
+template <int D>
+__global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p) {
+    const imi_cuda_prefix_attn_args &a = p.a;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const long long x = blockIdx.x * 8LL + (threadIdx.x >> 5);
+    if (x >= (long long) a.rows * a.n_head) return;
+    const int i = (int) (x / a.n_head), h = (int) (x % a.n_head);
+    if (a.length[i] < 0) return;
+    const int o0 = p.off[i], on = p.off[i + 1] - o0, n = p.pre_splits + on;
+    auto slot_of = [&](int k) -> long long {
+        return k < p.pre_splits ? x * p.pre_splits + k : p.own_slot0 + (long long) (o0 + k - p.pre_splits) * a.n_head + h;
+    };
+    float m = -INFINITY;
+    for (int k = lane; k < n; k += 32) m = fmaxf(m, p.pml[slot_of(k)].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float u = m == -INFINITY ? 0.0f : m;
+    // D / 4 lanes hold four dimensions each; at D 64 the warp's halves take every other piece
+    constexpr int G = 32 / (D / 4);
+    const int part = lane / (D / 4), c = lane % (D / 4) * 4;
+    float l = 0.0f;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = part; k < n; k += G) {
+        const long long slot = slot_of(k);
+        const float2 ml = p.pml[slot];
+        const float f = ex2(ml.x - u);
+        const float4 v = *(const float4 *) (p.po + slot * D + c);
+        l = fmaf(f, ml.y, l);
+        s.x = fmaf(f, v.x, s.x); s.y = fmaf(f, v.y, s.y); s.z = fmaf(f, v.z, s.z); s.w = fmaf(f, v.w, s.w);
+    }
+    if (G == 2) {
+        l += __shfl_xor_sync(~0u, l, 16);
+        s.x += __shfl_xor_sync(~0u, s.x, 16); s.y += __shfl_xor_sync(~0u, s.y, 16);
+        s.z += __shfl_xor_sync(~0u, s.z, 16); s.w += __shfl_xor_sync(~0u, s.w, 16);
+    }
+    if (part == 0) put_out(a, i * a.out_stride + (long long) h * D + c, scaled(s, l));
+    if (lane == 0 && a.lse) a.lse[x] = lse_of(m, l);
+}
+
+// ---- host ----
+// how a call is cut: pieces of the prompt, slots of the workspace
+struct PaPlan {
+    int splits, len;
+    size_t pre_slots, own_slots;
+    size_t off_bytes, bytes;
+};
+PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len) {
+    PaPlan p = {};
+    const int g = n_head / n_head_kv, R = 16, tiles = (rows * g + R - 1) / R;
+    const int steps = (prefix_len + PA_STEP - 1) / PA_STEP;
+    p.splits = prefix_len ? std::max(1, std::min(PA_PRE_ITEMS / std::max(1, tiles * n_head_kv), steps / PA_MIN_STEPS)) : 0;
+    if (p.splits) {
+        p.len = (steps + p.splits - 1) / p.splits * PA_STEP;
+        p.splits = (prefix_len + p.len - 1) / p.len;
+    }
+    p.pre_slots = (size_t) rows * n_head * p.splits;
+    p.own_slots = ((size_t) rows + (PA_OWN_ITEMS + n_head_kv - 1) / n_head_kv) * n_head;
+    p.off_bytes = ((size_t) (rows + 1) * 4 + 255) / 256 * 256;
+    const size_t slots = p.pre_slots + p.own_slots;
+    p.bytes = p.off_bytes + (slots * 8 + 255) / 256 * 256 + slots * head_dim * 4;
+    return p;
+}
+
+bool pa_shape_ok(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len, int width, int page) {
+    return rows >= 0 && rows <= PA_ROWS && n_head_kv >= 1 && n_head >= n_head_kv && n_head <= 1024 && n_head % n_head_kv == 0 &&
+           n_head / n_head_kv <= 16 && (head_dim == 64 || head_dim == 128) && prefix_len >= 0 && width >= 0 && page_ok(page) &&
+           (int64_t) width * page + prefix_len + page <= INT32_MAX;
+}
+
+template <typename T, int D, bool R8>
+cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
+    const imi_cuda_prefix_attn_args &a = p.a;
+    constexpr int ROWS = R8 ? 8 : 16;
+    void *args[] = { &p };
+    if ((long long) a.prefix_len + ((long long) a.width << p.shift) <= PA_DIRECT)
+        return launch_pdl((const void *) k_pa_direct<T, D, R8>, dim3(a.rows * a.n_head_kv), PA_DWARPS * 32,
+                          (size_t) PA_DWARPS * ROWS * (D + 4) * 4, st, args);
+    cudaError_t r = cudaSuccess;
+    if (pl.splits) {
+        const int items = (a.rows * p.g + 15) / 16 * a.n_head_kv * pl.splits;
+        r = launch_pdl((const void *) k_pa_pieces<T, D, false, false>, dim3(std::min(items, 148 * 16)), PA_WARPS * 32,
+                       (size_t) PA_WARPS * 16 * (D + 4) * 4, st, args);
+    }
+    if (r == cudaSuccess)
+        r = launch_pdl((const void *) k_pa_pieces<T, D, R8, true>, dim3(PA_OWN_ITEMS), PA_WARPS * 32,
+                       (size_t) PA_WARPS * ROWS * (D + 4) * 4 + (a.rows + 1) * 4, st, args);
+    if (r == cudaSuccess)
+        r = launch_pdl((const void *) k_join<D>, dim3((a.rows * a.n_head + 7) / 8), 256, 0, st, args);
+    return r;
+}
+template <typename T>
+cudaError_t launch_pa_t(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
+    const bool r8 = p.g <= 8;
+    if (p.a.head_dim == 64) return r8 ? launch_pa<T, 64, true>(p, pl, st) : launch_pa<T, 64, false>(p, pl, st);
+    return r8 ? launch_pa<T, 128, true>(p, pl, st) : launch_pa<T, 128, false>(p, pl, st);
+}
+template <typename T>
+cudaError_t raise_pa(int device) {
+    static SmemLimit lim;
+    return lim.raise(device,
+                     { (const void *) k_pa_direct<T, 64, true>, (const void *) k_pa_direct<T, 64, false>,
+                       (const void *) k_pa_direct<T, 128, true>, (const void *) k_pa_direct<T, 128, false>,
+                       (const void *) k_pa_pieces<T, 64, false, false>, (const void *) k_pa_pieces<T, 128, false, false>,
+                       (const void *) k_pa_pieces<T, 64, true, true>, (const void *) k_pa_pieces<T, 64, false, true>,
+                       (const void *) k_pa_pieces<T, 128, true, true>, (const void *) k_pa_pieces<T, 128, false, true> },
+                     96 * 1024);
+}
+
+}  // namespace
+}  // namespace imi
+
+using namespace imi;
+
+extern "C" size_t imi_cuda_prefix_attn_work(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len, int width,
+                                            int page) {
+    if (!pa_shape_ok(rows, n_head, n_head_kv, head_dim, prefix_len, width, page)) return 0;
+    return pa_plan(rows, n_head, n_head_kv, head_dim, prefix_len).bytes;
+}
+
+extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefix_attn_args *a, void *stream) {
+    if (!a) return set_error(IMI_E_ARG, "prefix_attn: null argument");
+    if (a->type != IMI_F16 && a->type != IMI_BF16) return set_error(IMI_E_ARG, "prefix_attn: q and pages are IMI_F16 or IMI_BF16");
+    if (a->out_type < IMI_F32 || a->out_type > IMI_BF16) return set_error(IMI_E_ARG, "prefix_attn: bad out_type");
+    if (!pa_shape_ok(a->rows, a->n_head, a->n_head_kv, a->head_dim, a->prefix_len, a->width, a->page))
+        return set_error(IMI_E_ARG, "prefix_attn: unsupported shape (rows up to " + std::to_string(PA_ROWS) +
+                                        ", head_dim 64 or 128, up to 16 heads per kv head, page a power of two in 16..256)");
+    if (a->n_pages < 0 || a->window < 0) return set_error(IMI_E_ARG, "prefix_attn: negative n_pages or window");
+    if (!std::isfinite(a->scale)) return set_error(IMI_E_ARG, "prefix_attn: scale is not finite");
+    if (a->rows == 0) return IMI_OK;
+    if (!a->q || !a->out || !a->length || !a->work) return set_error(IMI_E_ARG, "prefix_attn: null argument");
+    if ((a->prefix_len && !a->prefix) || (a->width && !a->table)) return set_error(IMI_E_ARG, "prefix_attn: no page list");
+    if ((a->prefix_len || a->width) && (!a->k_pages || !a->v_pages || a->n_pages < 1))
+        return set_error(IMI_E_ARG, "prefix_attn: no pages");
+    if (a->width && a->table_stride < a->width) return set_error(IMI_E_ARG, "prefix_attn: table_stride below width");
+    const int64_t row = (int64_t) a->n_head * a->head_dim;
+    if (a->q_stride < row || a->out_stride < row || a->q_stride % 8 || a->out_stride % 8)
+        return set_error(IMI_E_ARG, "prefix_attn: q and out rows are multiples of 8 elements apart, at least n_head * head_dim");
+    if (!aligned(a->q, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16) || !aligned(a->out, 16) || !aligned(a->work, 16) ||
+        !aligned(a->prefix, 4) || !aligned(a->table, 4) || !aligned(a->length, 4) || !aligned(a->lse, 4) || !aligned(a->status, 4))
+        return set_error(IMI_E_ARG, "prefix_attn: a buffer is not aligned (q, pages, out and work: 16 bytes)");
+    const PaPlan pl = pa_plan(a->rows, a->n_head, a->n_head_kv, a->head_dim, a->prefix_len);
+    if (a->work_bytes < pl.bytes)
+        return set_error(IMI_E_ARG, "prefix_attn: the workspace takes " + std::to_string(pl.bytes) + " bytes (imi_cuda_prefix_attn_work)");
+    OnDevice on(device);
+    if (!on.ok()) return set_error(IMI_E_NODEV, "no CUDA device " + std::to_string(device));
+    if (!all_on_device({ a->q, a->k_pages, a->v_pages, a->prefix, a->table, a->length, a->out, a->lse, a->work, a->status }, device))
+        return set_error(IMI_E_ARG, "prefix_attn: every buffer must be device memory of device " + std::to_string(device));
+    PaArgs p = {};
+    p.a = *a;
+    p.shift = log2i(a->page);
+    p.g = a->n_head / a->n_head_kv;
+    p.sl2 = a->scale * 1.44269504088896340736f;
+    p.pre_splits = pl.splits;
+    p.pre_len = pl.len;
+    p.off = (int *) a->work;
+    const size_t slots = pl.pre_slots + pl.own_slots;
+    p.pml = (float2 *) ((uint8_t *) a->work + pl.off_bytes);
+    p.po = (float *) ((uint8_t *) a->work + pl.off_bytes + (slots * 8 + 255) / 256 * 256);
+    p.own_slot0 = (int) pl.pre_slots;
+    const bool half = a->type == IMI_F16;
+    cudaError_t r = half ? raise_pa<__half>(device) : raise_pa<__nv_bfloat16>(device);
+    if (r == cudaSuccess)
+        r = half ? launch_pa_t<__half>(p, pl, (cudaStream_t) stream) : launch_pa_t<__nv_bfloat16>(p, pl, (cudaStream_t) stream);
+    if (r != cudaSuccess) return set_error(IMI_E_CUDA, std::string("prefix_attn: ") + cudaGetErrorString(r));
+    return IMI_OK;
+}

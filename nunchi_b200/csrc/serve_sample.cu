@@ -1,0 +1,621 @@
+// Sampling a word per row of scores (imi_cuda_sample): temperature, top-k, top-p and min-p, from a given uniform number.
+//
+// With w_j = exp((x_j - max x) / temperature) the three filters keep a prefix of the words ordered by (score, id): the
+// first k; those before which less than p of the mass lies; those of w >= m. So the kept set is "score above a value T,
+// and the first c of the words at T", and the pick is the first word, by id, at which the running kept mass exceeds
+// u times its total. Weights are held as integers of 2^-44 (1 is the largest word's): sums are exact whatever the order
+// they are made in, so atomics and parallel sums cannot change which word a border falls on, and 2^18 words fit 62 bits.
+// exp and the borders are computed in 64 bits: a border is missed only where two candidates differ by about 2^-44.
+//
+// A row is held in the shared memory of a cluster of 1 to 8 CTAs, as integer keys that order like the scores: it is
+// read from HBM once, and every later pass is over shared memory. A word of T is found by a histogram over 1,024
+// steps of score (counts, and masses for top-p), whose crossing bin, or everything down to it when that is few words,
+// is gathered and sorted by one CTA; a bin too full for that (masked words, all scores alike) is cut again, by keys.
+#include "common.cuh"
+#include "serve.h"
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+namespace cg = cooperative_groups;
+
+namespace imi {
+namespace {
+
+constexpr int SM_NT = 512, SM_NW = SM_NT / 32;
+constexpr int SM_BINS = 2 * SM_NT;       // two bins per thread in the scans
+constexpr int SM_LIST = 1024;            // words the leading CTA sorts at most
+constexpr int SM_TILE = 128;             // words of a warp's load: four per lane
+constexpr int SM_MAX_CLUSTER = 8;
+constexpr int SM_SLICE = 32768;          // words a CTA holds at most
+constexpr double SM_ONE = 17592186044416.0;   // 2^44
+constexpr double SM_FAR = 31.2;          // exp(-31.2) < 2^-45: such a word's weight rounds to 0
+static_assert((long long) SM_SLICE * SM_MAX_CLUSTER >= IMI_CUDA_SAMPLE_VOCAB, "a row fits a cluster");
+static_assert((long long) IMI_CUDA_SAMPLE_VOCAB <= 1 << 18, "the weights' sum fits 62 bits");
+
+typedef unsigned long long u64;
+
+struct SampleArgs {
+    imi_cuda_sample_args a;
+    int seg, slice;   // words per warp (a multiple of SM_TILE) and per CTA (SM_NW * seg)
+};
+
+// scores as unsigned keys in the same order; -infinity and NaN are 0, and so never kept; the zeros are one
+__device__ __forceinline__ uint32_t key_of(float x) {
+    x = __fadd_rn(x, 0.0f);
+    const uint32_t b = __float_as_uint(x);
+    const uint32_t k = b ^ ((uint32_t) ((int) b >> 31) | 0x80000000u);
+    return x > -INFINITY ? k : 0u;   // false for NaN too
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+struct Totals {
+    unsigned cnt;
+    u64 mass;
+};
+
+struct SampleShared {
+    unsigned cnt[SM_BINS];        // this CTA's histogram
+    u64 mass[SM_BINS];
+    u64 list[SM_LIST];            // leading CTA: (key, ~id) gathered; then sorted
+    u64 w[SM_LIST];
+    unsigned wc[SM_NW];           // scans over the CTA
+    u64 wm[SM_NW];
+    unsigned mx, mn, nvalid, idmin;   // what the cluster reads of this CTA
+    unsigned n_list, lo, hi;
+    Totals part;
+    int bin;                      // found in a scan: the crossing bin, and what lies above it
+    unsigned above, in_bin;
+    u64 mass_above;
+    unsigned T, c;                // the leading CTA's findings
+};
+
+// exclusive sums over the CTA's threads, and the totals
+__device__ __forceinline__ void scan2(SampleShared &s, unsigned &c, u64 &m, unsigned &tc, u64 &tm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned xc = c;
+    u64 xm = m;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned yc = __shfl_up_sync(~0u, xc, o);
+        const u64 ym = __shfl_up_sync(~0u, xm, o);
+        if (lane >= o) { xc += yc; xm += ym; }
+    }
+    __syncthreads();
+    if (lane == 31) { s.wc[warp] = xc; s.wm[warp] = xm; }
+    __syncthreads();
+    unsigned bc = 0;
+    u64 bm = 0;
+    tc = 0;
+    tm = 0;
+#pragma unroll
+    for (int w = 0; w < SM_NW; w++) {
+        if (w < warp) { bc += s.wc[w]; bm += s.wm[w]; }
+        tc += s.wc[w];
+        tm += s.wm[w];
+    }
+    c = bc + xc - c;
+    m = bm + xm - m;
+}
+
+// a word's weight, as a number and as an integer of 2^-44
+struct Weigher {
+    float xmax;
+    uint32_t kmax;
+    double inv;   // 1 / temperature
+    __device__ __forceinline__ double real(uint32_t k) const {
+        if (k == kmax) return 1.0;
+        const double z = ((double) xmax - (double) value_of(k)) * inv;
+        return z < SM_FAR ? exp(-z) : 0.0;
+    }
+    static __device__ __forceinline__ u64 whole(double w) {
+        // w * 2^44 <= 2^44: added to 2^52 its integer part, rounded to nearest, is the low mantissa
+        return (u64) __double_as_longlong(__fma_rn(w, SM_ONE, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    }
+    __device__ __forceinline__ u64 operator()(uint32_t k) const { return whole(real(k)); }
+};
+
+// sorted descending, n a power of two of at most SM_LIST
+__device__ __forceinline__ void sort_desc(u64 *v, int n) {
+    for (int k = 2; k <= n; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int i = threadIdx.x; i < n / 2; i += SM_NT) {
+                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                const u64 x = v[lo], y = v[hi];
+                if ((x < y) == ((lo & k) == 0)) { v[lo] = y; v[hi] = x; }
+            }
+            __syncthreads();
+        }
+}
+
+template <typename S>
+__global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ SampleArgs p) {
+    extern __shared__ __align__(16) uint8_t sm_raw[];
+    SampleShared &s = *(SampleShared *) sm_raw;
+    uint32_t *keys = (uint32_t *) (sm_raw + (sizeof(SampleShared) + 15) / 16 * 16);
+    const imi_cuda_sample_args &a = p.a;
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int) cl.num_blocks(), rank = (int) cl.block_rank();
+    const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int base = rank * p.slice;                       // this CTA's first word
+    if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = 0; }
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    const float temp = a.temperature ? a.temperature[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f,
+                min_p = a.min_p ? a.min_p[row] : 0.0f;
+    int top_k = a.top_k ? a.top_k[row] : 0;
+    float u = a.u[row];
+    u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;          // NaN: 0
+    const bool greedy = !(temp > 0.0f);
+    if (top_p <= 0.0f) top_k = 1;                           // the first word alone
+
+    // 1: the row as keys; the largest, the smallest, how many
+    const S *x = (const S *) a.scores + row * a.stride;
+    const bool vec = ((uintptr_t) (x + base) & (4 * sizeof(S) - 1)) == 0;
+    uint32_t mx = 0, mn = ~0u;
+    unsigned nv = 0;
+    uint32_t *mine = keys + warp * p.seg + 4 * lane;        // the words of a lane, tile by tile
+    const int first = base + warp * p.seg + 4 * lane;
+    auto load = [&](int i) -> float {
+        if constexpr (sizeof(S) == 4) return x[i];
+        else if constexpr (std::is_same<S, __half>::value) return __half2float(x[i]);
+        else return __bfloat162float(x[i]);
+    };
+    for (int o = 0; o < p.seg; o += SM_TILE) {
+        const int i = first + o;
+        float f[4];
+        if (vec && i + 4 <= a.vocab) {
+            if constexpr (sizeof(S) == 4) {
+                const float4 v = __ldg((const float4 *) (x + i));
+                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+            } else {
+                const uint2 v = __ldg((const uint2 *) (x + i));
+                const S *h = (const S *) &v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if constexpr (std::is_same<S, __half>::value) f[e] = __half2float(h[e]);
+                    else f[e] = __bfloat162float(h[e]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) f[e] = i + e < a.vocab ? load(i + e) : -INFINITY;
+        }
+        uint32_t k[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            k[e] = key_of(f[e]);
+            mx = max(mx, k[e]);
+            if (k[e]) { mn = min(mn, k[e]); nv++; }
+        }
+        *(uint4 *) (mine + o) = make_uint4(k[0], k[1], k[2], k[3]);
+    }
+    mx = __reduce_max_sync(~0u, mx);
+    mn = __reduce_min_sync(~0u, mn);
+    nv = __reduce_add_sync(~0u, nv);
+    if (lane == 0) { atomicMax(&s.mx, mx); atomicMin(&s.mn, mn); atomicAdd(&s.nvalid, nv); }
+    cl.sync();
+    mx = 0; mn = ~0u; nv = 0;
+    for (int r = 0; r < C; r++) {
+        const SampleShared &o = *cl.map_shared_rank(&s, r);
+        mx = max(mx, o.mx);
+        mn = min(mn, o.mn);
+        nv += o.nvalid;
+    }
+    auto emit = [&](int id, float lp, int kept) {
+        a.ids[row] = id;
+        if (a.logprob) a.logprob[row] = lp;
+        if (a.kept) a.kept[row] = kept;
+    };
+    if (nv == 0) {
+        if (rank == 0 && tid == 0) emit(-1, -INFINITY, 0);
+        cl.sync();   // no CTA leaves while another may read its shared memory
+        return;
+    }
+    const float xmax = value_of(mx);
+    if (greedy) {
+        unsigned id = ~0u;
+        for (int o = 0; o < p.seg; o += SM_TILE)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (mine[o + e] == mx) id = min(id, (unsigned) (first + o + e));
+        id = __reduce_min_sync(~0u, id);
+        if (lane == 0) atomicMin(&s.idmin, id);
+        cl.sync();
+        if (rank == 0 && tid == 0) {
+            for (int r = 0; r < C; r++) id = min(id, cl.map_shared_rank(&s, r)->idmin);
+            emit((int) id, 0.0f, 1);
+        }
+        cl.sync();
+        return;
+    }
+    const Weigher weigh = { xmax, mx, 1.0 / (double) temp };
+    const bool use_k = top_k > 0 && (unsigned) top_k < nv, use_p = top_p > 0.0f && top_p < 1.0f, use_m = min_p > 0.0f;
+    const double m = fmin((double) min_p, 1.0), pd = (double) top_p;
+
+    // the leading CTA's list of n words holds all that can be kept: the filters, and the pick by id. total_all: the mass
+    // that top-p's share is of where top-k does not cut the list
+    auto finish_list = [&](int n, u64 total_all) {
+        int n2 = 32;
+        while (n2 < n) n2 <<= 1;
+        for (int i = n + tid; i < n2; i += SM_NT) s.list[i] = 0;
+        __syncthreads();
+        sort_desc(s.list, n2);
+        if (use_k) n = min(n, top_k);
+        // two words per thread: weights, their sums, and how many pass
+        u64 wv[2], sum = 0;
+        unsigned pass = 0;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int j = 2 * tid + e;
+            const double w = j < n ? weigh.real((uint32_t) (s.list[j] >> 32)) : 0.0;
+            wv[e] = j < n ? Weigher::whole(w) : 0;
+            if (j < n) s.w[j] = wv[e];
+            if (j < n && (!use_m || j == 0 || w >= m)) pass++;
+            sum += wv[e];
+        }
+        unsigned ex = pass, tp;
+        u64 before = sum, total;
+        scan2(s, ex, before, tp, total);
+        const u64 of = use_k ? total : total_all;
+        const double lim = pd * (double) of;
+        unsigned keep = 0;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int j = 2 * tid + e;
+            if (j < n && (!use_p || j == 0 || (double) before < lim)) keep++;
+            before += wv[e];
+        }
+        unsigned K;
+        u64 dm = 0, dt;
+        scan2(s, keep, dm, K, dt);
+        K = min(K, tp);
+        // by id: (~id, place in the order of scores) sorted descending; the keys move to the histogram's memory
+        n2 = 32;
+        while (n2 < (int) K) n2 <<= 1;
+        for (int j = tid; j < n2; j += SM_NT) {
+            const u64 q = s.list[j];
+            s.cnt[j] = (unsigned) (q >> 32);
+            s.list[j] = j < (int) K ? q << 32 | (unsigned) j : 0;
+        }
+        __syncthreads();
+        sort_desc(s.list, n2);
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int j = 2 * tid + e;
+            wv[e] = j < (int) K ? s.w[(unsigned) s.list[j]] : 0;
+            sum += wv[e];
+        }
+        unsigned d0 = 0, d1;
+        before = sum;
+        scan2(s, d0, before, d1, total);
+        const double target = (double) u * (double) total;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int j = 2 * tid + e;
+            const u64 after = before + wv[e];
+            if (j < (int) K && (double) before <= target && (double) after > target) {
+                const uint32_t key = s.cnt[(unsigned) s.list[j]];
+                const unsigned id = ~(unsigned) (s.list[j] >> 32);
+                const double z = key == mx ? 0.0 : ((double) xmax - (double) value_of(key)) * weigh.inv;
+                emit((int) id, (float) (-z - log((double) total / SM_ONE)), (int) K);
+            }
+            before = after;
+        }
+    };
+
+    // one search: the value T, and how many words at T, at which the count reaches k (by_mass false) or the mass
+    // reaches p of the total (true). Only keys above `over` count; `extra` more mass lies at `over` itself. Returns true
+    // when the row is done (the list held all that can be kept).
+    const float range = fminf(__fadd_rn(xmax, -value_of(mn)), 64.0f);
+    const float scale = range > 0.0f ? __fdiv_rn((float) SM_BINS, range) : 0.0f;
+    auto search = [&](bool by_mass, uint32_t over, u64 extra, bool may_finish, uint32_t &T, unsigned &c) -> bool {
+        uint32_t klo = over + 1, khi = mx;        // keys still in question
+        unsigned above = 0;                        // words, and mass, above khi
+        u64 mass_above = 0, W = 0;
+        double lim = 0.0;
+        int in_bin = -1;                           // level 0's bin the search is in
+        for (int level = 0;; level++) {
+            auto bin0 = [&](uint32_t k) -> int {
+                if (k == mx) return 0;
+                return min(SM_BINS - 1, __float2int_rz(__fmul_rn(__fadd_rn(xmax, -value_of(k)), scale)));
+            };
+            const u64 width = ((u64) khi - klo) / SM_BINS + 1;   // keys per bin from level 1 on
+            auto bin_of = [&](uint32_t k) -> int { return level == 0 ? bin0(k) : (int) ((khi - k) / (uint32_t) width); };
+            for (int b = tid; b < SM_BINS; b += SM_NT) { s.cnt[b] = 0; s.mass[b] = 0; }
+            if (tid == 0) { s.n_list = 0; s.lo = ~0u; s.hi = 0; s.bin = -1; }
+            __syncthreads();
+            for (int o = 0; o < p.seg; o += SM_TILE) {
+                const uint4 q = *(const uint4 *) (mine + o);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t k = (&q.x)[e];
+                    if (k < klo || k > khi || k <= over || (level > 0 && bin0(k) != in_bin)) continue;
+                    const int b = bin_of(k);
+                    atomicAdd(&s.cnt[b], 1u);
+                    if (by_mass) {
+                        const u64 w = weigh(k);
+                        if (w) atomicAdd(&s.mass[b], w);
+                    }
+                }
+            }
+            cl.sync();
+            // every CTA adds up all of them and finds the bin
+            unsigned cn[2] = { 0, 0 };
+            u64 ms[2] = { 0, 0 };
+            for (int r = 0; r < C; r++) {
+                const SampleShared &o = *cl.map_shared_rank(&s, r);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    cn[e] += o.cnt[2 * tid + e];
+                    if (by_mass) ms[e] += o.mass[2 * tid + e];
+                }
+            }
+            unsigned c0 = cn[0] + cn[1], tc;
+            u64 m0 = ms[0] + ms[1], tm;
+            scan2(s, c0, m0, tc, tm);
+            if (by_mass && level == 0) {
+                W = tm + extra;
+                lim = pd * (double) W;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const unsigned ca = above + c0;
+                const u64 ma = mass_above + m0;
+                const bool here = by_mass ? (double) ma < lim && (double) (ma + ms[e]) >= lim && ms[e]
+                                          : ca < (unsigned) top_k && ca + cn[e] >= (unsigned) top_k;
+                if (here) {
+                    s.bin = 2 * tid + e;
+                    s.above = ca;
+                    s.mass_above = ma;
+                    s.in_bin = cn[e];
+                }
+                c0 += cn[e];
+                m0 += ms[e];
+            }
+            __syncthreads();
+            const int bin = s.bin;
+            if (bin < 0) {   // by mass, the border lies among the words at `over`
+                const u64 wt = weigh(over);
+                const double left = lim - (double) (mass_above + tm);
+                T = over;
+                c = wt ? (unsigned) fmax(1.0, ceil(left / (double) wt)) : 0;
+                cl.sync();   // the histograms have been read
+                return false;
+            }
+            above = s.above;
+            mass_above = s.mass_above;
+            const unsigned nb = s.in_bin;
+            const bool all = may_finish && level == 0 && above + nb <= SM_LIST;
+            if (level > 0 && width == 1) {   // one value
+                T = khi - bin;
+                if (by_mass) c = (unsigned) fmax(1.0, ceil((lim - (double) mass_above) / (double) weigh(T)));
+                else c = top_k - above;
+                c = min(c, nb);
+                cl.sync();
+                return false;
+            }
+            // the bin's words (or all down to it) to the leading CTA's list; their range where they are too many
+            const bool fits = all || nb <= SM_LIST;
+            SampleShared &lead = *cl.map_shared_rank(&s, 0);
+            for (int o = 0; o < p.seg; o += SM_TILE) {
+                const uint4 q = *(const uint4 *) (mine + o);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t k = (&q.x)[e];
+                    if (k < klo || k > khi || k <= over || (level > 0 && bin0(k) != in_bin)) continue;
+                    const int b = bin_of(k);
+                    if (!(all ? b <= bin : b == bin)) continue;
+                    if (fits) {
+                        const unsigned at = atomicAdd(&lead.n_list, 1u);
+                        if (at < SM_LIST) lead.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
+                    } else {
+                        atomicMin(&s.lo, k);
+                        atomicMax(&s.hi, k);
+                    }
+                }
+            }
+            cl.sync();
+            if (all) {
+                if (rank == 0) finish_list((int) min(above + nb, (unsigned) SM_LIST), W);
+                return true;
+            }
+            if (fits) {
+                if (rank == 0) {
+                    int n2 = 32;
+                    while (n2 < (int) nb) n2 <<= 1;
+                    for (int i = (int) nb + tid; i < n2; i += SM_NT) s.list[i] = 0;
+                    __syncthreads();
+                    sort_desc(s.list, n2);
+                    u64 wv[2] = { 0, 0 };
+                    unsigned dc = 0, dt;
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        if (by_mass && 2 * tid + e < (int) nb) wv[e] = weigh((uint32_t) (s.list[2 * tid + e] >> 32));
+                    u64 bm = wv[0] + wv[1], bt;
+                    scan2(s, dc, bm, dt, bt);
+                    bm += mass_above;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {   // the last word kept: T is its value, c its place among those of T
+                        const int j = 2 * tid + e;
+                        const bool lastk = by_mass ? j < (int) nb && (double) bm < lim && ((double) (bm + wv[e]) >= lim || j + 1 == (int) nb)
+                                                   : j == top_k - 1 - (int) above;
+                        if (lastk) {
+                            const uint32_t key = (uint32_t) (s.list[j] >> 32);
+                            int f = j;
+                            while (f > 0 && (uint32_t) (s.list[f - 1] >> 32) == key) f--;
+                            s.T = key;
+                            s.c = j - f + 1;
+                        }
+                        bm += wv[e];
+                    }
+                }
+                cl.sync();
+                T = lead.T;
+                c = lead.c;
+                cl.sync();   // read by all before the list is used again
+                return false;
+            }
+            uint32_t lo = ~0u, hi = 0;
+            for (int r = 0; r < C; r++) {
+                const SampleShared &o = *cl.map_shared_rank(&s, r);
+                lo = min(lo, o.lo);
+                hi = max(hi, o.hi);
+            }
+            if (level == 0) in_bin = bin;
+            klo = lo;
+            khi = hi;
+            cl.sync();   // read by all before they are cleared
+        }
+    };
+
+    uint32_t T = 0;          // kept: keys above T, and the first c words at T (T = 0: every valid word)
+    unsigned c = 0;
+    if (use_k && search(false, 0, 0, true, T, c)) { cl.sync(); return; }
+    if (use_p) {
+        const uint32_t over = use_k ? T : 0;
+        const u64 extra = use_k ? c * weigh(T) : 0;
+        uint32_t T2;
+        unsigned c2;
+        if (search(true, over, extra, !use_k, T2, c2)) { cl.sync(); return; }
+        c = T2 == T && use_k ? min(c, c2) : c2;
+        T = T2;
+    }
+    // the kept mass by id: per warp, then over the warps and the cluster
+    u64 sum = 0;
+    unsigned ties = 0, cnt = 0;
+    const u64 wT = T ? weigh(T) : 0;
+    const bool tie_in = T && (!use_m || T == mx || weigh.real(T) >= m);
+    auto take = [&](uint32_t k, u64 &w) -> bool {   // a kept word above T
+        w = 0;
+        if (k <= T) return false;
+        const double r = weigh.real(k);
+        if (use_m && k != mx && r < m) return false;
+        w = Weigher::whole(r);
+        return true;
+    };
+    for (int o = 0; o < p.seg; o += SM_TILE) {
+        const uint4 q = *(const uint4 *) (mine + o);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t k = (&q.x)[e];
+            u64 w;
+            if (take(k, w)) { cnt++; sum += w; }
+            else if (T && k == T) ties++;
+        }
+    }
+    ties = __reduce_add_sync(~0u, ties);
+    cnt = __reduce_add_sync(~0u, cnt);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    // this warp's share in front of the CTA's later warps
+    unsigned tb = lane == 0 ? ties : 0, tt;
+    u64 sb = lane == 0 ? sum : 0, st;
+    scan2(s, tb, sb, tt, st);
+    tb = __shfl_sync(~0u, tb, 0);
+    sb = __shfl_sync(~0u, sb, 0);
+    if (tid == 0) { s.part.cnt = tt; s.part.mass = st; s.nvalid = 0; }
+    __syncthreads();
+    if (lane == 0) atomicAdd(&s.nvalid, cnt);
+    cl.sync();
+    unsigned all_ties = 0, all_cnt = 0;
+    u64 all = 0;
+    for (int r = 0; r < C; r++) {
+        const SampleShared &o = *cl.map_shared_rank(&s, r);
+        if (r < rank) { tb += o.part.cnt; sb += o.part.mass; }
+        all_ties += o.part.cnt;
+        all += o.part.mass;
+        all_cnt += o.nvalid;
+    }
+    const unsigned ct = tie_in ? min(c, all_ties) : 0;
+    const u64 W = all + ct * wT;
+    const int kept = (int) (all_cnt + ct);
+    const double target = (double) u * (double) W;
+    auto mass_at = [&](u64 sum_, unsigned ties_) { return sum_ + min(ties_, ct) * wT; };
+    // the warp whose share the target falls in walks its words
+    if ((double) mass_at(sb, tb) <= target && (double) mass_at(sb + sum, tb + ties) > target) {
+        for (int o = 0; o < p.seg; o += SM_TILE) {
+            u64 w[4], ls = 0;
+            uint32_t k[4];
+            unsigned lt = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                k[e] = mine[o + e];
+                take(k[e], w[e]);
+                ls += w[e];
+                lt += T && k[e] == T;
+            }
+            u64 xs = ls;
+            unsigned xt = lt;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const u64 ys = __shfl_up_sync(~0u, xs, d);
+                const unsigned yt = __shfl_up_sync(~0u, xt, d);
+                if (lane >= d) { xs += ys; xt += yt; }
+            }
+            u64 b = sb + xs - ls;
+            unsigned bt = tb + xt - lt;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const unsigned at = bt + (T && k[e] == T);
+                const u64 after = b + w[e];
+                if ((double) mass_at(b, bt) <= target && (double) mass_at(after, at) > target) {
+                    const double z = k[e] == mx ? 0.0 : ((double) xmax - (double) value_of(k[e])) * weigh.inv;
+                    emit(first + o + e, (float) (-z - log((double) W / SM_ONE)), kept);
+                }
+                b = after;
+                bt = at;
+            }
+            sb += __shfl_sync(~0u, xs, 31);
+            tb += __shfl_sync(~0u, xt, 31);
+        }
+    }
+    cl.sync();
+}
+
+size_t sample_smem(int slice) { return (sizeof(SampleShared) + 15) / 16 * 16 + (size_t) slice * 4; }
+
+}  // namespace
+}  // namespace imi
+
+using namespace imi;
+
+extern "C" imi_cuda_status imi_cuda_sample(int device, const imi_cuda_sample_args *a, void *stream) {
+    if (!a || a->n < 0 || a->vocab < 1) return set_error(IMI_E_ARG, "sample: bad arguments");
+    if (a->vocab > IMI_CUDA_SAMPLE_VOCAB)
+        return set_error(IMI_E_ARG, "sample: at most " + std::to_string(IMI_CUDA_SAMPLE_VOCAB) + " words");
+    if (a->type < IMI_F32 || a->type > IMI_BF16) return set_error(IMI_E_ARG, "sample: bad type");
+    if (a->n == 0) return IMI_OK;
+    if (a->n > 65535) return set_error(IMI_E_ARG, "sample: at most 65535 rows");
+    if (!a->scores || !a->u || !a->ids) return set_error(IMI_E_ARG, "sample: null argument");
+    if (a->stride < a->vocab && a->n > 1) return set_error(IMI_E_ARG, "sample: stride below vocab");
+    if (!aligned(a->scores, a->type == IMI_F32 ? 4 : 2) || !aligned(a->u, 4) || !aligned(a->temperature, 4) || !aligned(a->top_k, 4) ||
+        !aligned(a->top_p, 4) || !aligned(a->min_p, 4) || !aligned(a->ids, 4) || !aligned(a->logprob, 4) || !aligned(a->kept, 4))
+        return set_error(IMI_E_ARG, "sample: a buffer is not aligned to its type");
+    OnDevice on(device);
+    if (!on.ok()) return set_error(IMI_E_NODEV, "no CUDA device " + std::to_string(device));
+    if (!all_on_device({ a->scores, a->u, a->temperature, a->top_k, a->top_p, a->min_p, a->ids, a->logprob, a->kept }, device))
+        return set_error(IMI_E_ARG, "sample: every buffer must be device memory of device " + std::to_string(device));
+    const void *fn = a->type == IMI_F32   ? (const void *) k_sample<float>
+                     : a->type == IMI_F16 ? (const void *) k_sample<__half>
+                                          : (const void *) k_sample<__nv_bfloat16>;
+    static SmemLimit lim;
+    cudaError_t r = lim.raise(device, { (const void *) k_sample<float>, (const void *) k_sample<__half>, (const void *) k_sample<__nv_bfloat16> },
+                              (int) sample_smem(SM_SLICE));
+    // CTAs per row: as many as hold the row, more while the rows leave SMs idle and a CTA keeps a tile per warp
+    int C = 1;
+    while (C < SM_MAX_CLUSTER && ((a->vocab + C - 1) / C > SM_SLICE || (a->n * C < 148 && a->vocab > C * SM_NW * SM_TILE))) C *= 2;
+    SampleArgs p = { *a, 0, 0 };
+    p.seg = ((a->vocab + C * SM_NW - 1) / (C * SM_NW) + SM_TILE - 1) / SM_TILE * SM_TILE;
+    p.slice = p.seg * SM_NW;
+    void *args[] = { &p };
+    if (r == cudaSuccess) r = launch_pdl(fn, dim3(a->n * C), SM_NT, sample_smem(p.slice), (cudaStream_t) stream, args, C);
+    if (r != cudaSuccess) return set_error(IMI_E_CUDA, std::string("sample: ") + cudaGetErrorString(r));
+    return IMI_OK;
+}

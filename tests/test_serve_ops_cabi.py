@@ -1,0 +1,88 @@
+"""The serving operators' refusals on the host: every bad argument is IMI_E_ARG with a message before any device work, and
+good ones without a device are IMI_E_NODEV. No GPU needed (the pointers are never followed)."""
+import ctypes as C
+
+import pytest
+
+import nunchi_b200 as nb
+
+P = 0x10000   # an aligned address that is never read
+
+
+def call(name, cls, good, **bad):
+    a = cls(**{**good, **bad})
+    st = getattr(nb.lib(), name)(0, C.addressof(a), None)
+    return st, nb.lib().imi_cuda_error().decode()
+
+
+MAP = dict(held=P, add=P, n=4, table=P, table_stride=8, width=8, free_pages=P, free_cap=9, n_free=P, page=16, n_pages=40, pos0=0, cap=12,
+           start=P, length=P, slots=P, pos=P, n_free_out=P, status=P)
+WRITE = dict(k=P, v=P, type=0, row_stride=512, head_stride=64, rows=5, slots=P, n_head_kv=8, head_dim=64, k_pages=P, v_pages=P, page_type=1,
+             page=64, n_pages=9, status=None)
+ATTN = dict(q=P, type=1, q_stride=2048, rows=4, n_head=32, n_head_kv=8, head_dim=64, k_pages=P, v_pages=P, page=64, n_pages=50, prefix=P,
+            prefix_len=1000, table=P, table_stride=9, width=9, length=P, scale=0.125, window=0, out=P, out_type=1, out_stride=2048, lse=P,
+            work=P, work_bytes=1 << 30, status=P)
+SAMPLE = dict(scores=P, type=0, stride=1000, n=3, vocab=1000, u=P, temperature=P, top_k=P, top_p=P, min_p=P, ids=P, logprob=P, kept=P)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(n=0), dict(n=4097), dict(held=None), dict(add=None), dict(table=None), dict(n_free=None), dict(start=None), dict(length=None),
+    dict(n_free_out=None), dict(status=None), dict(slots=None), dict(pos=None), dict(page=0), dict(page=24), dict(page=8), dict(page=512),
+    dict(n_pages=0), dict(n_pages=1 << 28), dict(width=0), dict(table_stride=7), dict(cap=-1), dict(free_cap=-1), dict(free_pages=None),
+    dict(pos0=-1), dict(pos0=2 ** 31 - 10), dict(held=P + 2), dict(status=P + 1)])
+def test_page_map_refuses(bad):
+    st, msg = call("imi_cuda_page_map", nb._PageMapArgs, MAP, **bad)
+    assert st == 1 and "page_map" in msg
+
+
+@pytest.mark.parametrize("bad", [
+    dict(rows=-1), dict(page_type=0), dict(page_type=3), dict(type=2), dict(type=-1), dict(n_head_kv=0), dict(head_dim=60), dict(head_dim=0),
+    dict(head_dim=264), dict(page=48), dict(n_pages=0), dict(k=None), dict(v=None), dict(slots=None), dict(k_pages=None), dict(v_pages=None),
+    dict(row_stride=-1), dict(head_stride=-1), dict(k=P + 2), dict(k_pages=P + 8), dict(slots=P + 2)])
+def test_page_write_refuses(bad):
+    st, msg = call("imi_cuda_page_write", nb._PageWriteArgs, WRITE, **bad)
+    assert st == 1 and "page_write" in msg
+
+
+@pytest.mark.parametrize("bad", [
+    dict(type=0), dict(type=3), dict(out_type=3), dict(out_type=-1), dict(rows=-1), dict(rows=4097), dict(n_head=33), dict(n_head=0),
+    dict(n_head_kv=0), dict(n_head=17 * 8), dict(head_dim=96), dict(prefix_len=-1), dict(width=-1), dict(page=100), dict(window=-1),
+    dict(n_pages=-1), dict(n_pages=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=None), dict(length=None),
+    dict(work=None), dict(prefix=None), dict(table=None), dict(k_pages=None), dict(v_pages=None), dict(table_stride=8), dict(q_stride=2040),
+    dict(q_stride=2052), dict(out_stride=2040), dict(out_stride=2050), dict(q=P + 8), dict(k_pages=P + 2), dict(out=P + 4), dict(work=P + 8),
+    dict(lse=P + 2), dict(work_bytes=100), dict(prefix_len=2 ** 31 - 1)])
+def test_prefix_attn_refuses(bad):
+    st, msg = call("imi_cuda_prefix_attn", nb._PrefixAttnArgs, ATTN, **bad)
+    assert st == 1 and "prefix_attn" in msg
+
+
+def test_prefix_attn_work():
+    w = nb.lib().imi_cuda_prefix_attn_work
+    assert w(64, 32, 8, 64, 1000, 20, 64) > 0 and w(0, 32, 8, 64, 0, 0, 16) > 0
+    for bad in ((-1, 32, 8, 64, 0, 1, 16), (1, 31, 8, 64, 0, 1, 16), (1, 32, 8, 80, 0, 1, 16), (1, 32, 8, 64, -1, 1, 16), (1, 32, 8, 64, 0, 1, 17)):
+        assert w(*bad) == 0
+    # the workspace of the largest batch serves every smaller one of the same heads
+    for prefix in (0, 1, 100, 5000, 100000):
+        sizes = [w(r, 32, 8, 64, prefix, 20, 64) for r in range(0, 300)]
+        assert all(x <= sizes[-1] for x in sizes)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(n=-1), dict(n=65536), dict(vocab=0), dict(vocab=262145, stride=300000), dict(type=3), dict(scores=None), dict(u=None), dict(ids=None),
+    dict(stride=999), dict(scores=P + 2), dict(top_k=P + 1), dict(kept=P + 2)])
+def test_sample_refuses(bad):
+    st, msg = call("imi_cuda_sample", nb._SampleArgs, SAMPLE, **bad)
+    assert st == 1 and "sample" in msg
+
+
+def test_null_argument_blocks():
+    for f in ("page_map", "page_write", "prefix_attn", "sample"):
+        assert getattr(nb.lib(), "imi_cuda_" + f)(0, None, None) == 1
+
+
+def test_no_such_device():
+    for name, cls, good in (("imi_cuda_page_map", nb._PageMapArgs, MAP), ("imi_cuda_page_write", nb._PageWriteArgs, WRITE),
+                            ("imi_cuda_prefix_attn", nb._PrefixAttnArgs, ATTN), ("imi_cuda_sample", nb._SampleArgs, SAMPLE)):
+        a = cls(**good)
+        for device in (-1, 4096):
+            assert getattr(nb.lib(), name)(device, C.addressof(a), None) == 8
