@@ -8,9 +8,14 @@
 // exp and the borders are computed in 64 bits: a border is missed only where two candidates differ by about 2^-44.
 //
 // A row is held in the shared memory of a cluster of 1 to 8 CTAs, as integer keys that order like the scores: it is
-// read from HBM once, and every later pass is over shared memory. A word of T is found by a histogram over 1,024
-// steps of score (counts, and masses for top-p), whose crossing bin, or everything down to it when that is few words,
-// is gathered and sorted by one CTA; a bin too full for that (masked words, all scores alike) is cut again, by keys.
+// read from HBM once, and every later pass is over shared memory.
+//   The short way: while loading, every thread keeps its own words' maximum. The r-th largest of a CTA's thread maxima is
+// a value that r of its words reach, so the smallest of these over the cluster, with r = ceil(k / CTAs), is one that k
+// words reach; for top-p alone r is set for about 500 words, for min-p alone the value follows from the maximum. The few
+// words above it are listed, and one CTA sorts them and applies the filters. Top-p's total mass is summed meanwhile.
+//   The long way, where the list would be too long or ends inside the nucleus: a histogram over 1,024 steps of score
+// (counts, masses), whose crossing bin is sorted by one CTA; a bin too full for that (masked words, all scores alike) is
+// cut again, by keys. Then every CTA sums its kept words by id.
 #include "common.cuh"
 #include "serve.h"
 
@@ -26,12 +31,14 @@ namespace {
 
 constexpr int SM_NT = 512, SM_NW = SM_NT / 32;
 constexpr int SM_BINS = 2 * SM_NT;       // two bins per thread in the scans
-constexpr int SM_LIST = 1024;            // words the leading CTA sorts at most
+constexpr int SM_LIST = 1024;            // words one CTA sorts at most
+constexpr int SM_AIM = 512;              // words listed for top-p alone, about
 constexpr int SM_TILE = 128;             // words of a warp's load: four per lane
 constexpr int SM_MAX_CLUSTER = 8;
 constexpr int SM_SLICE = 32768;          // words a CTA holds at most
 constexpr double SM_ONE = 17592186044416.0;   // 2^44
 constexpr double SM_FAR = 31.2;          // exp(-31.2) < 2^-45: such a word's weight rounds to 0
+constexpr int SM_TAB = 64;               // steps of the exponential's table
 static_assert((long long) SM_SLICE * SM_MAX_CLUSTER >= IMI_CUDA_SAMPLE_VOCAB, "a row fits a cluster");
 static_assert((long long) IMI_CUDA_SAMPLE_VOCAB <= 1 << 18, "the weights' sum fits 62 bits");
 
@@ -53,25 +60,25 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-struct Totals {
-    unsigned cnt;
-    u64 mass;
-};
-
 struct SampleShared {
-    unsigned cnt[SM_BINS];        // this CTA's histogram
-    u64 mass[SM_BINS];
-    u64 list[SM_LIST];            // leading CTA: (key, ~id) gathered; then sorted
-    u64 w[SM_LIST];
-    unsigned wc[SM_NW];           // scans over the CTA
+    union {
+        struct {
+            unsigned cnt[SM_BINS], mass[SM_BINS][2];   // this CTA's histogram; mass: low and high words
+        };
+        struct {
+            u64 list[SM_LIST], w[SM_LIST];   // (key, ~id) listed; weights in the list's order
+        };
+    };
+    double tab[SM_TAB];               // 2^(i / 64)
+    unsigned wc[SM_NW];               // scans over the CTA
     u64 wm[SM_NW];
-    unsigned mx, mn, nvalid, idmin;   // what the cluster reads of this CTA
-    unsigned n_list, lo, hi;
-    Totals part;
-    int bin;                      // found in a scan: the crossing bin, and what lies above it
-    unsigned above, in_bin;
+    // what the cluster reads of this CTA
+    u64 part_mass;
+    unsigned part_cnt, part_kept, mx, mn, nvalid, floor, idmin, n_list, lo, hi;
     u64 mass_above;
-    unsigned T, c;                // the leading CTA's findings
+    int bin;                          // found in a scan: the crossing bin, and what lies above it
+    unsigned above, in_bin;
+    unsigned T, c, done;              // the leading CTA's findings
 };
 
 // exclusive sums over the CTA's threads, and the totals
@@ -102,28 +109,63 @@ __device__ __forceinline__ void scan2(SampleShared &s, unsigned &c, u64 &m, unsi
     m = bm + xm - m;
 }
 
-// a word's weight, as a number and as an integer of 2^-44
+// A word's weight, as a number and as an integer of 2^-44. exp by table (Tang, ACM TOMS 15, 1989): with n the nearest
+// integer to z 64 / ln 2, exp(-z) = 2^(-n / 64) exp(r), r = n ln2 / 64 - z, |r| <= ln2 / 128, exp(r) to r^5 / 120 (the next
+// term is below 2^-54). n reaches 2,881 here, so the rounding of ln2 / 64 costs 2^-48 of a weight that is itself 2^-45 then.
 struct Weigher {
     float xmax;
     uint32_t kmax;
     double inv;   // 1 / temperature
+    const double *tab;
     __device__ __forceinline__ double real(uint32_t k) const {
         if (k == kmax) return 1.0;
         const double z = ((double) xmax - (double) value_of(k)) * inv;
-        return z < SM_FAR ? exp(-z) : 0.0;
+        if (!(z < SM_FAR)) return 0.0;
+        constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: adding it leaves the nearest integer in the low bits
+        const double b = __fma_rn(z, -64.0 * 1.4426950408889634074, MAGIC);
+        const int n = __double2loint(b);               // <= 0
+        const double r = __fma_rn(__dadd_rn(b, -MAGIC), -0.69314718055994530942 / 64.0, -z);
+        double e = __fma_rn(r, 1.0 / 120.0, 1.0 / 24.0);
+        e = __fma_rn(r, e, 1.0 / 6.0);
+        e = __fma_rn(r, e, 0.5);
+        e = __fma_rn(r, e, 1.0);
+        e = __fma_rn(r, e, 1.0);
+        e = __dmul_rn(e, tab[n & (SM_TAB - 1)]);
+        return __hiloint2double(__double2hiint(e) + (n >> 6) * (1 << 20), __double2loint(e));
     }
     static __device__ __forceinline__ u64 whole(double w) {
         // w * 2^44 <= 2^44: added to 2^52 its integer part, rounded to nearest, is the low mantissa
         return (u64) __double_as_longlong(__fma_rn(w, SM_ONE, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
     }
     __device__ __forceinline__ u64 operator()(uint32_t k) const { return whole(real(k)); }
+    __device__ __forceinline__ float logprob(uint32_t k, u64 total) const {
+        const double z = k == kmax ? 0.0 : ((double) xmax - (double) value_of(k)) * inv;
+        return (float) (-z - log((double) total / SM_ONE));
+    }
 };
 
-// sorted descending, n a power of two of at most SM_LIST
+// v[0..n) sorted descending (all different, n at most SM_LIST, room up to the next power of two)
 __device__ __forceinline__ void sort_desc(u64 *v, int n) {
-    for (int k = 2; k <= n; k <<= 1)
+    const int tid = threadIdx.x;
+    if (n <= 256) {   // each value's place counted: a pass over n values, against 36 exchanges with a barrier each
+        u64 x = 0;
+        int place = 0;
+        if (tid < n) {
+            x = v[tid];
+            for (int j = 0; j < n; j++) place += v[j] > x;
+        }
+        __syncthreads();
+        if (tid < n) v[place] = x;
+        __syncthreads();
+        return;
+    }
+    int n2 = 512;
+    while (n2 < n) n2 <<= 1;
+    for (int i = n + tid; i < n2; i += SM_NT) v[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= n2; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = threadIdx.x; i < n / 2; i += SM_NT) {
+            for (int i = tid; i < n2 / 2; i += SM_NT) {
                 const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
                 const u64 x = v[lo], y = v[hi];
                 if ((x < y) == ((lo & k) == 0)) { v[lo] = y; v[hi] = x; }
@@ -133,7 +175,14 @@ __device__ __forceinline__ void sort_desc(u64 *v, int n) {
 }
 
 template <typename S>
-__global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ SampleArgs p) {
+__device__ __forceinline__ float score_at(const S *x, int i) {
+    if constexpr (sizeof(S) == 4) return x[i];
+    else if constexpr (std::is_same<S, __half>::value) return __half2float(x[i]);
+    else return __bfloat162float(x[i]);
+}
+
+template <typename S>
+__global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ SampleArgs p) {
     extern __shared__ __align__(16) uint8_t sm_raw[];
     SampleShared &s = *(SampleShared *) sm_raw;
     uint32_t *keys = (uint32_t *) (sm_raw + (sizeof(SampleShared) + 15) / 16 * 16);
@@ -142,7 +191,8 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
     const int C = (int) cl.num_blocks(), rank = (int) cl.block_rank();
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int base = rank * p.slice;                       // this CTA's first word
-    if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = 0; }
+    if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = 0; s.floor = 1; }
+    if (tid < SM_TAB) s.tab[tid] = exp2((double) tid / SM_TAB);
     __syncthreads();
     pdl_wait();
     pdl_trigger();
@@ -153,19 +203,16 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
     u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;          // NaN: 0
     const bool greedy = !(temp > 0.0f);
     if (top_p <= 0.0f) top_k = 1;                           // the first word alone
+    const bool use_k = top_k > 0 && top_k < a.vocab, use_p = top_p > 0.0f && top_p < 1.0f, use_m = min_p > 0.0f;
+    const double m = fmin((double) min_p, 1.0), pd = (double) top_p;
 
-    // 1: the row as keys; the largest, the smallest, how many
+    // the row as keys; the largest
     const S *x = (const S *) a.scores + row * a.stride;
     const bool vec = ((uintptr_t) (x + base) & (4 * sizeof(S) - 1)) == 0;
-    uint32_t mx = 0, mn = ~0u;
-    unsigned nv = 0;
+    uint32_t mx = 0;
     uint32_t *mine = keys + warp * p.seg + 4 * lane;        // the words of a lane, tile by tile
     const int first = base + warp * p.seg + 4 * lane;
-    auto load = [&](int i) -> float {
-        if constexpr (sizeof(S) == 4) return x[i];
-        else if constexpr (std::is_same<S, __half>::value) return __half2float(x[i]);
-        else return __bfloat162float(x[i]);
-    };
+#pragma unroll 4
     for (int o = 0; o < p.seg; o += SM_TILE) {
         const int i = first + o;
         float f[4];
@@ -177,42 +224,45 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
                 const uint2 v = __ldg((const uint2 *) (x + i));
                 const S *h = (const S *) &v;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if constexpr (std::is_same<S, __half>::value) f[e] = __half2float(h[e]);
-                    else f[e] = __bfloat162float(h[e]);
-                }
+                for (int e = 0; e < 4; e++) f[e] = score_at(h, e);
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) f[e] = i + e < a.vocab ? load(i + e) : -INFINITY;
+            for (int e = 0; e < 4; e++) f[e] = i + e < a.vocab ? score_at(x, i + e) : -INFINITY;
         }
         uint32_t k[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             k[e] = key_of(f[e]);
             mx = max(mx, k[e]);
-            if (k[e]) { mn = min(mn, k[e]); nv++; }
         }
         *(uint4 *) (mine + o) = make_uint4(k[0], k[1], k[2], k[3]);
     }
-    mx = __reduce_max_sync(~0u, mx);
-    mn = __reduce_min_sync(~0u, mn);
-    nv = __reduce_add_sync(~0u, nv);
-    if (lane == 0) { atomicMax(&s.mx, mx); atomicMin(&s.mn, mn); atomicAdd(&s.nvalid, nv); }
+    // the r-th largest of the threads' maxima, to 20 bits downwards
+    const bool by_k = use_k && top_k <= SM_LIST, by_p = !use_k && use_p, by_m = !use_k && !use_p && use_m;
+    const int r_th = by_k ? (top_k + C - 1) / C : by_p ? SM_AIM / C : 0;
+    const bool lists = !greedy && r_th <= SM_NT && (by_k || by_p || by_m);
+    uint32_t floor = 0;
+    if (lists && r_th)
+        for (int b = 31; b >= 12; b--)
+            if (__syncthreads_count(mx >= (floor | 1u << b)) >= r_th) floor |= 1u << b;
+    const uint32_t wmax = __reduce_max_sync(~0u, mx);
+    if (lane == 0) atomicMax(&s.mx, wmax);
+    if (tid == 0) s.floor = max(floor, 1u);
     cl.sync();
-    mx = 0; mn = ~0u; nv = 0;
+    mx = 0;
+    floor = ~0u;
     for (int r = 0; r < C; r++) {
         const SampleShared &o = *cl.map_shared_rank(&s, r);
         mx = max(mx, o.mx);
-        mn = min(mn, o.mn);
-        nv += o.nvalid;
+        floor = min(floor, o.floor);
     }
     auto emit = [&](int id, float lp, int kept) {
         a.ids[row] = id;
         if (a.logprob) a.logprob[row] = lp;
         if (a.kept) a.kept[row] = kept;
     };
-    if (nv == 0) {
+    if (mx == 0) {
         if (rank == 0 && tid == 0) emit(-1, -INFINITY, 0);
         cl.sync();   // no CTA leaves while another may read its shared memory
         return;
@@ -220,10 +270,11 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
     const float xmax = value_of(mx);
     if (greedy) {
         unsigned id = ~0u;
-        for (int o = 0; o < p.seg; o += SM_TILE)
+        if (wmax == mx)
+            for (int o = 0; o < p.seg; o += SM_TILE)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (mine[o + e] == mx) id = min(id, (unsigned) (first + o + e));
+                for (int e = 0; e < 4; e++)
+                    if (mine[o + e] == mx) id = min(id, (unsigned) (first + o + e));
         id = __reduce_min_sync(~0u, id);
         if (lane == 0) atomicMin(&s.idmin, id);
         cl.sync();
@@ -234,18 +285,13 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
         cl.sync();
         return;
     }
-    const Weigher weigh = { xmax, mx, 1.0 / (double) temp };
-    const bool use_k = top_k > 0 && (unsigned) top_k < nv, use_p = top_p > 0.0f && top_p < 1.0f, use_m = min_p > 0.0f;
-    const double m = fmin((double) min_p, 1.0), pd = (double) top_p;
+    const Weigher weigh = { xmax, mx, 1.0 / (double) temp, s.tab };
 
-    // the leading CTA's list of n words holds all that can be kept: the filters, and the pick by id. total_all: the mass
-    // that top-p's share is of where top-k does not cut the list
-    auto finish_list = [&](int n, u64 total_all) {
-        int n2 = 32;
-        while (n2 < n) n2 <<= 1;
-        for (int i = n + tid; i < n2; i += SM_NT) s.list[i] = 0;
-        __syncthreads();
-        sort_desc(s.list, n2);
+    // The list of n words, which reaches down to some value, ends the row if all that can be kept is in it: the filters, and
+    // the pick by id. of_all: the mass that top-p's share is of where top-k does not cut the list. False: the nucleus goes on
+    // below the list.
+    auto finish_list = [&](int n, u64 of_all) -> bool {
+        sort_desc(s.list, n);
         if (use_k) n = min(n, top_k);
         // two words per thread: weights, their sums, and how many pass
         u64 wv[2], sum = 0;
@@ -262,34 +308,47 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
         unsigned ex = pass, tp;
         u64 before = sum, total;
         scan2(s, ex, before, tp, total);
-        const u64 of = use_k ? total : total_all;
-        const double lim = pd * (double) of;
-        unsigned keep = 0;
+        int K = (int) tp;
+        if (use_p) {
+            const double lim = pd * (double) (use_k ? total : of_all);
+            if (!use_k && (double) total < lim) return false;
+            unsigned keep = 0, all;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int j = 2 * tid + e;
-            if (j < n && (!use_p || j == 0 || (double) before < lim)) keep++;
-            before += wv[e];
-        }
-        unsigned K;
-        u64 dm = 0, dt;
-        scan2(s, keep, dm, K, dt);
-        K = min(K, tp);
-        // by id: (~id, place in the order of scores) sorted descending; the keys move to the histogram's memory
-        n2 = 32;
-        while (n2 < (int) K) n2 <<= 1;
-        for (int j = tid; j < n2; j += SM_NT) {
-            const u64 q = s.list[j];
-            s.cnt[j] = (unsigned) (q >> 32);
-            s.list[j] = j < (int) K ? q << 32 | (unsigned) j : 0;
+            for (int e = 0; e < 2; e++) {
+                const int j = 2 * tid + e;
+                if (j < n && (j == 0 || (double) before < lim)) keep++;
+                before += wv[e];
+            }
+            u64 d0 = 0, d1;
+            scan2(s, keep, d0, all, d1);
+            K = min(K, (int) all);
         }
         __syncthreads();
-        sort_desc(s.list, n2);
+        if (K <= 128) {   // each word's running sum by id counted directly
+            u64 b = 0, t = 0, q = 0, w = 0;
+            if (tid < K) {
+                q = s.list[tid];
+                w = s.w[tid];
+                for (int j = 0; j < K; j++) {
+                    const u64 wj = s.w[j];
+                    t += wj;
+                    if ((unsigned) s.list[j] > (unsigned) q) b += wj;   // ~id larger: id smaller
+                }
+                const double target = (double) u * (double) t;
+                if ((double) b <= target && (double) (b + w) > target)
+                    emit((int) ~(unsigned) q, weigh.logprob((uint32_t) (q >> 32), t), K);
+            }
+            return true;
+        }
+        // by id: (~id, place in the order of scores) sorted descending
+        for (int j = tid; j < K; j += SM_NT) s.list[j] = s.list[j] << 32 | (unsigned) j;
+        __syncthreads();
+        sort_desc(s.list, K);
         sum = 0;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const int j = 2 * tid + e;
-            wv[e] = j < (int) K ? s.w[(unsigned) s.list[j]] : 0;
+            wv[e] = j < K ? s.w[(unsigned) s.list[j]] : 0;
             sum += wv[e];
         }
         unsigned d0 = 0, d1;
@@ -300,25 +359,109 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
         for (int e = 0; e < 2; e++) {
             const int j = 2 * tid + e;
             const u64 after = before + wv[e];
-            if (j < (int) K && (double) before <= target && (double) after > target) {
-                const uint32_t key = s.cnt[(unsigned) s.list[j]];
-                const unsigned id = ~(unsigned) (s.list[j] >> 32);
-                const double z = key == mx ? 0.0 : ((double) xmax - (double) value_of(key)) * weigh.inv;
-                emit((int) id, (float) (-z - log((double) total / SM_ONE)), (int) K);
+            if (j < K && (double) before <= target && (double) after > target) {
+                const int id = (int) ~(unsigned) (s.list[j] >> 32);
+                emit(id, weigh.logprob(key_of(score_at(x, id)), total), K);
             }
             before = after;
         }
+        return true;
     };
 
-    // one search: the value T, and how many words at T, at which the count reaches k (by_mass false) or the mass
-    // reaches p of the total (true). Only keys above `over` count; `extra` more mass lies at `over` itself. Returns true
-    // when the row is done (the list held all that can be kept).
+    u64 W0 = 0;              // the row's whole mass, where the short way has summed it
+    if (lists) {
+        if (by_m) {          // what w >= m can reach, downwards by more than the roundings on the way
+            const double lo = (double) xmax + (double) temp * log(m);
+            floor = max(key_of((float) (lo - 1e-6 * (fabs(lo) + fabs((double) xmax) + (double) temp))), 1u);
+        }
+        u64 sum = 0;
+        for (int o = 0; o < p.seg; o += SM_TILE) {
+            const uint4 q = *(const uint4 *) (mine + o);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t k = (&q.x)[e];
+                if (k >= floor) {
+                    const unsigned at = atomicAdd(&s.n_list, 1u);
+                    if (at < SM_LIST) s.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
+                }
+                if (by_p && k) sum += weigh(k);
+            }
+        }
+        if (by_p) {
+            unsigned d0 = 0, d1;
+            u64 t;
+            scan2(s, d0, sum, d1, t);
+            if (tid == 0) s.part_mass = t;
+        }
+        cl.sync();
+        unsigned n = 0;
+        for (int r = 0; r < C; r++) {
+            const SampleShared &o = *cl.map_shared_rank(&s, r);
+            n += o.n_list;
+            if (by_p) W0 += o.part_mass;
+        }
+        if (n <= SM_LIST) {
+            if (rank == 0) {
+                unsigned at = s.n_list;
+                for (int r = 1; r < C; r++) {
+                    const SampleShared &o = *cl.map_shared_rank(&s, r);
+                    const unsigned c = o.n_list;
+                    for (unsigned i = tid; i < c; i += SM_NT) s.list[at + i] = o.list[i];
+                    at += c;
+                }
+                __syncthreads();
+            }
+            if (!by_p) {
+                cl.sync();   // the lists have been read
+                if (rank == 0) finish_list((int) n, 0);
+                return;
+            }
+            if (rank == 0) {
+                const bool ok = finish_list((int) n, W0);
+                if (tid == 0) s.done = ok;
+            }
+            cl.sync();
+            if (cl.map_shared_rank(&s, 0)->done) {
+                cl.sync();
+                return;
+            }
+        }
+        cl.sync();
+    }
+
+    // ---- the long way ----
+    // the smallest key, and how many there are
+    {
+        uint32_t mn = ~0u;
+        unsigned nv = 0;
+        for (int o = 0; o < p.seg; o += SM_TILE) {
+            const uint4 q = *(const uint4 *) (mine + o);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t k = (&q.x)[e];
+                if (k) { mn = min(mn, k); nv++; }
+            }
+        }
+        mn = __reduce_min_sync(~0u, mn);
+        nv = __reduce_add_sync(~0u, nv);
+        if (lane == 0) { atomicMin(&s.mn, mn); atomicAdd(&s.nvalid, nv); }
+    }
+    cl.sync();
+    uint32_t mn = ~0u;
+    unsigned nv = 0;
+    for (int r = 0; r < C; r++) {
+        const SampleShared &o = *cl.map_shared_rank(&s, r);
+        mn = min(mn, o.mn);
+        nv += o.nvalid;
+    }
+    // One search: the value T, and how many words c at T, at which the count reaches k (by_mass false) or the mass
+    // reaches p of the total (true). Only keys above `over` count; `extra` more mass lies at `over` itself.
     const float range = fminf(__fadd_rn(xmax, -value_of(mn)), 64.0f);
     const float scale = range > 0.0f ? __fdiv_rn((float) SM_BINS, range) : 0.0f;
-    auto search = [&](bool by_mass, uint32_t over, u64 extra, bool may_finish, uint32_t &T, unsigned &c) -> bool {
+    auto search = [&](bool by_mass, uint32_t over, u64 extra, uint32_t &T, unsigned &c) {
         uint32_t klo = over + 1, khi = mx;        // keys still in question
         unsigned above = 0;                        // words, and mass, above khi
-        u64 mass_above = 0, W = 0;
+        u64 mass_above = 0;
         double lim = 0.0;
         int in_bin = -1;                           // level 0's bin the search is in
         for (int level = 0;; level++) {
@@ -327,21 +470,27 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
                 return min(SM_BINS - 1, __float2int_rz(__fmul_rn(__fadd_rn(xmax, -value_of(k)), scale)));
             };
             const u64 width = ((u64) khi - klo) / SM_BINS + 1;   // keys per bin from level 1 on
-            auto bin_of = [&](uint32_t k) -> int { return level == 0 ? bin0(k) : (int) ((khi - k) / (uint32_t) width); };
-            for (int b = tid; b < SM_BINS; b += SM_NT) { s.cnt[b] = 0; s.mass[b] = 0; }
-            if (tid == 0) { s.n_list = 0; s.lo = ~0u; s.hi = 0; s.bin = -1; }
+            auto bin_of = [&](uint32_t k) -> int {               // -1: not in question
+                if (k < klo || k > khi) return -1;
+                if (level == 0) return bin0(k);
+                return bin0(k) == in_bin ? (int) ((khi - k) / (uint32_t) width) : -1;
+            };
+            for (int b = tid; b < SM_BINS; b += SM_NT) s.cnt[b] = s.mass[b][0] = s.mass[b][1] = 0;
+            if (tid == 0) { s.bin = -1; s.lo = ~0u; s.hi = 0; s.n_list = 0; }
             __syncthreads();
             for (int o = 0; o < p.seg; o += SM_TILE) {
                 const uint4 q = *(const uint4 *) (mine + o);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t k = (&q.x)[e];
-                    if (k < klo || k > khi || k <= over || (level > 0 && bin0(k) != in_bin)) continue;
                     const int b = bin_of(k);
+                    if (b < 0) continue;
                     atomicAdd(&s.cnt[b], 1u);
-                    if (by_mass) {
+                    if (by_mass) {   // 64-bit addition by halves: the carry is what the low half's old value shows
                         const u64 w = weigh(k);
-                        if (w) atomicAdd(&s.mass[b], w);
+                        const unsigned wl = (unsigned) w, old = atomicAdd(&s.mass[b][0], wl);
+                        const unsigned wh = (unsigned) (w >> 32) + (old + wl < old);
+                        if (wh) atomicAdd(&s.mass[b][1], wh);
                     }
                 }
             }
@@ -354,16 +503,13 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     cn[e] += o.cnt[2 * tid + e];
-                    if (by_mass) ms[e] += o.mass[2 * tid + e];
+                    if (by_mass) ms[e] += (u64) o.mass[2 * tid + e][1] << 32 | o.mass[2 * tid + e][0];
                 }
             }
             unsigned c0 = cn[0] + cn[1], tc;
             u64 m0 = ms[0] + ms[1], tm;
             scan2(s, c0, m0, tc, tm);
-            if (by_mass && level == 0) {
-                W = tm + extra;
-                lim = pd * (double) W;
-            }
+            if (by_mass && level == 0) lim = pd * (double) (tm + extra);
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const unsigned ca = above + c0;
@@ -379,42 +525,37 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
                 c0 += cn[e];
                 m0 += ms[e];
             }
-            __syncthreads();
+            cl.sync();   // every CTA has read the histograms (whose memory the lists share) and knows the bin
             const int bin = s.bin;
             if (bin < 0) {   // by mass, the border lies among the words at `over`
                 const u64 wt = weigh(over);
-                const double left = lim - (double) (mass_above + tm);
                 T = over;
-                c = wt ? (unsigned) fmax(1.0, ceil(left / (double) wt)) : 0;
-                cl.sync();   // the histograms have been read
-                return false;
+                c = wt ? (unsigned) fmax(1.0, ceil((lim - (double) (mass_above + tm)) / (double) wt)) : 0;
+                cl.sync();   // read by all before it is written again (here and below)
+                return;
             }
             above = s.above;
             mass_above = s.mass_above;
             const unsigned nb = s.in_bin;
-            const bool all = may_finish && level == 0 && above + nb <= SM_LIST;
             if (level > 0 && width == 1) {   // one value
                 T = khi - bin;
                 if (by_mass) c = (unsigned) fmax(1.0, ceil((lim - (double) mass_above) / (double) weigh(T)));
                 else c = top_k - above;
                 c = min(c, nb);
                 cl.sync();
-                return false;
+                return;
             }
-            // the bin's words (or all down to it) to the leading CTA's list; their range where they are too many
-            const bool fits = all || nb <= SM_LIST;
-            SampleShared &lead = *cl.map_shared_rank(&s, 0);
+            // the bin's words to a list; their range where they are too many
+            const bool fits = nb <= SM_LIST;
             for (int o = 0; o < p.seg; o += SM_TILE) {
                 const uint4 q = *(const uint4 *) (mine + o);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t k = (&q.x)[e];
-                    if (k < klo || k > khi || k <= over || (level > 0 && bin0(k) != in_bin)) continue;
-                    const int b = bin_of(k);
-                    if (!(all ? b <= bin : b == bin)) continue;
+                    if (bin_of(k) != bin) continue;
                     if (fits) {
-                        const unsigned at = atomicAdd(&lead.n_list, 1u);
-                        if (at < SM_LIST) lead.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
+                        const unsigned at = atomicAdd(&s.n_list, 1u);
+                        if (at < SM_LIST) s.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
                     } else {
                         atomicMin(&s.lo, k);
                         atomicMax(&s.hi, k);
@@ -422,29 +563,29 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
                 }
             }
             cl.sync();
-            if (all) {
-                if (rank == 0) finish_list((int) min(above + nb, (unsigned) SM_LIST), W);
-                return true;
-            }
             if (fits) {
                 if (rank == 0) {
-                    int n2 = 32;
-                    while (n2 < (int) nb) n2 <<= 1;
-                    for (int i = (int) nb + tid; i < n2; i += SM_NT) s.list[i] = 0;
+                    unsigned n = s.n_list;
+                    for (int r = 1; r < C; r++) {
+                        const SampleShared &o = *cl.map_shared_rank(&s, r);
+                        const unsigned oc = o.n_list;
+                        for (unsigned i = tid; i < oc; i += SM_NT) s.list[n + i] = o.list[i];
+                        n += oc;
+                    }
                     __syncthreads();
-                    sort_desc(s.list, n2);
+                    sort_desc(s.list, (int) n);
                     u64 wv[2] = { 0, 0 };
                     unsigned dc = 0, dt;
 #pragma unroll
                     for (int e = 0; e < 2; e++)
-                        if (by_mass && 2 * tid + e < (int) nb) wv[e] = weigh((uint32_t) (s.list[2 * tid + e] >> 32));
+                        if (by_mass && 2 * tid + e < (int) n) wv[e] = weigh((uint32_t) (s.list[2 * tid + e] >> 32));
                     u64 bm = wv[0] + wv[1], bt;
                     scan2(s, dc, bm, dt, bt);
                     bm += mass_above;
 #pragma unroll
                     for (int e = 0; e < 2; e++) {   // the last word kept: T is its value, c its place among those of T
                         const int j = 2 * tid + e;
-                        const bool lastk = by_mass ? j < (int) nb && (double) bm < lim && ((double) (bm + wv[e]) >= lim || j + 1 == (int) nb)
+                        const bool lastk = by_mass ? j < (int) n && (double) bm < lim && ((double) (bm + wv[e]) >= lim || j + 1 == (int) n)
                                                    : j == top_k - 1 - (int) above;
                         if (lastk) {
                             const uint32_t key = (uint32_t) (s.list[j] >> 32);
@@ -457,10 +598,11 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
                     }
                 }
                 cl.sync();
+                const SampleShared &lead = *cl.map_shared_rank(&s, 0);
                 T = lead.T;
                 c = lead.c;
-                cl.sync();   // read by all before the list is used again
-                return false;
+                cl.sync();
+                return;
             }
             uint32_t lo = ~0u, hi = 0;
             for (int r = 0; r < C; r++) {
@@ -477,14 +619,15 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
 
     uint32_t T = 0;          // kept: keys above T, and the first c words at T (T = 0: every valid word)
     unsigned c = 0;
-    if (use_k && search(false, 0, 0, true, T, c)) { cl.sync(); return; }
+    const bool cut = use_k && (unsigned) top_k < nv;
+    if (cut) search(false, 0, 0, T, c);
     if (use_p) {
-        const uint32_t over = use_k ? T : 0;
-        const u64 extra = use_k ? c * weigh(T) : 0;
+        const uint32_t over = T;
+        const u64 extra = cut ? c * weigh(T) : 0;
         uint32_t T2;
         unsigned c2;
-        if (search(true, over, extra, !use_k, T2, c2)) { cl.sync(); return; }
-        c = T2 == T && use_k ? min(c, c2) : c2;
+        search(true, over, extra, T2, c2);
+        c = T2 == T && cut ? min(c, c2) : c2;
         T = T2;
     }
     // the kept mass by id: per warp, then over the warps and the cluster
@@ -520,18 +663,18 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
     scan2(s, tb, sb, tt, st);
     tb = __shfl_sync(~0u, tb, 0);
     sb = __shfl_sync(~0u, sb, 0);
-    if (tid == 0) { s.part.cnt = tt; s.part.mass = st; s.nvalid = 0; }
+    if (tid == 0) { s.part_cnt = tt; s.part_mass = st; s.part_kept = 0; }
     __syncthreads();
-    if (lane == 0) atomicAdd(&s.nvalid, cnt);
+    if (lane == 0) atomicAdd(&s.part_kept, cnt);
     cl.sync();
     unsigned all_ties = 0, all_cnt = 0;
     u64 all = 0;
     for (int r = 0; r < C; r++) {
         const SampleShared &o = *cl.map_shared_rank(&s, r);
-        if (r < rank) { tb += o.part.cnt; sb += o.part.mass; }
-        all_ties += o.part.cnt;
-        all += o.part.mass;
-        all_cnt += o.nvalid;
+        if (r < rank) { tb += o.part_cnt; sb += o.part_mass; }
+        all_ties += o.part_cnt;
+        all += o.part_mass;
+        all_cnt += o.part_kept;
     }
     const unsigned ct = tie_in ? min(c, all_ties) : 0;
     const u64 W = all + ct * wT;
@@ -566,8 +709,7 @@ __global__ void __launch_bounds__(SM_NT) k_sample(const __grid_constant__ Sample
                 const unsigned at = bt + (T && k[e] == T);
                 const u64 after = b + w[e];
                 if ((double) mass_at(b, bt) <= target && (double) mass_at(after, at) > target) {
-                    const double z = k[e] == mx ? 0.0 : ((double) xmax - (double) value_of(k[e])) * weigh.inv;
-                    emit(first + o + e, (float) (-z - log((double) W / SM_ONE)), kept);
+                    emit(first + o + e, weigh.logprob(k[e], W), kept);
                 }
                 b = after;
                 bt = at;
