@@ -49,15 +49,22 @@ struct SampleArgs {
     int seg, slice;   // words per warp (a multiple of SM_TILE) and per CTA (SM_NW * seg)
 };
 
-// scores as unsigned keys in the same order; -infinity and NaN are 0, and so never kept; the zeros are one
+// scores as unsigned keys in the same order; NaN is -infinity, whose key no kept word has; the zeros are one
+constexpr uint32_t KEY_NONE = 0x007FFFFFu;
 __device__ __forceinline__ uint32_t key_of(float x) {
-    x = __fadd_rn(x, 0.0f);
-    const uint32_t b = __float_as_uint(x);
-    const uint32_t k = b ^ ((uint32_t) ((int) b >> 31) | 0x80000000u);
-    return x > -INFINITY ? k : 0u;   // false for NaN too
+    const uint32_t b = __float_as_uint(__fadd_rn(fmaxf(x, -INFINITY), 0.0f));
+    return b ^ ((uint32_t) ((int) b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+// the same as a 64-bit number, by integer operations: the conversion unit takes about eight times as long for one. Numbers
+// below 2^-126 become 0; infinity becomes a number (the callers look at the key).
+__device__ __forceinline__ double wide_of(uint32_t k) {
+    const uint32_t b = k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu), r = b & 0x7FFFFFFFu;
+    const uint32_t hi = r >= 0x00800000u ? (b & 0x80000000u) | ((r >> 3) + 0x38000000u) : 0u;
+    return __hiloint2double((int) hi, (int) (b << 29));
 }
 
 struct SampleShared {
@@ -113,14 +120,12 @@ __device__ __forceinline__ void scan2(SampleShared &s, unsigned &c, u64 &m, unsi
 // integer to z 64 / ln 2, exp(-z) = 2^(-n / 64) exp(r), r = n ln2 / 64 - z, |r| <= ln2 / 128, exp(r) to r^5 / 120 (the next
 // term is below 2^-54). n reaches 2,881 here, so the rounding of ln2 / 64 costs 2^-48 of a weight that is itself 2^-45 then.
 struct Weigher {
-    float xmax;
+    double xmax;
     uint32_t kmax;
     double inv;   // 1 / temperature
     const double *tab;
-    __device__ __forceinline__ double real(uint32_t k) const {
-        if (k == kmax) return 1.0;
-        const double z = ((double) xmax - (double) value_of(k)) * inv;
-        if (!(z < SM_FAR)) return 0.0;
+    __device__ __forceinline__ double real(uint32_t k) const {   // no branches: several words are in flight at once
+        const double z = (xmax - wide_of(k)) * inv;
         constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: adding it leaves the nearest integer in the low bits
         const double b = __fma_rn(z, -64.0 * 1.4426950408889634074, MAGIC);
         const int n = __double2loint(b);               // <= 0
@@ -131,7 +136,8 @@ struct Weigher {
         e = __fma_rn(r, e, 1.0);
         e = __fma_rn(r, e, 1.0);
         e = __dmul_rn(e, tab[n & (SM_TAB - 1)]);
-        return __hiloint2double(__double2hiint(e) + (n >> 6) * (1 << 20), __double2loint(e));
+        e = __hiloint2double(__double2hiint(e) + (n >> 6) * (1 << 20), __double2loint(e));
+        return k == kmax ? 1.0 : z < SM_FAR && k > KEY_NONE ? e : 0.0;
     }
     static __device__ __forceinline__ u64 whole(double w) {
         // w * 2^44 <= 2^44: added to 2^52 its integer part, rounded to nearest, is the low mantissa
@@ -139,7 +145,7 @@ struct Weigher {
     }
     __device__ __forceinline__ u64 operator()(uint32_t k) const { return whole(real(k)); }
     __device__ __forceinline__ float logprob(uint32_t k, u64 total) const {
-        const double z = k == kmax ? 0.0 : ((double) xmax - (double) value_of(k)) * inv;
+        const double z = k == kmax ? 0.0 : (xmax - (double) value_of(k)) * inv;
         return (float) (-z - log((double) total / SM_ONE));
     }
 };
@@ -152,6 +158,7 @@ __device__ __forceinline__ void sort_desc(u64 *v, int n) {
         int place = 0;
         if (tid < n) {
             x = v[tid];
+#pragma unroll 8
             for (int j = 0; j < n; j++) place += v[j] > x;
         }
         __syncthreads();
@@ -182,6 +189,26 @@ __device__ __forceinline__ float score_at(const S *x, int i) {
 }
 
 template <typename S>
+__device__ __forceinline__ void load4(const S *x, float (&f)[4]) {
+    if constexpr (sizeof(S) == 4) {
+        const float4 v = __ldg((const float4 *) x);
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else {
+        const uint2 v = __ldg((const uint2 *) x);
+#pragma unroll
+        for (int e = 0; e < 4; e++) f[e] = score_at((const S *) &v, e);
+    }
+}
+
+// a value of every CTA of the cluster: lane r holds CTA r's (other lanes `none`), read at once
+#define OF_CTAS(field, none) (lane < C ? cl.map_shared_rank(&s, lane)->field : (none))
+__device__ __forceinline__ u64 sum8(u64 v) {   // over the first 8 lanes, to all
+#pragma unroll
+    for (int o = 4; o; o >>= 1) v += __shfl_down_sync(~0u, v, o);
+    return __shfl_sync(~0u, v, 0);
+}
+
+template <typename S>
 __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ SampleArgs p) {
     extern __shared__ __align__(16) uint8_t sm_raw[];
     SampleShared &s = *(SampleShared *) sm_raw;
@@ -191,7 +218,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     const int C = (int) cl.num_blocks(), rank = (int) cl.block_rank();
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int base = rank * p.slice;                       // this CTA's first word
-    if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = 0; s.floor = 1; }
+    if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = 0; s.floor = KEY_NONE + 1; }
     if (tid < SM_TAB) s.tab[tid] = exp2((double) tid / SM_TAB);
     __syncthreads();
     pdl_wait();
@@ -212,31 +239,28 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     uint32_t mx = 0;
     uint32_t *mine = keys + warp * p.seg + 4 * lane;        // the words of a lane, tile by tile
     const int first = base + warp * p.seg + 4 * lane;
-#pragma unroll 4
-    for (int o = 0; o < p.seg; o += SM_TILE) {
-        const int i = first + o;
+    auto put = [&](int o, const float (&f)[4]) {
+        uint4 k = make_uint4(key_of(f[0]), key_of(f[1]), key_of(f[2]), key_of(f[3]));
+        mx = max(max(mx, max(k.x, k.y)), max(k.z, k.w));
+        *(uint4 *) (mine + o) = k;
+    };
+    const int inside = a.vocab - (base + warp * p.seg);     // words of the row in this warp's part
+    const int whole = vec ? max(0, min(p.seg, inside / SM_TILE * SM_TILE)) : 0;
+    int o = 0;
+    for (; o + 4 * SM_TILE <= whole; o += 4 * SM_TILE) {    // four tiles' loads in flight
+        float f[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) load4(x + first + o + t * SM_TILE, f[t]);
+#pragma unroll
+        for (int t = 0; t < 4; t++) put(o + t * SM_TILE, f[t]);
+    }
+    for (; o < p.seg; o += SM_TILE) {
         float f[4];
-        if (vec && i + 4 <= a.vocab) {
-            if constexpr (sizeof(S) == 4) {
-                const float4 v = __ldg((const float4 *) (x + i));
-                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-            } else {
-                const uint2 v = __ldg((const uint2 *) (x + i));
-                const S *h = (const S *) &v;
+        if (o < whole) load4(x + first + o, f);
+        else
 #pragma unroll
-                for (int e = 0; e < 4; e++) f[e] = score_at(h, e);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) f[e] = i + e < a.vocab ? score_at(x, i + e) : -INFINITY;
-        }
-        uint32_t k[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            k[e] = key_of(f[e]);
-            mx = max(mx, k[e]);
-        }
-        *(uint4 *) (mine + o) = make_uint4(k[0], k[1], k[2], k[3]);
+            for (int e = 0; e < 4; e++) f[e] = first + o + e < a.vocab ? score_at(x, first + o + e) : -INFINITY;
+        put(o, f);
     }
     // the r-th largest of the threads' maxima, to 20 bits downwards
     const bool by_k = use_k && top_k <= SM_LIST, by_p = !use_k && use_p, by_m = !use_k && !use_p && use_m;
@@ -248,21 +272,16 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             if (__syncthreads_count(mx >= (floor | 1u << b)) >= r_th) floor |= 1u << b;
     const uint32_t wmax = __reduce_max_sync(~0u, mx);
     if (lane == 0) atomicMax(&s.mx, wmax);
-    if (tid == 0) s.floor = max(floor, 1u);
+    if (tid == 0) s.floor = max(floor, KEY_NONE + 1);
     cl.sync();
-    mx = 0;
-    floor = ~0u;
-    for (int r = 0; r < C; r++) {
-        const SampleShared &o = *cl.map_shared_rank(&s, r);
-        mx = max(mx, o.mx);
-        floor = min(floor, o.floor);
-    }
+    mx = __reduce_max_sync(~0u, OF_CTAS(mx, 0u));
+    floor = __reduce_min_sync(~0u, OF_CTAS(floor, ~0u));
     auto emit = [&](int id, float lp, int kept) {
         a.ids[row] = id;
         if (a.logprob) a.logprob[row] = lp;
         if (a.kept) a.kept[row] = kept;
     };
-    if (mx == 0) {
+    if (mx <= KEY_NONE) {
         if (rank == 0 && tid == 0) emit(-1, -INFINITY, 0);
         cl.sync();   // no CTA leaves while another may read its shared memory
         return;
@@ -278,14 +297,12 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
         id = __reduce_min_sync(~0u, id);
         if (lane == 0) atomicMin(&s.idmin, id);
         cl.sync();
-        if (rank == 0 && tid == 0) {
-            for (int r = 0; r < C; r++) id = min(id, cl.map_shared_rank(&s, r)->idmin);
-            emit((int) id, 0.0f, 1);
-        }
+        id = __reduce_min_sync(~0u, OF_CTAS(idmin, ~0u));
+        if (rank == 0 && tid == 0) emit((int) id, 0.0f, 1);
         cl.sync();
         return;
     }
-    const Weigher weigh = { xmax, mx, 1.0 / (double) temp, s.tab };
+    const Weigher weigh = { (double) xmax, mx, 1.0 / (double) temp, s.tab };
 
     // The list of n words, which reaches down to some value, ends the row if all that can be kept is in it: the filters, and
     // the pick by id. of_all: the mass that top-p's share is of where top-k does not cut the list. False: the nucleus goes on
@@ -329,6 +346,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             if (tid < K) {
                 q = s.list[tid];
                 w = s.w[tid];
+#pragma unroll 4
                 for (int j = 0; j < K; j++) {
                     const u64 wj = s.w[j];
                     t += wj;
@@ -368,23 +386,47 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
         return true;
     };
 
+    // the CTAs' lists: how many words together, and all of them to the leading CTA's
+    auto collect_count = [&]() -> unsigned { return __reduce_add_sync(~0u, OF_CTAS(n_list, 0u)); };
+    auto collect = [&]() {
+        const unsigned c = OF_CTAS(n_list, 0u);
+        unsigned before = c;
+#pragma unroll
+        for (int d = 1; d < SM_MAX_CLUSTER; d <<= 1) {
+            const unsigned y = __shfl_up_sync(~0u, before, d);
+            if (lane >= d) before += y;
+        }
+        before -= c;
+        const int r = warp % SM_MAX_CLUSTER;   // two warps per CTA of the cluster
+        const unsigned at = __shfl_sync(~0u, before, r), n = __shfl_sync(~0u, c, r);
+        if (r > 0 && r < C) {
+            const SampleShared &o = *cl.map_shared_rank(&s, r);
+            for (unsigned i = (warp / SM_MAX_CLUSTER) * 32 + lane; i < n; i += SM_NT / SM_MAX_CLUSTER) s.list[at + i] = o.list[i];
+        }
+        __syncthreads();
+    };
+
     u64 W0 = 0;              // the row's whole mass, where the short way has summed it
     if (lists) {
         if (by_m) {          // what w >= m can reach, downwards by more than the roundings on the way
             const double lo = (double) xmax + (double) temp * log(m);
-            floor = max(key_of((float) (lo - 1e-6 * (fabs(lo) + fabs((double) xmax) + (double) temp))), 1u);
+            floor = max(key_of((float) (lo - 1e-6 * (fabs(lo) + fabs((double) xmax) + (double) temp))), KEY_NONE + 1);
         }
         u64 sum = 0;
         for (int o = 0; o < p.seg; o += SM_TILE) {
             const uint4 q = *(const uint4 *) (mine + o);
+            if (max(max(q.x, q.y), max(q.z, q.w)) >= floor)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t k = (&q.x)[e];
-                if (k >= floor) {
-                    const unsigned at = atomicAdd(&s.n_list, 1u);
-                    if (at < SM_LIST) s.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t k = (&q.x)[e];
+                    if (k >= floor) {
+                        const unsigned at = atomicAdd(&s.n_list, 1u);
+                        if (at < SM_LIST) s.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
+                    }
                 }
-                if (by_p && k) sum += weigh(k);
+            if (by_p) {   // the weight of -infinity is 0
+                const u64 w0 = weigh(q.x), w1 = weigh(q.y), w2 = weigh(q.z), w3 = weigh(q.w);
+                sum += (w0 + w1) + (w2 + w3);
             }
         }
         if (by_p) {
@@ -394,23 +436,10 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             if (tid == 0) s.part_mass = t;
         }
         cl.sync();
-        unsigned n = 0;
-        for (int r = 0; r < C; r++) {
-            const SampleShared &o = *cl.map_shared_rank(&s, r);
-            n += o.n_list;
-            if (by_p) W0 += o.part_mass;
-        }
+        if (by_p) W0 = sum8(OF_CTAS(part_mass, 0ull));
+        const unsigned n = collect_count();
         if (n <= SM_LIST) {
-            if (rank == 0) {
-                unsigned at = s.n_list;
-                for (int r = 1; r < C; r++) {
-                    const SampleShared &o = *cl.map_shared_rank(&s, r);
-                    const unsigned c = o.n_list;
-                    for (unsigned i = tid; i < c; i += SM_NT) s.list[at + i] = o.list[i];
-                    at += c;
-                }
-                __syncthreads();
-            }
+            if (rank == 0) collect();
             if (!by_p) {
                 cl.sync();   // the lists have been read
                 if (rank == 0) finish_list((int) n, 0);
@@ -431,7 +460,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
 
     // ---- the long way ----
     // the smallest key, and how many there are
-    {
+    if (use_k || use_p) {
         uint32_t mn = ~0u;
         unsigned nv = 0;
         for (int o = 0; o < p.seg; o += SM_TILE) {
@@ -439,21 +468,16 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const uint32_t k = (&q.x)[e];
-                if (k) { mn = min(mn, k); nv++; }
+                if (k > KEY_NONE) { mn = min(mn, k); nv++; }
             }
         }
         mn = __reduce_min_sync(~0u, mn);
         nv = __reduce_add_sync(~0u, nv);
         if (lane == 0) { atomicMin(&s.mn, mn); atomicAdd(&s.nvalid, nv); }
+        cl.sync();
     }
-    cl.sync();
-    uint32_t mn = ~0u;
-    unsigned nv = 0;
-    for (int r = 0; r < C; r++) {
-        const SampleShared &o = *cl.map_shared_rank(&s, r);
-        mn = min(mn, o.mn);
-        nv += o.nvalid;
-    }
+    const uint32_t mn = __reduce_min_sync(~0u, OF_CTAS(mn, ~0u));
+    const unsigned nv = __reduce_add_sync(~0u, OF_CTAS(nvalid, 0u));
     // One search: the value T, and how many words c at T, at which the count reaches k (by_mass false) or the mass
     // reaches p of the total (true). Only keys above `over` count; `extra` more mass lies at `over` itself.
     const float range = fminf(__fadd_rn(xmax, -value_of(mn)), 64.0f);
@@ -480,14 +504,17 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             __syncthreads();
             for (int o = 0; o < p.seg; o += SM_TILE) {
                 const uint4 q = *(const uint4 *) (mine + o);
+                u64 wv[4];
+                if (by_mass)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) wv[e] = weigh((&q.x)[e]);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const uint32_t k = (&q.x)[e];
-                    const int b = bin_of(k);
+                    const int b = bin_of((&q.x)[e]);
                     if (b < 0) continue;
                     atomicAdd(&s.cnt[b], 1u);
                     if (by_mass) {   // 64-bit addition by halves: the carry is what the low half's old value shows
-                        const u64 w = weigh(k);
+                        const u64 w = wv[e];
                         const unsigned wl = (unsigned) w, old = atomicAdd(&s.mass[b][0], wl);
                         const unsigned wh = (unsigned) (w >> 32) + (old + wl < old);
                         if (wh) atomicAdd(&s.mass[b][1], wh);
@@ -498,14 +525,19 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             // every CTA adds up all of them and finds the bin
             unsigned cn[2] = { 0, 0 };
             u64 ms[2] = { 0, 0 };
-            for (int r = 0; r < C; r++) {
-                const SampleShared &o = *cl.map_shared_rank(&s, r);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    cn[e] += o.cnt[2 * tid + e];
-                    if (by_mass) ms[e] += (u64) o.mass[2 * tid + e][1] << 32 | o.mass[2 * tid + e][0];
+            for (int r = 0; r < SM_MAX_CLUSTER; r++)
+                if (r < C) {
+                    const SampleShared &o = *cl.map_shared_rank(&s, r);
+                    const uint2 v = *(const uint2 *) &o.cnt[2 * tid];
+                    cn[0] += v.x;
+                    cn[1] += v.y;
+                    if (by_mass) {
+                        const uint4 w = *(const uint4 *) &o.mass[2 * tid][0];
+                        ms[0] += (u64) w.y << 32 | w.x;
+                        ms[1] += (u64) w.w << 32 | w.z;
+                    }
                 }
-            }
             unsigned c0 = cn[0] + cn[1], tc;
             u64 m0 = ms[0] + ms[1], tm;
             scan2(s, c0, m0, tc, tm);
@@ -565,14 +597,8 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             cl.sync();
             if (fits) {
                 if (rank == 0) {
-                    unsigned n = s.n_list;
-                    for (int r = 1; r < C; r++) {
-                        const SampleShared &o = *cl.map_shared_rank(&s, r);
-                        const unsigned oc = o.n_list;
-                        for (unsigned i = tid; i < oc; i += SM_NT) s.list[n + i] = o.list[i];
-                        n += oc;
-                    }
-                    __syncthreads();
+                    const unsigned n = collect_count();
+                    collect();
                     sort_desc(s.list, (int) n);
                     u64 wv[2] = { 0, 0 };
                     unsigned dc = 0, dt;
@@ -604,23 +630,17 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 cl.sync();
                 return;
             }
-            uint32_t lo = ~0u, hi = 0;
-            for (int r = 0; r < C; r++) {
-                const SampleShared &o = *cl.map_shared_rank(&s, r);
-                lo = min(lo, o.lo);
-                hi = max(hi, o.hi);
-            }
             if (level == 0) in_bin = bin;
-            klo = lo;
-            khi = hi;
+            klo = __reduce_min_sync(~0u, OF_CTAS(lo, ~0u));
+            khi = __reduce_max_sync(~0u, OF_CTAS(hi, 0u));
             cl.sync();   // read by all before they are cleared
         }
     };
 
-    uint32_t T = 0;          // kept: keys above T, and the first c words at T (T = 0: every valid word)
+    uint32_t T = KEY_NONE;   // kept: keys above T, and the first c words at T (KEY_NONE: every valid word)
     unsigned c = 0;
     const bool cut = use_k && (unsigned) top_k < nv;
-    if (cut) search(false, 0, 0, T, c);
+    if (cut) search(false, KEY_NONE, 0, T, c);
     if (use_p) {
         const uint32_t over = T;
         const u64 extra = cut ? c * weigh(T) : 0;
@@ -633,25 +653,32 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     // the kept mass by id: per warp, then over the warps and the cluster
     u64 sum = 0;
     unsigned ties = 0, cnt = 0;
-    const u64 wT = T ? weigh(T) : 0;
-    const bool tie_in = T && (!use_m || T == mx || weigh.real(T) >= m);
-    auto take = [&](uint32_t k, u64 &w) -> bool {   // a kept word above T
-        w = 0;
-        if (k <= T) return false;
-        const double r = weigh.real(k);
-        if (use_m && k != mx && r < m) return false;
-        w = Weigher::whole(r);
-        return true;
-    };
-    for (int o = 0; o < p.seg; o += SM_TILE) {
-        const uint4 q = *(const uint4 *) (mine + o);
+    const u64 wT = T > KEY_NONE ? weigh(T) : 0;
+    const bool tie_in = T > KEY_NONE && (!use_m || T == mx || weigh.real(T) >= m);
+    const bool ties_count = T > KEY_NONE;
+    // the kept words above T among four: their weights (else 0), how many; and how many words at T
+    auto take = [&](const uint4 &q, u64 (&w)[4], unsigned &kept, unsigned &at) {
+        w[0] = w[1] = w[2] = w[3] = 0;
+        kept = at = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) at += ties_count && (&q.x)[e] == T;
+        if (max(max(q.x, q.y), max(q.z, q.w)) <= T) return;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const uint32_t k = (&q.x)[e];
-            u64 w;
-            if (take(k, w)) { cnt++; sum += w; }
-            else if (T && k == T) ties++;
+            const double r = weigh.real(k);
+            const bool in = k > T && (!use_m || k == mx || r >= m);
+            w[e] = in ? Weigher::whole(r) : 0;
+            kept += in;
         }
+    };
+    for (int o = 0; o < p.seg; o += SM_TILE) {
+        u64 w[4];
+        unsigned kept, at;
+        take(*(const uint4 *) (mine + o), w, kept, at);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+        cnt += kept;
+        ties += at;
     }
     ties = __reduce_add_sync(~0u, ties);
     cnt = __reduce_add_sync(~0u, cnt);
@@ -663,59 +690,62 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     scan2(s, tb, sb, tt, st);
     tb = __shfl_sync(~0u, tb, 0);
     sb = __shfl_sync(~0u, sb, 0);
-    if (tid == 0) { s.part_cnt = tt; s.part_mass = st; s.part_kept = 0; }
+    if (tid == 0) { s.part_cnt = tt; s.part_mass = st; s.part_kept = 0; s.bin = -1; }
     __syncthreads();
     if (lane == 0) atomicAdd(&s.part_kept, cnt);
     cl.sync();
-    unsigned all_ties = 0, all_cnt = 0;
-    u64 all = 0;
-    for (int r = 0; r < C; r++) {
-        const SampleShared &o = *cl.map_shared_rank(&s, r);
-        if (r < rank) { tb += o.part_cnt; sb += o.part_mass; }
-        all_ties += o.part_cnt;
-        all += o.part_mass;
-        all_cnt += o.part_kept;
-    }
+    const unsigned rt = OF_CTAS(part_cnt, 0u);
+    const u64 rm = OF_CTAS(part_mass, 0ull);
+    const unsigned all_ties = __reduce_add_sync(~0u, rt), all_cnt = __reduce_add_sync(~0u, OF_CTAS(part_kept, 0u));
+    const u64 all = sum8(rm);
+    tb += __reduce_add_sync(~0u, lane < rank ? rt : 0u);
+    sb += sum8(lane < rank ? rm : 0ull);
     const unsigned ct = tie_in ? min(c, all_ties) : 0;
     const u64 W = all + ct * wT;
     const int kept = (int) (all_cnt + ct);
     const double target = (double) u * (double) W;
     auto mass_at = [&](u64 sum_, unsigned ties_) { return sum_ + min(ties_, ct) * wT; };
-    // the warp whose share the target falls in walks its words
-    if ((double) mass_at(sb, tb) <= target && (double) mass_at(sb + sum, tb + ties) > target) {
-        for (int o = 0; o < p.seg; o += SM_TILE) {
-            u64 w[4], ls = 0;
-            uint32_t k[4];
-            unsigned lt = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                k[e] = mine[o + e];
-                take(k[e], w[e]);
-                ls += w[e];
-                lt += T && k[e] == T;
+    // the warp whose share the target falls in is found; all warps of its CTA take its tiles, then one the tile's words
+    if (lane == 0 && (double) mass_at(sb, tb) <= target && (double) mass_at(sb + sum, tb + ties) > target) {
+        s.bin = warp;
+        s.mass_above = sb;
+        s.above = tb;
+    }
+    __syncthreads();
+    const int cross = s.bin;
+    if (cross >= 0) {
+        uint32_t *seg = keys + cross * p.seg + 4 * lane;
+        u64 b0 = s.mass_above;
+        unsigned t0 = s.above;
+        for (int o0 = 0; o0 < p.seg; o0 += SM_NW * SM_TILE) {   // rounds of a tile per warp
+            const int o = o0 + warp * SM_TILE;
+            const bool any = o < p.seg;
+            u64 w[4] = { 0, 0, 0, 0 };
+            unsigned n, lt = 0;
+            uint4 q = make_uint4(0, 0, 0, 0);
+            if (any) {
+                q = *(const uint4 *) (seg + o);
+                take(q, w, n, lt);
             }
-            u64 xs = ls;
-            unsigned xt = lt;
+            const u64 ls = (w[0] + w[1]) + (w[2] + w[3]);
+            u64 b = ls, tm;
+            unsigned bt = lt, tc;
+            scan2(s, bt, b, tc, tm);
+            b += b0;
+            bt += t0;
+            if (any && (double) mass_at(b, bt) <= target && (double) mass_at(b + ls, bt + lt) > target)
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const u64 ys = __shfl_up_sync(~0u, xs, d);
-                const unsigned yt = __shfl_up_sync(~0u, xt, d);
-                if (lane >= d) { xs += ys; xt += yt; }
-            }
-            u64 b = sb + xs - ls;
-            unsigned bt = tb + xt - lt;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const unsigned at = bt + (T && k[e] == T);
-                const u64 after = b + w[e];
-                if ((double) mass_at(b, bt) <= target && (double) mass_at(after, at) > target) {
-                    emit(first + o + e, weigh.logprob(k[e], W), kept);
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t k = (&q.x)[e];
+                    const unsigned at = bt + (ties_count && k == T);
+                    const u64 after = b + w[e];
+                    if ((double) mass_at(b, bt) <= target && (double) mass_at(after, at) > target)
+                        emit(base + cross * p.seg + 4 * lane + o + e, weigh.logprob(k, W), kept);
+                    b = after;
+                    bt = at;
                 }
-                b = after;
-                bt = at;
-            }
-            sb += __shfl_sync(~0u, xs, 31);
-            tb += __shfl_sync(~0u, xt, 31);
+            b0 += tm;
+            t0 += tc;
         }
     }
     cl.sync();
