@@ -9,13 +9,14 @@
 //
 // A row is held in the shared memory of a cluster of 1 to 8 CTAs, as integer keys that order like the scores: it is
 // read from HBM once, and every later pass is over shared memory.
-//   The short way: while loading, every thread keeps its own words' maximum. The r-th largest of a CTA's thread maxima is
-// a value that r of its words reach, so the smallest of these over the cluster, with r = ceil(k / CTAs), is one that k
-// words reach; for top-p alone r is set for about 500 words, for min-p alone the value follows from the maximum. The few
-// words above it are listed, and one CTA sorts them and applies the filters. Top-p's total mass is summed meanwhile.
-//   The long way, where the list would be too long or ends inside the nucleus: a histogram over 1,024 steps of score
-// (counts, masses), whose crossing bin is sorted by one CTA; a bin too full for that (masked words, all scores alike) is
-// cut again, by keys. Then every CTA sums its kept words by id.
+//   The list: while loading, every thread keeps its own words' maximum. The r-th largest of a CTA's thread maxima is a value
+// that r of its words reach, so the smallest of these over the cluster, with r = ceil(k / CTAs), is one that k words reach;
+// for top-p alone r is set for about 400 words, for min-p alone the value follows from the maximum. The words above it are
+// listed, and one CTA applies the filters to the list. What top-p needs of the other words is their mass: it is summed
+// in 32 bits, and only where the nucleus's end depends on the error of that sum, or lies below the list, in full.
+//   A nucleus, or a top-k, that goes on below the list: a histogram over 1,024 steps of score, of masses (or counts), is
+// searched, the crossing bin's words listed and searched in turn; a bin too full for a list (scores crowded in few steps,
+// masked words) is cut again, by keys, until it fits or is a single value. Then every CTA sums its kept words by id.
 #include "common.cuh"
 #include "serve.h"
 
@@ -31,14 +32,19 @@ namespace {
 
 constexpr int SM_NT = 512, SM_NW = SM_NT / 32;
 constexpr int SM_BINS = 2 * SM_NT;       // two bins per thread in the scans
-constexpr int SM_LIST = 1024;            // words one CTA sorts at most
-constexpr int SM_AIM = 512;              // words listed for top-p alone, about
+constexpr int SM_LIST = 768;             // words of a list at most
+constexpr int SM_AIM = 384;              // words listed for top-p alone, about
+constexpr int SM_SHORT = SM_NT / 4;      // words of a list that are all compared with one another
+constexpr int SM_PILES = 256;            // piles that a search in a longer list throws its words into
+constexpr int SM_STEPS = 256;            // steps in which the threads' maxima are ranked
+// the 32-bit mass's relative error at most: of a word's exponent (up to 45) 2^-23 twice, in powers of 2, its exp2 2^-22, the
+// sum of up to 64 words of a thread 2^-18; the threads' sums are added in 64 bits
+constexpr double SM_MASS_ERR = 45 * 0.7 * 2.4e-7 + 2.4e-7 + 3.9e-6;
 constexpr int SM_TILE = 128;             // words of a warp's load: four per lane
 constexpr int SM_MAX_CLUSTER = 8;
 constexpr int SM_SLICE = 32768;          // words a CTA holds at most
 constexpr double SM_ONE = 17592186044416.0;   // 2^44
 constexpr double SM_FAR = 31.2;          // exp(-31.2) < 2^-45: such a word's weight rounds to 0
-constexpr int SM_TAB = 64;               // steps of the exponential's table
 static_assert((long long) SM_SLICE * SM_MAX_CLUSTER >= IMI_CUDA_SAMPLE_VOCAB, "a row fits a cluster");
 static_assert((long long) IMI_CUDA_SAMPLE_VOCAB <= 1 << 18, "the weights' sum fits 62 bits");
 
@@ -59,33 +65,37 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// the same as a 64-bit number, by integer operations: the conversion unit takes about eight times as long for one. Numbers
-// below 2^-126 become 0; infinity becomes a number (the callers look at the key).
-__device__ __forceinline__ double wide_of(uint32_t k) {
-    const uint32_t b = k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu), r = b & 0x7FFFFFFFu;
-    const uint32_t hi = r >= 0x00800000u ? (b & 0x80000000u) | ((r >> 3) + 0x38000000u) : 0u;
-    return __hiloint2double((int) hi, (int) (b << 29));
-}
-
 struct SampleShared {
     union {
         struct {
             unsigned cnt[SM_BINS], mass[SM_BINS][2];   // this CTA's histogram; mass: low and high words
         };
         struct {
-            u64 list[SM_LIST], w[SM_LIST];   // (key, ~id) listed; weights in the list's order
+            u64 list[SM_LIST];               // leading CTA: (key, ~id) of all CTAs' words
+            u64 w[SM_LIST];                  // this CTA's words until they are there; then the list's weights
+            unsigned pile[SM_PILES][2];      // masses, low and high words
+            unsigned short member[SM_LIST];
+        };
+        struct {
+            u64 list_[SM_LIST];
+            unsigned steps[SM_STEPS];        // the threads' maxima ranked
         };
     };
-    double tab[SM_TAB];               // 2^(i / 64)
     unsigned wc[SM_NW];               // scans over the CTA
     u64 wm[SM_NW];
     // what the cluster reads of this CTA
-    u64 part_mass;
-    unsigned part_cnt, part_kept, mx, mn, nvalid, floor, idmin, n_list, lo, hi;
+    unsigned mx, mn, lmin, nvalid, floor, idmin, n_list, n_all, at_lead, part_kept, lo, hi;
+    // of every CTA of the cluster, written here by it: read after a barrier, and never by two exchanges in a row
+    unsigned all_mx[SM_MAX_CLUSTER], all_floor[SM_MAX_CLUSTER], all_n[SM_MAX_CLUSTER], all_cnt[SM_MAX_CLUSTER], all_kept[SM_MAX_CLUSTER];
+    double all_near[SM_MAX_CLUSTER];
+    u64 all_mass[SM_MAX_CLUSTER], all_sum[SM_MAX_CLUSTER];
     u64 mass_above;
     int bin;                          // found in a scan: the crossing bin, and what lies above it
     unsigned above, in_bin;
     unsigned T, c, done;              // the leading CTA's findings
+    u64 found, found_after;           // a search in the list
+    u64 total;
+    unsigned n_member;
 };
 
 // exclusive sums over the CTA's threads, and the totals
@@ -116,28 +126,30 @@ __device__ __forceinline__ void scan2(SampleShared &s, unsigned &c, u64 &m, unsi
     m = bm + xm - m;
 }
 
-// A word's weight, as a number and as an integer of 2^-44. exp by table (Tang, ACM TOMS 15, 1989): with n the nearest
-// integer to z 64 / ln 2, exp(-z) = 2^(-n / 64) exp(r), r = n ln2 / 64 - z, |r| <= ln2 / 128, exp(r) to r^5 / 120 (the next
-// term is below 2^-54). n reaches 2,881 here, so the rounding of ln2 / 64 costs 2^-48 of a weight that is itself 2^-45 then.
+// A word's weight, as a number and as an integer of 2^-44. With n the nearest integer to -z / ln 2, exp(-z) = 2^n exp(r),
+// |r| <= ln2 / 2; exp(r) by the polynomial through its values at 11 Chebyshev nodes (relative error below 2^-51). A table
+// and a shorter polynomial took twice as long: 32 lanes' reads of it fall on a few banks.
 struct Weigher {
     double xmax;
     uint32_t kmax;
     double inv;   // 1 / temperature
-    const double *tab;
     __device__ __forceinline__ double real(uint32_t k) const {   // no branches: several words are in flight at once
-        const double z = (xmax - wide_of(k)) * inv;
+        const double z = (xmax - (double) value_of(k)) * inv;
         constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: adding it leaves the nearest integer in the low bits
-        const double b = __fma_rn(z, -64.0 * 1.4426950408889634074, MAGIC);
-        const int n = __double2loint(b);               // <= 0
-        const double r = __fma_rn(__dadd_rn(b, -MAGIC), -0.69314718055994530942 / 64.0, -z);
-        double e = __fma_rn(r, 1.0 / 120.0, 1.0 / 24.0);
-        e = __fma_rn(r, e, 1.0 / 6.0);
-        e = __fma_rn(r, e, 0.5);
+        const double b = __fma_rn(z, -1.4426950408889634074, MAGIC);
+        const double r = __fma_rn(__dadd_rn(b, -MAGIC), -0.69314718055994530942, -z);
+        double e = __fma_rn(r, 2.7626357241447223e-07, 2.764018079620985e-06);
+        e = __fma_rn(r, e, 2.4801504346997686e-05);
+        e = __fma_rn(r, e, 0.00019841170270440067);
+        e = __fma_rn(r, e, 0.0013888888932488599);
+        e = __fma_rn(r, e, 0.008333333385667782);
+        e = __fma_rn(r, e, 0.04166666666657314);
+        e = __fma_rn(r, e, 0.16666666666554406);
+        e = __fma_rn(r, e, 0.5000000000000006);
+        e = __fma_rn(r, e, 1.0000000000000067);
         e = __fma_rn(r, e, 1.0);
-        e = __fma_rn(r, e, 1.0);
-        e = __dmul_rn(e, tab[n & (SM_TAB - 1)]);
-        e = __hiloint2double(__double2hiint(e) + (n >> 6) * (1 << 20), __double2loint(e));
-        return k == kmax ? 1.0 : z < SM_FAR && k > KEY_NONE ? e : 0.0;
+        e = __hiloint2double(__double2hiint(e) + __double2loint(b) * (1 << 20), __double2loint(e));
+        return k == kmax ? 1.0 : z < SM_FAR ? e : 0.0;   // z NaN or infinite (infinities): 0
     }
     static __device__ __forceinline__ u64 whole(double w) {
         // w * 2^44 <= 2^44: added to 2^52 its integer part, rounded to nearest, is the low mantissa
@@ -150,35 +162,66 @@ struct Weigher {
     }
 };
 
-// v[0..n) sorted descending (all different, n at most SM_LIST, room up to the next power of two)
-__device__ __forceinline__ void sort_desc(u64 *v, int n) {
-    const int tid = threadIdx.x;
-    if (n <= 256) {   // each value's place counted: a pass over n values, against 36 exchanges with a barrier each
-        u64 x = 0;
-        int place = 0;
-        if (tid < n) {
-            x = v[tid];
-#pragma unroll 8
-            for (int j = 0; j < n; j++) place += v[j] > x;
-        }
-        __syncthreads();
-        if (tid < n) v[place] = x;
-        __syncthreads();
-        return;
-    }
-    int n2 = 512;
-    while (n2 < n) n2 <<= 1;
-    for (int i = n + tid; i < n2; i += SM_NT) v[i] = 0;
+// 64-bit addition by halves: the carry is what the low half's old value shows
+__device__ __forceinline__ void add64(unsigned (&at)[2], u64 w) {
+    const unsigned wl = (unsigned) w, old = atomicAdd(&at[0], wl), wh = (unsigned) (w >> 32) + (old + wl < old);
+    if (wh) atomicAdd(&at[1], wh);
+}
+// A search in the list of n words: in the order of ord (larger first; no two alike), the word with cross(b, b + weight) where
+// b is what lies before it, `above` more than the words in front of it in the list. pile(word) is 0..SM_PILES-1 in that order,
+// or -1 for a word that is not in question. The piles' sums show which pile it is in, a comparison of that pile's words which it
+// is: no sort. s.found is 0 if there is none; s.found_after is the sum up to and with it.
+template <typename P, typename W, typename O, typename X>
+__device__ __forceinline__ void search_list(SampleShared &s, int n, u64 above, P pile, W weight, O ord, X cross) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    for (int i = tid; i < SM_PILES; i += SM_NT) s.pile[i][0] = s.pile[i][1] = 0;
+    if (tid == 0) { s.found = s.found_after = 0; s.n_member = 0; }
     __syncthreads();
-    for (int k = 2; k <= n2; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int i = tid; i < n2 / 2; i += SM_NT) {
-                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                const u64 x = v[lo], y = v[hi];
-                if ((x < y) == ((lo & k) == 0)) { v[lo] = y; v[hi] = x; }
-            }
-            __syncthreads();
+    for (int i = tid; i < n; i += SM_NT) {
+        const int b = pile(s.list[i]);
+        if (b >= 0) add64(s.pile[b], weight(i));
+    }
+    __syncthreads();
+    u64 v[SM_PILES / 32], sum = 0;
+#pragma unroll
+    for (int e = 0; e < SM_PILES / 32; e++) {
+        const unsigned *q = s.pile[SM_PILES / 32 * lane + e];
+        sum += v[e] = (u64) q[1] << 32 | q[0];
+    }
+    u64 b = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(~0u, b, o);
+        if (lane >= o) b += y;
+    }
+    b += above - sum;
+    int at = -1;
+    u64 before = 0;
+#pragma unroll
+    for (int e = 0; e < SM_PILES / 32; e++) {
+        if (at < 0 && cross(b, b + v[e])) { at = SM_PILES / 32 * lane + e; before = b; }
+        b += v[e];
+    }
+    const unsigned who = __ballot_sync(~0u, at >= 0);
+    if (!who) return;   // the same for every warp
+    at = __shfl_sync(~0u, at, __ffs(who) - 1);
+    before = __shfl_sync(~0u, before, __ffs(who) - 1);
+    for (int i = tid; i < n; i += SM_NT)
+        if (pile(s.list[i]) == at) s.member[atomicAdd(&s.n_member, 1u)] = (unsigned short) i;
+    __syncthreads();
+    const int m = (int) s.n_member;
+    for (int i = tid; i < m; i += SM_NT) {
+        const int j0 = s.member[i];
+        const auto mine = ord(s.list[j0]);
+        u64 x = before;
+        for (int k = 0; k < m; k++) {
+            const int j = s.member[k];
+            if (ord(s.list[j]) > mine) x += weight(j);
         }
+        const u64 y = x + weight(j0);
+        if (cross(x, y)) { s.found = s.list[j0]; s.found_after = y; }
+    }
+    __syncthreads();
 }
 
 template <typename S>
@@ -202,7 +245,8 @@ __device__ __forceinline__ void load4(const S *x, float (&f)[4]) {
 
 // a value of every CTA of the cluster: lane r holds CTA r's (other lanes `none`), read at once
 #define OF_CTAS(field, none) (lane < C ? cl.map_shared_rank(&s, lane)->field : (none))
-__device__ __forceinline__ u64 sum8(u64 v) {   // over the first 8 lanes, to all
+template <typename V>
+__device__ __forceinline__ V sum8(V v) {   // over the first 8 lanes, to all
 #pragma unroll
     for (int o = 4; o; o >>= 1) v += __shfl_down_sync(~0u, v, o);
     return __shfl_sync(~0u, v, 0);
@@ -218,9 +262,10 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     const int C = (int) cl.num_blocks(), rank = (int) cl.block_rank();
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int base = rank * p.slice;                       // this CTA's first word
-    if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = 0; s.floor = KEY_NONE + 1; }
-    if (tid < SM_TAB) s.tab[tid] = exp2((double) tid / SM_TAB);
+    if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = s.n_all = 0; s.floor = s.lmin = ~0u; }
+    if (tid < SM_STEPS) s.steps[tid] = 0;
     __syncthreads();
+    auto started = cl.barrier_arrive();   // this CTA's shared memory may be written by the others
     pdl_wait();
     pdl_trigger();
     const float temp = a.temperature ? a.temperature[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f,
@@ -247,12 +292,30 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     const int inside = a.vocab - (base + warp * p.seg);     // words of the row in this warp's part
     const int whole = vec ? max(0, min(p.seg, inside / SM_TILE * SM_TILE)) : 0;
     int o = 0;
-    for (; o + 4 * SM_TILE <= whole; o += 4 * SM_TILE) {    // four tiles' loads in flight
-        float f[4][4];
+    if constexpr (sizeof(S) == 4) {
+        for (; o + 4 * SM_TILE <= whole; o += 4 * SM_TILE) {   // four tiles' loads in flight
+            float f[4][4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) load4(x + first + o + t * SM_TILE, f[t]);
+            for (int t = 0; t < 4; t++) load4(x + first + o + t * SM_TILE, f[t]);
 #pragma unroll
-        for (int t = 0; t < 4; t++) put(o + t * SM_TILE, f[t]);
+            for (int t = 0; t < 4; t++) put(o + t * SM_TILE, f[t]);
+        }
+    } else if (((uintptr_t) (x + base) & 15) == 0) {           // 16 bytes per lane, two tiles at once; which lane has a word
+        for (; o + 8 * SM_TILE <= whole; o += 8 * SM_TILE) {   // does not matter to what follows
+            uint4 v[4];
+            const S *at = x + first + 4 * lane + o;
+#pragma unroll
+            for (int t = 0; t < 4; t++) v[t] = __ldg((const uint4 *) (at + t * 2 * SM_TILE));
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float f[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f[e] = score_at((const S *) &v[t], 4 * h + e);
+                    put(o + t * 2 * SM_TILE + 4 * lane + 4 * h, f);
+                }
+        }
     }
     for (; o < p.seg; o += SM_TILE) {
         float f[4];
@@ -262,20 +325,55 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             for (int e = 0; e < 4; e++) f[e] = first + o + e < a.vocab ? score_at(x, first + o + e) : -INFINITY;
         put(o, f);
     }
-    // the r-th largest of the threads' maxima, to 20 bits downwards
+    // the value that the r-th largest of the threads' maxima reaches: the maxima ranked in 256 steps, all steps down to the
+    // one of the r-th taken whole
     const bool by_k = use_k && top_k <= SM_LIST, by_p = !use_k && use_p, by_m = !use_k && !use_p && use_m;
     const int r_th = by_k ? (top_k + C - 1) / C : by_p ? SM_AIM / C : 0;
     const bool lists = !greedy && r_th <= SM_NT && (by_k || by_p || by_m);
-    uint32_t floor = 0;
-    if (lists && r_th)
-        for (int b = 31; b >= 12; b--)
-            if (__syncthreads_count(mx >= (floor | 1u << b)) >= r_th) floor |= 1u << b;
-    const uint32_t wmax = __reduce_max_sync(~0u, mx);
+    const uint32_t lmx = mx, wmax = __reduce_max_sync(~0u, mx);
     if (lane == 0) atomicMax(&s.mx, wmax);
-    if (tid == 0) s.floor = max(floor, KEY_NONE + 1);
+    if (lists && r_th) {
+        const uint32_t wmin = __reduce_min_sync(~0u, mx > KEY_NONE ? mx : ~0u);
+        if (lane == 0) atomicMin(&s.lmin, wmin);
+        __syncthreads();
+        // masked words of low values must not stretch the steps: what lies further down shares the last one
+        const float top = value_of(s.mx), span = fminf(__fadd_rn(top, -value_of(min(s.lmin, s.mx))), 64.0f);
+        const float sc = span > 0.0f ? __fdiv_rn((float) SM_STEPS, span) : 0.0f;
+        const int st = lmx <= KEY_NONE || lmx == s.mx ? (lmx <= KEY_NONE ? SM_STEPS - 1 : 0)
+                                                      : min(SM_STEPS - 1, __float2int_rz(__fmul_rn(__fadd_rn(top, -value_of(lmx)), sc)));
+        unsigned *h = s.steps;
+        atomicAdd(&h[st], 1u);
+        __syncthreads();
+        unsigned c8[8], c = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) c += c8[e] = h[8 * lane + e];
+        unsigned up = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned y = __shfl_up_sync(~0u, up, o);
+            if (lane >= o) up += y;
+        }
+        int step = SM_STEPS;
+        unsigned run = up - c;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (run < (unsigned) r_th && run + c8[e] >= (unsigned) r_th) step = 8 * lane + e;
+            run += c8[e];
+        }
+        step = __reduce_min_sync(~0u, step);
+        const uint32_t low = __reduce_min_sync(~0u, st <= step ? lmx : ~0u);
+        if (lane == 0) atomicMin(&s.floor, low);
+    }
+    __syncthreads();
+    cl.barrier_wait(std::move(started));
+    if (tid < C) {
+        SampleShared &o = *cl.map_shared_rank(&s, tid);
+        o.all_mx[rank] = s.mx;
+        o.all_floor[rank] = s.floor;
+    }
     cl.sync();
-    mx = __reduce_max_sync(~0u, OF_CTAS(mx, 0u));
-    floor = __reduce_min_sync(~0u, OF_CTAS(floor, ~0u));
+    mx = __reduce_max_sync(~0u, lane < C ? s.all_mx[lane] : 0u);
+    uint32_t floor = max(__reduce_min_sync(~0u, lane < C ? s.all_floor[lane] : ~0u), KEY_NONE + 1);
     auto emit = [&](int id, float lp, int kept) {
         a.ids[row] = id;
         if (a.logprob) a.logprob[row] = lp;
@@ -283,7 +381,6 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     };
     if (mx <= KEY_NONE) {
         if (rank == 0 && tid == 0) emit(-1, -INFINITY, 0);
-        cl.sync();   // no CTA leaves while another may read its shared memory
         return;
     }
     const float xmax = value_of(mx);
@@ -295,124 +392,152 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 for (int e = 0; e < 4; e++)
                     if (mine[o + e] == mx) id = min(id, (unsigned) (first + o + e));
         id = __reduce_min_sync(~0u, id);
-        if (lane == 0) atomicMin(&s.idmin, id);
+        if (lane == 0 && id != ~0u) atomicMin(&cl.map_shared_rank(&s, 0)->idmin, id);
         cl.sync();
-        id = __reduce_min_sync(~0u, OF_CTAS(idmin, ~0u));
-        if (rank == 0 && tid == 0) emit((int) id, 0.0f, 1);
-        cl.sync();
+        if (rank == 0 && tid == 0) emit((int) s.idmin, 0.0f, 1);
         return;
     }
-    const Weigher weigh = { (double) xmax, mx, 1.0 / (double) temp, s.tab };
+    const Weigher weigh = { (double) xmax, mx, 1.0 / (double) temp };
 
-    // The list of n words, which reaches down to some value, ends the row if all that can be kept is in it: the filters, and
-    // the pick by id. of_all: the mass that top-p's share is of where top-k does not cut the list. False: the nucleus goes on
-    // below the list.
-    auto finish_list = [&](int n, u64 of_all) -> bool {
-        sort_desc(s.list, n);
-        if (use_k) n = min(n, top_k);
-        // two words per thread: weights, their sums, and how many pass
-        u64 wv[2], sum = 0;
-        unsigned pass = 0;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int j = 2 * tid + e;
-            const double w = j < n ? weigh.real((uint32_t) (s.list[j] >> 32)) : 0.0;
-            wv[e] = j < n ? Weigher::whole(w) : 0;
-            if (j < n) s.w[j] = wv[e];
-            if (j < n && (!use_m || j == 0 || w >= m)) pass++;
-            sum += wv[e];
+    // searches in the leading CTA's list
+    constexpr u64 PASS = 1ull << 63;   // with a weight: the word passes min-p
+    auto weigh_list = [&](int n) {
+        for (int i = tid; i < n; i += SM_NT) {
+            const double w = weigh.real((uint32_t) (s.list[i] >> 32));
+            s.w[i] = Weigher::whole(w) | (!use_m || w >= m ? PASS : 0);
         }
-        unsigned ex = pass, tp;
-        u64 before = sum, total;
-        scan2(s, ex, before, tp, total);
-        int K = (int) tp;
-        if (use_p) {
-            const double lim = pd * (double) (use_k ? total : of_all);
-            if (!use_k && (double) total < lim) return false;
-            unsigned keep = 0, all;
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int j = 2 * tid + e;
-                if (j < n && (j == 0 || (double) before < lim)) keep++;
-                before += wv[e];
-            }
-            u64 d0 = 0, d1;
-            scan2(s, keep, d0, all, d1);
-            K = min(K, (int) all);
+    };
+    // the smallest and the largest of f(word) over the list
+    auto ends = [&](int n, auto f, uint32_t &lo, uint32_t &hi) {
+        uint32_t l = ~0u, h = 0;
+        for (int i = tid; i < n; i += SM_NT) {
+            const uint32_t v = f(s.list[i]);
+            l = min(l, v);
+            h = max(h, v);
         }
+        l = __reduce_min_sync(~0u, l);
+        h = __reduce_max_sync(~0u, h);
         __syncthreads();
-        if (K <= 128) {   // each word's running sum by id counted directly
-            u64 b = 0, t = 0, q = 0, w = 0;
-            if (tid < K) {
-                q = s.list[tid];
-                w = s.w[tid];
+        if (lane == 0) s.wm[warp] = (u64) l << 32 | h;
+        __syncthreads();
+        const u64 v = s.wm[lane % SM_NW];
+        lo = __reduce_min_sync(~0u, (unsigned) (v >> 32));
+        hi = __reduce_max_sync(~0u, (unsigned) v);
+    };
+    auto by_score = [&](int n, u64 above, auto weight, auto cross) {
+        uint32_t lo, hi;
+        ends(n, [](u64 q) { return (uint32_t) (q >> 32); }, lo, hi);
+        const float top = value_of(hi), sp = fminf(__fadd_rn(top, -value_of(lo)), 3e38f), f = sp > 0.0f ? __fdiv_rn((float) SM_PILES, sp) : 0.0f;
+        search_list(s, n, above, [&](u64 q) -> int {
+            const uint32_t k = (uint32_t) (q >> 32);
+            return k == hi ? 0 : min(SM_PILES - 1, __float2int_rz(__fmul_rn(__fadd_rn(top, -value_of(k)), f)));
+        }, weight, [](u64 q) { return q; }, cross);
+    };
+    auto whole_of = [&](int i) -> u64 { return s.w[i] & ~PASS; };
+    // what the list's words from `last` on upwards weigh together
+    auto list_mass = [&](int n, u64 last, bool pass, unsigned &cnt) -> u64 {
+        u64 sum = 0, total;
+        unsigned c = 0;
+        for (int i = tid; i < n; i += SM_NT)
+            if (s.list[i] >= last && (!pass || (s.w[i] & PASS))) { sum += s.w[i] & ~PASS; c++; }
+        scan2(s, c, sum, cnt, total);
+        return total;
+    };
+    // a short list: four threads per word compare it with all others. The word's place in the order of scores, the mass before
+    // it and with it (all four threads)
+    struct Place {
+        bool in;
+        int rank;
+        u64 before, after;
+    };
+    auto quad = [&](u64 v) {
+        v += __shfl_xor_sync(~0u, v, 1);
+        return v + __shfl_xor_sync(~0u, v, 2);
+    };
+    auto place = [&](int n) -> Place {
+        Place r = { tid / 4 < n, 0, 0, 0 };
+        if (r.in) {
+            const u64 q = s.list[tid / 4];
 #pragma unroll 4
-                for (int j = 0; j < K; j++) {
-                    const u64 wj = s.w[j];
-                    t += wj;
-                    if ((unsigned) s.list[j] > (unsigned) q) b += wj;   // ~id larger: id smaller
-                }
-                const double target = (double) u * (double) t;
-                if ((double) b <= target && (double) (b + w) > target)
-                    emit((int) ~(unsigned) q, weigh.logprob((uint32_t) (q >> 32), t), K);
-            }
-            return true;
+            for (int j = tid & 3; j < n; j += 4)
+                if (s.list[j] > q) { r.rank++; r.before += s.w[j] & ~PASS; }
         }
-        // by id: (~id, place in the order of scores) sorted descending
-        for (int j = tid; j < K; j += SM_NT) s.list[j] = s.list[j] << 32 | (unsigned) j;
+        r.rank += __shfl_xor_sync(~0u, r.rank, 1);
+        r.rank += __shfl_xor_sync(~0u, r.rank, 2);
+        r.before = quad(r.before);
+        r.after = r.in ? r.before + (s.w[tid / 4] & ~PASS) : 0;
+        return r;
+    };
+    auto short_pick = [&](int n, bool keep) {
+        const int i = tid / 4;
+        keep = keep && (s.w[i] & PASS);
+        const u64 w = keep ? s.w[i] & ~PASS : 0, q = i < n ? s.list[i] : 0;
         __syncthreads();
-        sort_desc(s.list, K);
-        sum = 0;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int j = 2 * tid + e;
-            wv[e] = j < K ? s.w[(unsigned) s.list[j]] : 0;
-            sum += wv[e];
+        if ((tid & 3) == 0 && i < n) s.w[i] = w;
+        const int K = __syncthreads_count(keep) / 4;
+        u64 b = 0, t = 0;
+#pragma unroll 4
+        for (int j = tid & 3; j < n; j += 4) {
+            const u64 wj = s.w[j];
+            t += wj;
+            if ((unsigned) s.list[j] > (unsigned) q) b += wj;   // ~id larger: id smaller
+        }
+        b = quad(b);
+        t = quad(t);
+        const double target = (double) u * (double) t;
+        if ((tid & 3) == 0 && keep && (double) b <= target && (double) (b + w) > target)
+            emit((int) ~(unsigned) q, weigh.logprob((uint32_t) (q >> 32), t), K);
+    };
+    // the pick, by id, among the list's words from `last` on upwards that pass min-p
+    auto pick = [&](int n, u64 last) {
+        unsigned K;
+        const u64 total = list_mass(n, last, true, K);
+        const double target = (double) u * (double) total;
+        uint32_t lo, hi;   // of ~id: larger first
+        ends(n, [](u64 q) { return (uint32_t) q; }, lo, hi);
+        const float f = __fdiv_rn((float) SM_PILES, (float) (hi - lo + 1));
+        search_list(s, n, 0, [&](u64 q) -> int { return min(SM_PILES - 1, (int) __fmul_rn((float) (hi - (unsigned) q), f)); }, [&](int i) -> u64 { return s.list[i] >= last && (s.w[i] & PASS) ? s.w[i] & ~PASS : 0; },
+            [](u64 q) { return (unsigned) q; }, [&](u64 b, u64 e) { return (double) b <= target && (double) e > target; });
+        if (tid == 0) emit((int) ~(unsigned) s.found, weigh.logprob((uint32_t) (s.found >> 32), total), (int) K);
+    };
+
+    // this CTA's words to the leading one's list, behind those that came before, and its count to every CTA (too many words are
+    // cut: the counts show it). A cluster barrier comes next
+    auto push_list = [&]() {
+        __syncthreads();
+        SampleShared &lead = *cl.map_shared_rank(&s, 0);
+        const unsigned n = s.n_list;
+        if (tid == 0) s.at_lead = atomicAdd(&lead.n_all, n);
+        __syncthreads();
+        const unsigned at = s.at_lead;
+        for (unsigned i = tid; i < min(n, (unsigned) SM_LIST); i += SM_NT)
+            if (at + i < SM_LIST) lead.list[at + i] = s.w[i];
+        if (tid < C) cl.map_shared_rank(&s, tid)->all_n[rank] = n;
+    };
+    auto list_length = [&]() -> int { return (int) __reduce_add_sync(~0u, lane < C ? s.all_n[lane] : 0u); };
+
+    // the row's whole mass, in full: every CTA's part summed, then the cluster's
+    auto whole_mass = [&]() -> u64 {
+        u64 sum = 0;
+        for (int o = 0; o < p.seg; o += SM_TILE) {
+            const uint4 q = *(const uint4 *) (mine + o);
+            const u64 w0 = weigh(q.x), w1 = weigh(q.y), w2 = weigh(q.z), w3 = weigh(q.w);   // the weight of -infinity is 0
+            sum += (w0 + w1) + (w2 + w3);
         }
         unsigned d0 = 0, d1;
-        before = sum;
-        scan2(s, d0, before, d1, total);
-        const double target = (double) u * (double) total;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int j = 2 * tid + e;
-            const u64 after = before + wv[e];
-            if (j < K && (double) before <= target && (double) after > target) {
-                const int id = (int) ~(unsigned) (s.list[j] >> 32);
-                emit(id, weigh.logprob(key_of(score_at(x, id)), total), K);
-            }
-            before = after;
-        }
-        return true;
+        u64 t;
+        scan2(s, d0, sum, d1, t);
+        if (tid < C) cl.map_shared_rank(&s, tid)->all_mass[rank] = t;
+        cl.sync();
+        return sum8(lane < C ? s.all_mass[lane] : 0ull);
     };
-
-    // the CTAs' lists: how many words together, and all of them to the leading CTA's
-    auto collect_count = [&]() -> unsigned { return __reduce_add_sync(~0u, OF_CTAS(n_list, 0u)); };
-    auto collect = [&]() {
-        const unsigned c = OF_CTAS(n_list, 0u);
-        unsigned before = c;
-#pragma unroll
-        for (int d = 1; d < SM_MAX_CLUSTER; d <<= 1) {
-            const unsigned y = __shfl_up_sync(~0u, before, d);
-            if (lane >= d) before += y;
-        }
-        before -= c;
-        const int r = warp % SM_MAX_CLUSTER;   // two warps per CTA of the cluster
-        const unsigned at = __shfl_sync(~0u, before, r), n = __shfl_sync(~0u, c, r);
-        if (r > 0 && r < C) {
-            const SampleShared &o = *cl.map_shared_rank(&s, r);
-            for (unsigned i = (warp / SM_MAX_CLUSTER) * 32 + lane; i < n; i += SM_NT / SM_MAX_CLUSTER) s.list[at + i] = o.list[i];
-        }
-        __syncthreads();
-    };
-
-    u64 W0 = 0;              // the row's whole mass, where the short way has summed it
     if (lists) {
         if (by_m) {          // what w >= m can reach, downwards by more than the roundings on the way
             const double lo = (double) xmax + (double) temp * log(m);
             floor = max(key_of((float) (lo - 1e-6 * (fabs(lo) + fabs((double) xmax) + (double) temp))), KEY_NONE + 1);
         }
-        u64 sum = 0;
+        const float c2 = (float) (weigh.inv * 1.4426950408889634074);
+        float near = 0.0f;
         for (int o = 0; o < p.seg; o += SM_TILE) {
             const uint4 q = *(const uint4 *) (mine + o);
             if (max(max(q.x, q.y), max(q.z, q.w)) >= floor)
@@ -421,48 +546,131 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                     const uint32_t k = (&q.x)[e];
                     if (k >= floor) {
                         const unsigned at = atomicAdd(&s.n_list, 1u);
-                        if (at < SM_LIST) s.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
+                        if (at < SM_LIST) s.w[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
                     }
                 }
-            if (by_p) {   // the weight of -infinity is 0
-                const u64 w0 = weigh(q.x), w1 = weigh(q.y), w2 = weigh(q.z), w3 = weigh(q.w);
-                sum += (w0 + w1) + (w2 + w3);
+            if (by_p) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float y = __fmul_rn(__fadd_rn(value_of((&q.x)[i]), -xmax), c2);
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(y));
+                }
+                near = __fadd_rn(near, __fadd_rn(__fadd_rn(e[0], e[1]), __fadd_rn(e[2], e[3])));
             }
         }
+        double near_sum = (double) near;
         if (by_p) {
-            unsigned d0 = 0, d1;
-            u64 t;
-            scan2(s, d0, sum, d1, t);
-            if (tid == 0) s.part_mass = t;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) near_sum += __shfl_xor_sync(~0u, near_sum, d);
+            if (lane == 0) s.wm[warp] = (u64) __double_as_longlong(near_sum);
         }
+        __syncthreads();
+        if (by_p && warp == 0) {
+            double t = lane < SM_NW ? __longlong_as_double((long long) s.wm[lane]) : 0.0;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(~0u, t, d);
+            if (lane < C) cl.map_shared_rank(&s, lane)->all_near[rank] = t;   // to every CTA
+        }
+        push_list();
         cl.sync();
-        if (by_p) W0 = sum8(OF_CTAS(part_mass, 0ull));
-        const unsigned n = collect_count();
+        const double nearW = by_p ? sum8(lane < C ? s.all_near[lane] : 0.0) * SM_ONE : 0.0;
+        const int n = list_length();
+        if (!by_p && rank != 0 && n <= SM_LIST) return;   // nobody reads this CTA's shared memory any more
         if (n <= SM_LIST) {
-            if (rank == 0) collect();
             if (!by_p) {
-                cl.sync();   // the lists have been read
-                if (rank == 0) finish_list((int) n, 0);
+                weigh_list(n);
+                if (n <= SM_SHORT) {
+                    __syncthreads();
+                    const Place at = place(n);
+                    bool keep = at.in && (!use_k || at.rank < top_k);
+                    if (use_p) {
+                        if (at.in && at.rank == (use_k ? min(top_k, n) : n) - 1) s.total = at.after;
+                        __syncthreads();
+                        keep = keep && (at.rank == 0 || (double) at.before < pd * (double) s.total);
+                    }
+                    short_pick(n, keep);
+                    return;
+                }
+                u64 last = 0;   // the last word kept
+                if (use_k && n > top_k) {
+                    by_score(n, 0, [](int) { return 1ull; }, [&](u64 b, u64 e) { return b < (u64) top_k && e >= (u64) top_k; });
+                    last = s.found;
+                }
+                __syncthreads();
+                if (use_p) {
+                    unsigned d;
+                    const double lim = pd * (double) list_mass(n, last, false, d);
+                    by_score(n, 0, [&](int i) -> u64 { return s.list[i] >= last ? s.w[i] & ~PASS : 0; },
+                             [&](u64 b, u64 e) { return (double) b < lim && (double) e >= lim; });
+                    last = s.found;
+                    __syncthreads();
+                }
+                pick(n, last);
                 return;
             }
+            // 0: the nucleus ends below the list, 1: it ends in it, 2: where it ends depends on the mass's error
+            u64 last = 0, total = 0;
+            Place at = {};
+            const bool short_list = n <= SM_SHORT;
+            auto to_mass = [&](double lim) {
+                by_score(n, 0, whole_of, [&](u64 b, u64 e) { return (double) b < lim && (double) e >= lim; });
+                last = s.found;
+            };
+            auto tell = [&](unsigned v) {   // the leading CTA's thread 0, to every CTA
+                for (int r = 0; r < C; r++) cl.map_shared_rank(&s, r)->done = v;
+            };
+            auto before = [&](double lim) { return at.in && (at.rank == 0 || (double) at.before < lim); };
             if (rank == 0) {
-                const bool ok = finish_list((int) n, W0);
-                if (tid == 0) s.done = ok;
+                unsigned d;
+                weigh_list(n);
+                __syncthreads();
+                const double lo = pd * nearW * (1.0 - SM_MASS_ERR), hi = pd * nearW * (1.0 + SM_MASS_ERR);
+                bool sure;
+                if (short_list) {
+                    at = place(n);
+                    if (at.in && at.rank == n - 1) s.total = at.after;
+                    sure = !__syncthreads_or(before(lo) != before(hi));
+                    total = s.total;
+                    sure = sure && (double) total >= hi;
+                } else {
+                    total = list_mass(n, 0, false, d);
+                    to_mass(lo);
+                    sure = (double) s.found_after >= hi;
+                }
+                if (tid == 0) tell((double) total < lo ? 0 : sure ? 1 : 2);   // NaN: 2
             }
             cl.sync();
-            if (cl.map_shared_rank(&s, 0)->done) {
-                cl.sync();
+            const unsigned done = s.done;
+            auto finish = [&](double lim) {
+                if (short_list) short_pick(n, before(lim));
+                else pick(n, last);
+            };
+            if (done == 1) {
+                if (rank == 0) finish(pd * nearW);
                 return;
+            }
+            if (done == 2) {
+                const double lim = pd * (double) whole_mass();
+                if (rank == 0) {
+                    if (!short_list) to_mass(lim);
+                    if (tid == 0) tell((double) total >= lim);
+                }
+                cl.sync();
+                if (s.done) {
+                    if (rank == 0) finish(lim);
+                    return;
+                }
             }
         }
         cl.sync();
     }
 
     // ---- the long way ----
-    // the smallest key, and how many there are
-    if (use_k || use_p) {
-        uint32_t mn = ~0u;
-        unsigned nv = 0;
+    // for top-k the smallest key, and how many there are
+    uint32_t mn = ~0u;
+    unsigned nv = 0;
+    if (use_k) {
         for (int o = 0; o < p.seg; o += SM_TILE) {
             const uint4 q = *(const uint4 *) (mine + o);
 #pragma unroll
@@ -475,24 +683,50 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
         nv = __reduce_add_sync(~0u, nv);
         if (lane == 0) { atomicMin(&s.mn, mn); atomicAdd(&s.nvalid, nv); }
         cl.sync();
+        mn = __reduce_min_sync(~0u, OF_CTAS(mn, ~0u));
+        nv = __reduce_add_sync(~0u, OF_CTAS(nvalid, 0u));
     }
-    const uint32_t mn = __reduce_min_sync(~0u, OF_CTAS(mn, ~0u));
-    const unsigned nv = __reduce_add_sync(~0u, OF_CTAS(nvalid, 0u));
     // One search: the value T, and how many words c at T, at which the count reaches k (by_mass false) or the mass
     // reaches p of the total (true). Only keys above `over` count; `extra` more mass lies at `over` itself.
-    const float range = fminf(__fadd_rn(xmax, -value_of(mn)), 64.0f);
-    const float scale = range > 0.0f ? __fdiv_rn((float) SM_BINS, range) : 0.0f;
+    float scale = 0.0f;
+    auto bin0 = [&](uint32_t k) -> int {
+        if (k == mx) return 0;
+        return min(SM_BINS - 1, __float2int_rz(__fmul_rn(__fadd_rn(xmax, -value_of(k)), scale)));
+    };
+    // the list holds the last word kept: the one before which less than lim lies and with which lim is reached, of weights or
+    // (by_mass false) of words. T and c of it to every CTA
+    auto end_in_list = [&](int n, bool by_mass, u64 above, double lim, uint32_t &T, unsigned &c) {
+        if (rank == 0) {
+            weigh_list(n);
+            __syncthreads();
+            by_score(n, above, [&](int i) -> u64 { return by_mass ? s.w[i] & ~PASS : 1; },
+                     [&](u64 b, u64 e) { return (double) b < lim && (double) e >= lim; });
+            const u64 q = s.found;
+            unsigned mine = 0;
+            for (int i = tid; i < n; i += SM_NT) mine += s.list[i] >= q && s.list[i] >> 32 == q >> 32;
+            u64 d0 = 0, d1;
+            unsigned at;
+            scan2(s, mine, d0, at, d1);
+            if (tid < C) {   // to every CTA
+                SampleShared &o = *cl.map_shared_rank(&s, tid);
+                o.T = (uint32_t) (q >> 32);
+                o.c = at;
+            }
+        }
+        cl.sync();
+        T = s.T;
+        c = s.c;
+    };
     auto search = [&](bool by_mass, uint32_t over, u64 extra, uint32_t &T, unsigned &c) {
+        // the steps of level 0: down to the smallest score, or to where weights vanish; at most 64 (masked words of low values)
+        const float range = fminf(by_mass ? temp * (float) SM_FAR : __fadd_rn(xmax, -value_of(mn)), 64.0f);
+        scale = range > 0.0f ? fminf(__fdiv_rn((float) SM_BINS, range), 3e38f) : 0.0f;
         uint32_t klo = over + 1, khi = mx;        // keys still in question
         unsigned above = 0;                        // words, and mass, above khi
         u64 mass_above = 0;
         double lim = 0.0;
         int in_bin = -1;                           // level 0's bin the search is in
         for (int level = 0;; level++) {
-            auto bin0 = [&](uint32_t k) -> int {
-                if (k == mx) return 0;
-                return min(SM_BINS - 1, __float2int_rz(__fmul_rn(__fadd_rn(xmax, -value_of(k)), scale)));
-            };
             const u64 width = ((u64) khi - klo) / SM_BINS + 1;   // keys per bin from level 1 on
             auto bin_of = [&](uint32_t k) -> int {               // -1: not in question
                 if (k < klo || k > khi) return -1;
@@ -500,7 +734,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 return bin0(k) == in_bin ? (int) ((khi - k) / (uint32_t) width) : -1;
             };
             for (int b = tid; b < SM_BINS; b += SM_NT) s.cnt[b] = s.mass[b][0] = s.mass[b][1] = 0;
-            if (tid == 0) { s.bin = -1; s.lo = ~0u; s.hi = 0; s.n_list = 0; }
+            if (tid == 0) { s.bin = -1; s.lo = ~0u; s.hi = 0; s.n_list = s.n_all = 0; }
             __syncthreads();
             for (int o = 0; o < p.seg; o += SM_TILE) {
                 const uint4 q = *(const uint4 *) (mine + o);
@@ -513,12 +747,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                     const int b = bin_of((&q.x)[e]);
                     if (b < 0) continue;
                     atomicAdd(&s.cnt[b], 1u);
-                    if (by_mass) {   // 64-bit addition by halves: the carry is what the low half's old value shows
-                        const u64 w = wv[e];
-                        const unsigned wl = (unsigned) w, old = atomicAdd(&s.mass[b][0], wl);
-                        const unsigned wh = (unsigned) (w >> 32) + (old + wl < old);
-                        if (wh) atomicAdd(&s.mass[b][1], wh);
-                    }
+                    if (by_mass) add64(s.mass[b], wv[e]);
                 }
             }
             cl.sync();
@@ -587,49 +816,20 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                     if (bin_of(k) != bin) continue;
                     if (fits) {
                         const unsigned at = atomicAdd(&s.n_list, 1u);
-                        if (at < SM_LIST) s.list[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
+                        if (at < SM_LIST) s.w[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
                     } else {
                         atomicMin(&s.lo, k);
                         atomicMax(&s.hi, k);
                     }
                 }
             }
-            cl.sync();
             if (fits) {
-                if (rank == 0) {
-                    const unsigned n = collect_count();
-                    collect();
-                    sort_desc(s.list, (int) n);
-                    u64 wv[2] = { 0, 0 };
-                    unsigned dc = 0, dt;
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-                        if (by_mass && 2 * tid + e < (int) n) wv[e] = weigh((uint32_t) (s.list[2 * tid + e] >> 32));
-                    u64 bm = wv[0] + wv[1], bt;
-                    scan2(s, dc, bm, dt, bt);
-                    bm += mass_above;
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {   // the last word kept: T is its value, c its place among those of T
-                        const int j = 2 * tid + e;
-                        const bool lastk = by_mass ? j < (int) n && (double) bm < lim && ((double) (bm + wv[e]) >= lim || j + 1 == (int) n)
-                                                   : j == top_k - 1 - (int) above;
-                        if (lastk) {
-                            const uint32_t key = (uint32_t) (s.list[j] >> 32);
-                            int f = j;
-                            while (f > 0 && (uint32_t) (s.list[f - 1] >> 32) == key) f--;
-                            s.T = key;
-                            s.c = j - f + 1;
-                        }
-                        bm += wv[e];
-                    }
-                }
+                push_list();
                 cl.sync();
-                const SampleShared &lead = *cl.map_shared_rank(&s, 0);
-                T = lead.T;
-                c = lead.c;
-                cl.sync();
+                end_in_list((int) nb, by_mass, by_mass ? mass_above : above, by_mass ? lim : (double) top_k, T, c);
                 return;
             }
+            cl.sync();
             if (level == 0) in_bin = bin;
             klo = __reduce_min_sync(~0u, OF_CTAS(lo, ~0u));
             khi = __reduce_max_sync(~0u, OF_CTAS(hi, 0u));
@@ -690,20 +890,27 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     scan2(s, tb, sb, tt, st);
     tb = __shfl_sync(~0u, tb, 0);
     sb = __shfl_sync(~0u, sb, 0);
-    if (tid == 0) { s.part_cnt = tt; s.part_mass = st; s.part_kept = 0; s.bin = -1; }
+    if (tid == 0) { s.part_kept = 0; s.bin = -1; }
     __syncthreads();
     if (lane == 0) atomicAdd(&s.part_kept, cnt);
+    __syncthreads();
+    if (tid < C) {
+        SampleShared &o = *cl.map_shared_rank(&s, tid);
+        o.all_cnt[rank] = tt;
+        o.all_sum[rank] = st;
+        o.all_kept[rank] = s.part_kept;
+    }
     cl.sync();
-    const unsigned rt = OF_CTAS(part_cnt, 0u);
-    const u64 rm = OF_CTAS(part_mass, 0ull);
-    const unsigned all_ties = __reduce_add_sync(~0u, rt), all_cnt = __reduce_add_sync(~0u, OF_CTAS(part_kept, 0u));
+    const unsigned rt = lane < C ? s.all_cnt[lane] : 0u;
+    const u64 rm = lane < C ? s.all_sum[lane] : 0ull;
+    const unsigned all_ties = __reduce_add_sync(~0u, rt), all_cnt = __reduce_add_sync(~0u, lane < C ? s.all_kept[lane] : 0u);
     const u64 all = sum8(rm);
     tb += __reduce_add_sync(~0u, lane < rank ? rt : 0u);
     sb += sum8(lane < rank ? rm : 0ull);
     const unsigned ct = tie_in ? min(c, all_ties) : 0;
-    const u64 W = all + ct * wT;
+    const u64 kept_mass = all + ct * wT;
     const int kept = (int) (all_cnt + ct);
-    const double target = (double) u * (double) W;
+    const double target = (double) u * (double) kept_mass;
     auto mass_at = [&](u64 sum_, unsigned ties_) { return sum_ + min(ties_, ct) * wT; };
     // the warp whose share the target falls in is found; all warps of its CTA take its tiles, then one the tile's words
     if (lane == 0 && (double) mass_at(sb, tb) <= target && (double) mass_at(sb + sum, tb + ties) > target) {
@@ -740,7 +947,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                     const unsigned at = bt + (ties_count && k == T);
                     const u64 after = b + w[e];
                     if ((double) mass_at(b, bt) <= target && (double) mass_at(after, at) > target)
-                        emit(base + cross * p.seg + 4 * lane + o + e, weigh.logprob(k, W), kept);
+                        emit(base + cross * p.seg + 4 * lane + o + e, weigh.logprob(k, kept_mass), kept);
                     b = after;
                     bt = at;
                 }
@@ -748,7 +955,6 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             t0 += tc;
         }
     }
-    cl.sync();
 }
 
 size_t sample_smem(int slice) { return (sizeof(SampleShared) + 15) / 16 * 16 + (size_t) slice * 4; }
