@@ -44,7 +44,6 @@ constexpr int SM_TILE = 128;             // words of a warp's load: four per lan
 constexpr int SM_MAX_CLUSTER = 8;
 constexpr int SM_SLICE = 32768;          // words a CTA holds at most
 constexpr double SM_ONE = 17592186044416.0;   // 2^44
-constexpr double SM_FAR = 31.2;          // exp(-31.2) < 2^-45: such a word's weight rounds to 0
 static_assert((long long) SM_SLICE * SM_MAX_CLUSTER >= IMI_CUDA_SAMPLE_VOCAB, "a row fits a cluster");
 static_assert((long long) IMI_CUDA_SAMPLE_VOCAB <= 1 << 18, "the weights' sum fits 62 bits");
 
@@ -80,6 +79,7 @@ struct SampleShared {
             u64 list_[SM_LIST];
             unsigned steps[SM_STEPS];        // the threads' maxima ranked
         };
+        unsigned queue[SM_NW][64];           // the warps' kept words
     };
     unsigned wc[SM_NW];               // scans over the CTA
     u64 wm[SM_NW];
@@ -91,7 +91,7 @@ struct SampleShared {
     u64 all_mass[SM_MAX_CLUSTER], all_sum[SM_MAX_CLUSTER];
     u64 mass_above;
     int bin;                          // found in a scan: the crossing bin, and what lies above it
-    unsigned above, in_bin;
+    unsigned above;
     unsigned T, c, done;              // the leading CTA's findings
     u64 found, found_after;           // a search in the list
     u64 total;
@@ -126,39 +126,47 @@ __device__ __forceinline__ void scan2(SampleShared &s, unsigned &c, u64 &m, unsi
     m = bm + xm - m;
 }
 
-// A word's weight, as a number and as an integer of 2^-44. With n the nearest integer to -z / ln 2, exp(-z) = 2^n exp(r),
-// |r| <= ln2 / 2; exp(r) by the polynomial through its values at 11 Chebyshev nodes (relative error below 2^-51). A table
-// and a shorter polynomial took twice as long: 32 lanes' reads of it fall on a few banks.
+// A word's weight, as a number and as an integer of 2^-44. With y = -z log2 e and n the nearest integer to it, exp(-z) = 2^n 2^r,
+// |r| <= 1/2; 2^r by the polynomial through its values at 11 Chebyshev nodes (relative error below 2^-51). A table and a
+// shorter polynomial took twice as long: 32 lanes' reads of it fall on a few banks. What bounds a pass of this over a row is the
+// 15 operations in 64 bits (two cycles of a scheduler each).
 struct Weigher {
-    double xmax;
+    double xmax, c;    // the largest score; log2(e) / temperature
+    float low;         // scores further down than this weigh 0; they are raised to it
     uint32_t kmax;
-    double inv;   // 1 / temperature
-    __device__ __forceinline__ double real(uint32_t k) const {   // no branches: several words are in flight at once
-        const double z = (xmax - (double) value_of(k)) * inv;
+    bool odd;          // an infinite largest score, temperatures out of all proportion, a min-p below the weights' resolution
+    __device__ __forceinline__ double real(float x) const {   // no branches: several words are in flight at once
         constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: adding it leaves the nearest integer in the low bits
-        const double b = __fma_rn(z, -1.4426950408889634074, MAGIC);
-        const double r = __fma_rn(__dadd_rn(b, -MAGIC), -0.69314718055994530942, -z);
-        double e = __fma_rn(r, 2.7626357241447223e-07, 2.764018079620985e-06);
-        e = __fma_rn(r, e, 2.4801504346997686e-05);
-        e = __fma_rn(r, e, 0.00019841170270440067);
-        e = __fma_rn(r, e, 0.0013888888932488599);
-        e = __fma_rn(r, e, 0.008333333385667782);
-        e = __fma_rn(r, e, 0.04166666666657314);
-        e = __fma_rn(r, e, 0.16666666666554406);
-        e = __fma_rn(r, e, 0.5000000000000006);
-        e = __fma_rn(r, e, 1.0000000000000067);
+        const double d = (double) fmaxf(x, low) - xmax, b = __fma_rn(d, c, MAGIC);
+        const double r = __fma_rn(d, c, -__dadd_rn(b, -MAGIC));
+        double e = __fma_rn(r, 7.072585949269224e-09, 1.0208690299958306e-07);
+        e = __fma_rn(r, e, 1.321544258792169e-06);
+        e = __fma_rn(r, e, 1.5252657260200837e-05);
+        e = __fma_rn(r, e, 0.0001540353044173605);
+        e = __fma_rn(r, e, 0.0013333558230164974);
+        e = __fma_rn(r, e, 0.009618129107606888);
+        e = __fma_rn(r, e, 0.05550410866444772);
+        e = __fma_rn(r, e, 0.24022650695910097);
+        e = __fma_rn(r, e, 0.69314718055995);
         e = __fma_rn(r, e, 1.0);
-        e = __hiloint2double(__double2hiint(e) + __double2loint(b) * (1 << 20), __double2loint(e));
-        return k == kmax ? 1.0 : z < SM_FAR ? e : 0.0;   // z NaN or infinite (infinities): 0
+        return __hiloint2double(__double2hiint(e) + __double2loint(b) * (1 << 20), __double2loint(e));
     }
-    static __device__ __forceinline__ u64 whole(double w) {
-        // w * 2^44 <= 2^44: added to 2^52 its integer part, rounded to nearest, is the low mantissa
-        return (u64) __double_as_longlong(__fma_rn(w, SM_ONE, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    __device__ __noinline__ double rare(uint32_t k) const {
+        if (k == kmax) return 1.0;
+        const double z = (xmax - (double) value_of(k)) * (c * 0.69314718055994530942);
+        return k > KEY_NONE && z >= 0.0 ? exp(-z) : 0.0;   // z NaN: below an infinite score
     }
+    __device__ __forceinline__ double real(uint32_t k) const { return odd ? rare(k) : real(value_of(k)); }
+    // w * 2^44 <= 2^44: added to 2^52 its integer part, rounded to nearest, is the low mantissa. raw: with the exponent's bits
+    // still in place, which sums of n words hold n times (as 64 bits go)
+    static constexpr u64 RAW = 0x4330000000000000ull;
+    static __device__ __forceinline__ u64 raw(double w) { return (u64) __double_as_longlong(__fma_rn(w, SM_ONE, 4503599627370496.0)); }
+    static __device__ __forceinline__ u64 whole(double w) { return raw(w) - RAW; }
     __device__ __forceinline__ u64 operator()(uint32_t k) const { return whole(real(k)); }
+    __device__ __forceinline__ u64 raw4(uint4 q) const { return (raw(real(q.x)) + raw(real(q.y))) + (raw(real(q.z)) + raw(real(q.w))); }
     __device__ __forceinline__ float logprob(uint32_t k, u64 total) const {
-        const double z = k == kmax ? 0.0 : (xmax - (double) value_of(k)) * inv;
-        return (float) (-z - log((double) total / SM_ONE));
+        const double d = k == kmax ? 0.0 : ((double) value_of(k) - xmax) * c * 0.69314718055994530942;
+        return (float) (d - log((double) total / SM_ONE));
     }
 };
 
@@ -231,17 +239,8 @@ __device__ __forceinline__ float score_at(const S *x, int i) {
     else return __bfloat162float(x[i]);
 }
 
-template <typename S>
-__device__ __forceinline__ void load4(const S *x, float (&f)[4]) {
-    if constexpr (sizeof(S) == 4) {
-        const float4 v = __ldg((const float4 *) x);
-        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-    } else {
-        const uint2 v = __ldg((const uint2 *) x);
-#pragma unroll
-        for (int e = 0; e < 4; e++) f[e] = score_at((const S *) &v, e);
-    }
-}
+template <typename S> struct Four { typedef uint2 T; };   // four scores
+template <> struct Four<float> { typedef uint4 T; };
 
 // a value of every CTA of the cluster: lane r holds CTA r's (other lanes `none`), read at once
 #define OF_CTAS(field, none) (lane < C ? cl.map_shared_rank(&s, lane)->field : (none))
@@ -292,35 +291,26 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     const int inside = a.vocab - (base + warp * p.seg);     // words of the row in this warp's part
     const int whole = vec ? max(0, min(p.seg, inside / SM_TILE * SM_TILE)) : 0;
     int o = 0;
-    if constexpr (sizeof(S) == 4) {
-        for (; o + 4 * SM_TILE <= whole; o += 4 * SM_TILE) {   // four tiles' loads in flight
-            float f[4][4];
+    constexpr int BATCH = sizeof(S) == 4 ? 4 : 6;           // tiles' loads in flight
+    for (; o + BATCH * SM_TILE <= whole; o += BATCH * SM_TILE) {
+        typename Four<S>::T v[BATCH];
 #pragma unroll
-            for (int t = 0; t < 4; t++) load4(x + first + o + t * SM_TILE, f[t]);
+        for (int t = 0; t < BATCH; t++) v[t] = __ldg((const typename Four<S>::T *) (x + first + o + t * SM_TILE));
 #pragma unroll
-            for (int t = 0; t < 4; t++) put(o + t * SM_TILE, f[t]);
-        }
-    } else if (((uintptr_t) (x + base) & 15) == 0) {           // 16 bytes per lane, two tiles at once; which lane has a word
-        for (; o + 8 * SM_TILE <= whole; o += 8 * SM_TILE) {   // does not matter to what follows
-            uint4 v[4];
-            const S *at = x + first + 4 * lane + o;
+        for (int t = 0; t < BATCH; t++) {
+            float f[4];
 #pragma unroll
-            for (int t = 0; t < 4; t++) v[t] = __ldg((const uint4 *) (at + t * 2 * SM_TILE));
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float f[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) f[e] = score_at((const S *) &v[t], 4 * h + e);
-                    put(o + t * 2 * SM_TILE + 4 * lane + 4 * h, f);
-                }
+            for (int e = 0; e < 4; e++) f[e] = score_at((const S *) &v[t], e);
+            put(o + t * SM_TILE, f);
         }
     }
     for (; o < p.seg; o += SM_TILE) {
         float f[4];
-        if (o < whole) load4(x + first + o, f);
-        else
+        if (o < whole) {
+            const typename Four<S>::T v = __ldg((const typename Four<S>::T *) (x + first + o));
+#pragma unroll
+            for (int e = 0; e < 4; e++) f[e] = score_at((const S *) &v, e);
+        } else
 #pragma unroll
             for (int e = 0; e < 4; e++) f[e] = first + o + e < a.vocab ? score_at(x, first + o + e) : -INFINITY;
         put(o, f);
@@ -397,7 +387,9 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
         if (rank == 0 && tid == 0) emit((int) s.idmin, 0.0f, 1);
         return;
     }
-    const Weigher weigh = { (double) xmax, mx, 1.0 / (double) temp };
+    // 32.5 temperatures down a weight is below 2^-46, and rounds to 0
+    const Weigher weigh = { (double) xmax, 1.4426950408889634074 / (double) temp, __fmaf_rn(-32.5f, temp, xmax), mx,
+                            !(temp >= fabsf(xmax) * 0x1p-16f && temp > 1e-30f && temp < 1e30f) || (use_m && m < 1e-12) };
 
     // searches in the leading CTA's list
     constexpr u64 PASS = 1ull << 63;   // with a weight: the word passes min-p
@@ -521,9 +513,9 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
         u64 sum = 0;
         for (int o = 0; o < p.seg; o += SM_TILE) {
             const uint4 q = *(const uint4 *) (mine + o);
-            const u64 w0 = weigh(q.x), w1 = weigh(q.y), w2 = weigh(q.z), w3 = weigh(q.w);   // the weight of -infinity is 0
-            sum += (w0 + w1) + (w2 + w3);
+            sum += weigh.raw4(q);   // the weight of -infinity is 0
         }
+        sum -= (u64) (p.seg / 32) * Weigher::RAW;
         unsigned d0 = 0, d1;
         u64 t;
         scan2(s, d0, sum, d1, t);
@@ -536,7 +528,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             const double lo = (double) xmax + (double) temp * log(m);
             floor = max(key_of((float) (lo - 1e-6 * (fabs(lo) + fabs((double) xmax) + (double) temp))), KEY_NONE + 1);
         }
-        const float c2 = (float) (weigh.inv * 1.4426950408889634074);
+        const float c2 = (float) weigh.c;
         float near = 0.0f;
         for (int o = 0; o < p.seg; o += SM_TILE) {
             const uint4 q = *(const uint4 *) (mine + o);
@@ -689,9 +681,9 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     // One search: the value T, and how many words c at T, at which the count reaches k (by_mass false) or the mass
     // reaches p of the total (true). Only keys above `over` count; `extra` more mass lies at `over` itself.
     float scale = 0.0f;
-    auto bin0 = [&](uint32_t k) -> int {
-        if (k == mx) return 0;
-        return min(SM_BINS - 1, __float2int_rz(__fmul_rn(__fadd_rn(xmax, -value_of(k)), scale)));
+    auto bin0 = [&](uint32_t k) -> int {   // rounded by an addition: the conversion unit is slow. The largest, infinite too: 0
+        const float y = fminf(fmaxf(__fmul_rn(__fadd_rn(xmax, -value_of(k)), scale), 0.0f), (float) (SM_BINS - 1));
+        return (int) (__float_as_uint(__fadd_rn(y, 8388608.0f)) & (SM_BINS - 1));
     };
     // the list holds the last word kept: the one before which less than lim lies and with which lim is reached, of weights or
     // (by_mass false) of words. T and c of it to every CTA
@@ -719,7 +711,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     };
     auto search = [&](bool by_mass, uint32_t over, u64 extra, uint32_t &T, unsigned &c) {
         // the steps of level 0: down to the smallest score, or to where weights vanish; at most 64 (masked words of low values)
-        const float range = fminf(by_mass ? temp * (float) SM_FAR : __fadd_rn(xmax, -value_of(mn)), 64.0f);
+        const float range = fminf(by_mass ? temp * 31.2f : __fadd_rn(xmax, -value_of(mn)), 64.0f);
         scale = range > 0.0f ? fminf(__fdiv_rn((float) SM_BINS, range), 3e38f) : 0.0f;
         uint32_t klo = over + 1, khi = mx;        // keys still in question
         unsigned above = 0;                        // words, and mass, above khi
@@ -746,8 +738,8 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 for (int e = 0; e < 4; e++) {
                     const int b = bin_of((&q.x)[e]);
                     if (b < 0) continue;
-                    atomicAdd(&s.cnt[b], 1u);
                     if (by_mass) add64(s.mass[b], wv[e]);
+                    else atomicAdd(&s.cnt[b], 1u);
                 }
             }
             cl.sync();
@@ -758,10 +750,11 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             for (int r = 0; r < SM_MAX_CLUSTER; r++)
                 if (r < C) {
                     const SampleShared &o = *cl.map_shared_rank(&s, r);
-                    const uint2 v = *(const uint2 *) &o.cnt[2 * tid];
-                    cn[0] += v.x;
-                    cn[1] += v.y;
-                    if (by_mass) {
+                    if (!by_mass) {
+                        const uint2 v = *(const uint2 *) &o.cnt[2 * tid];
+                        cn[0] += v.x;
+                        cn[1] += v.y;
+                    } else {
                         const uint4 w = *(const uint4 *) &o.mass[2 * tid][0];
                         ms[0] += (u64) w.y << 32 | w.x;
                         ms[1] += (u64) w.w << 32 | w.z;
@@ -781,7 +774,6 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                     s.bin = 2 * tid + e;
                     s.above = ca;
                     s.mass_above = ma;
-                    s.in_bin = cn[e];
                 }
                 c0 += cn[e];
                 m0 += ms[e];
@@ -797,38 +789,43 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             }
             above = s.above;
             mass_above = s.mass_above;
-            const unsigned nb = s.in_bin;
             if (level > 0 && width == 1) {   // one value
                 T = khi - bin;
                 if (by_mass) c = (unsigned) fmax(1.0, ceil((lim - (double) mass_above) / (double) weigh(T)));
                 else c = top_k - above;
-                c = min(c, nb);
                 cl.sync();
                 return;
             }
-            // the bin's words to a list; their range where they are too many
-            const bool fits = nb <= SM_LIST;
+            // the bin's words to a list
             for (int o = 0; o < p.seg; o += SM_TILE) {
                 const uint4 q = *(const uint4 *) (mine + o);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t k = (&q.x)[e];
                     if (bin_of(k) != bin) continue;
-                    if (fits) {
-                        const unsigned at = atomicAdd(&s.n_list, 1u);
-                        if (at < SM_LIST) s.w[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
-                    } else {
-                        atomicMin(&s.lo, k);
-                        atomicMax(&s.hi, k);
-                    }
+                    const unsigned at = atomicAdd(&s.n_list, 1u);
+                    if (at < SM_LIST) s.w[at] = ((u64) k << 32) | (uint32_t) ~(uint32_t) (first + o + e);
                 }
             }
-            if (fits) {
-                push_list();
-                cl.sync();
-                end_in_list((int) nb, by_mass, by_mass ? mass_above : above, by_mass ? lim : (double) top_k, T, c);
+            push_list();
+            cl.sync();
+            const int nb = list_length();
+            if (nb <= SM_LIST) {
+                end_in_list(nb, by_mass, by_mass ? mass_above : above, by_mass ? lim : (double) top_k, T, c);
                 return;
             }
+            uint32_t l = ~0u, h = 0;   // too many: their range
+            for (int o = 0; o < p.seg; o += SM_TILE) {
+                const uint4 q = *(const uint4 *) (mine + o);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t k = (&q.x)[e];
+                    if (bin_of(k) == bin) { l = min(l, k); h = max(h, k); }
+                }
+            }
+            l = __reduce_min_sync(~0u, l);
+            h = __reduce_max_sync(~0u, h);
+            if (lane == 0) { atomicMin(&s.lo, l); atomicMax(&s.hi, h); }
             cl.sync();
             if (level == 0) in_bin = bin;
             klo = __reduce_min_sync(~0u, OF_CTAS(lo, ~0u));
@@ -858,11 +855,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     const bool ties_count = T > KEY_NONE;
     // the kept words above T among four: their weights (else 0), how many; and how many words at T
     auto take = [&](const uint4 &q, u64 (&w)[4], unsigned &kept, unsigned &at) {
-        w[0] = w[1] = w[2] = w[3] = 0;
         kept = at = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) at += ties_count && (&q.x)[e] == T;
-        if (max(max(q.x, q.y), max(q.z, q.w)) <= T) return;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const uint32_t k = (&q.x)[e];
@@ -870,15 +863,50 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             const bool in = k > T && (!use_m || k == mx || r >= m);
             w[e] = in ? Weigher::whole(r) : 0;
             kept += in;
+            at += ties_count && k == T;
         }
     };
-    for (int o = 0; o < p.seg; o += SM_TILE) {
-        u64 w[4];
-        unsigned kept, at;
-        take(*(const uint4 *) (mine + o), w, kept, at);
-        sum += (w[0] + w[1]) + (w[2] + w[3]);
-        cnt += kept;
-        ties += at;
+    if (!ties_count && !use_m) {   // no filter
+        for (int o = 0; o < p.seg; o += SM_TILE) {
+            const uint4 q = *(const uint4 *) (mine + o);
+            sum += weigh.raw4(q);
+            cnt += (q.x > KEY_NONE) + (q.y > KEY_NONE) + (q.z > KEY_NONE) + (q.w > KEY_NONE);
+        }
+        sum -= (u64) (p.seg / 32) * Weigher::RAW;
+    } else {
+        // the words above T are few: each warp queues them, and weighs 32 at once
+        uint32_t *queue = s.queue[warp];
+        int n = 0;
+        __syncthreads();   // the lists in this memory are done with
+        auto flush = [&](int have) {
+            __syncwarp();
+            const uint32_t k = lane < have ? queue[lane] : KEY_NONE;
+            const double r = weigh.real(k);
+            const bool in = k > KEY_NONE && (!use_m || k == mx || r >= m);
+            sum += in ? Weigher::whole(r) : 0;
+            cnt += in;
+            const uint32_t rest = queue[32 + lane];
+            __syncwarp();
+            queue[lane] = rest;
+            __syncwarp();
+        };
+        for (int o = 0; o < p.seg; o += SM_TILE) {
+            const uint4 q = *(const uint4 *) (mine + o);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t k = (&q.x)[e];
+                ties += ties_count && k == T;
+                const unsigned in = __ballot_sync(~0u, k > T);
+                if (!in) continue;
+                if (k > T) queue[n + __popc(in & ((1u << lane) - 1))] = k;
+                n += __popc(in);
+                if (n >= 32) {
+                    flush(32);
+                    n -= 32;
+                }
+            }
+        }
+        flush(n);
     }
     ties = __reduce_add_sync(~0u, ties);
     cnt = __reduce_add_sync(~0u, cnt);

@@ -442,6 +442,12 @@ def test_sample_masked_infinite_and_nan():
     for f in FILTERS[:8] + [dict(t=0.0), dict(t=1e-30), dict(t=1e30)]:
         for u in (0.0, 0.4, 0.9999):
             run_sample(x, u, **f)
+    y = scores(3, 5000, "f32", 9)
+    for t in (1e-7, 1e-4, 3e-3, 1e5, 3e30, inf):                 # from the greedy pick to equal shares
+        run_sample(y, [0.0, 0.5, 0.999], t=t)
+        run_sample(y, [0.0, 0.5, 0.999], t=t, p=0.7)
+    for m in (1e-11, 1e-14, 1e-20):                              # below the weights' resolution: kept words count
+        run_sample(y, 0.3, m=m, t=0.2)
     big = torch.full((3, 50000), low, device="cuda")             # nearly all masked by the lowest value
     big[:, 40000:40030] = torch.randn((3, 30), device="cuda")
     for f in FILTERS:
