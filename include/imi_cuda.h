@@ -255,7 +255,8 @@ enum {
     IMI_DEV_TABLE = 2,   /* a request longer than its block table's row holds */
     IMI_DEV_CAP = 3,     /* the step's new positions exceed the slot arrays */
     IMI_DEV_POOL = 4,    /* not enough free pages (or a free count outside the list) */
-    IMI_DEV_LENGTH = 5   /* a negative number of new positions */
+    IMI_DEV_LENGTH = 5,  /* a negative number of new positions */
+    IMI_DEV_WAIT = 6     /* a bounded device-side wait gave up (the call's outputs are not usable) */
 };
 
 /* Block tables and slot maps from the requests' lengths.

@@ -36,6 +36,10 @@ struct PaArgs {
     float2 *pml;                // then own slots (off[row] + piece) * n_head + head; (m, l) per slot
     int own_slot0;              // the first own slot
     int *off;                   // own pieces in front of each row [rows + 1]
+    // the prompt on the 5th-generation tensor cores (k_pa_mma): units of PM_ROWS query rows of a kv head, `tiles` position
+    // tiles each, in one line cut every `per` tiles; pair: both streams of a CTA on one row tile
+    bool mma, pair;
+    int tiles, per, rtiles;
 };
 
 template <typename T> struct Half2;
@@ -414,7 +418,7 @@ __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     return chunk;
 }
 
-// the pieces: CTA items 0..pre_items-1 are (piece, row tile, kv head) of the prompt, then (piece, kv head) of own positions
+// the pieces: (piece, row tile, kv head) of the prompt or, OWN, (piece, kv head) of the conversations' own positions
 template <typename T, int D, bool R8, bool OWN>
 __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_pieces(const __grid_constant__ PaArgs p) {
     constexpr int ROWS = R8 ? 8 : 16;
@@ -423,7 +427,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_pieces(const __grid_consta
     const imi_cuda_prefix_attn_args &a = p.a;
     float *sh = shf;
     int *off = (int *) (shf + PA_WARPS * ROWS * (D + 4));
-    pdl_wait();
+    // own pieces behind a launch for the prompt: that launch has let them start when all of its CTAs had done their own wait,
+    // and shares nothing with them; they wait for it at their end, so that k_join, which waits for them, has both
+    const bool early = OWN && a.prefix_len > 0;
+    if (!early) pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2;
     const long long ps = (long long) a.n_head_kv * a.page * D;
@@ -496,8 +503,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_pieces(const __grid_consta
             if (c == 0) p.pml[slot] = make_float2(m, l);
         });
     }
-    if (OWN) pdl_wait();
+    if (early) pdl_wait();
 }
+
+#include "serve_mma.cuh"
 
 // out and lse of every (row, head) from its pieces: one warp each
 template <int D>
@@ -510,9 +519,14 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p) 
     if (x >= (long long) a.rows * a.n_head) return;
     const int i = (int) (x / a.n_head), h = (int) (x % a.n_head);
     if (a.length[i] < 0) return;
-    const int o0 = p.off[i], on = p.off[i + 1] - o0, n = p.pre_splits + on;
+    int np = p.pre_splits;   // the prompt's pieces of this row
+    if (p.mma) {
+        const long long u0 = (long long) (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.tiles;
+        np = (int) (((u0 + p.tiles - 1) / p.per - u0 / p.per + 1) * (p.pair ? 2 : 1));
+    }
+    const int o0 = p.off[i], on = p.off[i + 1] - o0, n = np + on;
     auto slot_of = [&](int k) -> long long {
-        return k < p.pre_splits ? x * p.pre_splits + k : p.own_slot0 + (long long) (o0 + k - p.pre_splits) * a.n_head + h;
+        return k < np ? x * p.pre_splits + k : p.own_slot0 + (long long) (o0 + k - np) * a.n_head + h;
     };
     float m = -INFINITY;
     for (int k = lane; k < n; k += 32) m = fmaxf(m, p.pml[slot_of(k)].x);
@@ -544,16 +558,28 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p) 
 // ---- host ----
 // how a call is cut: pieces of the prompt, slots of the workspace
 struct PaPlan {
-    int splits, len;
+    int splits, len;        // pieces of a query row over the prompt at most; positions of a piece (k_pa_pieces)
+    bool mma, pair;
+    int tiles, per, rtiles, grid;
     size_t pre_slots, own_slots;
     size_t off_bytes, bytes;
 };
 PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len) {
     PaPlan p = {};
     const int g = n_head / n_head_kv, R = 16, tiles = (rows * g + R - 1) / R;
+    p.mma = rows * g > PM_MIN_ROWS && prefix_len > 0;
+    if (p.mma) {
+        p.pair = rows * g <= PM_M;
+        p.rtiles = p.pair ? 1 : (rows * g + PM_ROWS - 1) / PM_ROWS;
+        p.tiles = (prefix_len + PM_N - 1) / PM_N;
+        const long long total = (long long) p.rtiles * n_head_kv * p.tiles;
+        p.per = (int) std::max<long long>(PM_MIN_TILES, std::min<long long>(PM_MAX_TILES, (total + 147) / 148));
+        p.grid = (int) ((total + p.per - 1) / p.per);
+        p.splits = ((p.tiles + p.per - 1) / p.per + 1) * (p.pair ? 2 : 1);
+    }
     const int steps = (prefix_len + PA_STEP - 1) / PA_STEP;
-    p.splits = prefix_len ? std::max(1, std::min(PA_PRE_ITEMS / std::max(1, tiles * n_head_kv), steps / PA_MIN_STEPS)) : 0;
-    if (p.splits) {
+    if (!p.mma) p.splits = prefix_len ? std::max(1, std::min(PA_PRE_ITEMS / std::max(1, tiles * n_head_kv), steps / PA_MIN_STEPS)) : 0;
+    if (p.splits && !p.mma) {
         p.len = (steps + p.splits - 1) / p.splits * PA_STEP;
         p.splits = (prefix_len + p.len - 1) / p.len;
     }
@@ -580,7 +606,9 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
         return launch_pdl((const void *) k_pa_direct<T, D, R8>, dim3(a.rows * a.n_head_kv), PA_DWARPS * 32,
                           (size_t) PA_DWARPS * ROWS * (D + 4) * 4, st, args);
     cudaError_t r = cudaSuccess;
-    if (pl.splits) {
+    if (pl.mma) {
+        r = launch_pdl((const void *) k_pa_mma<T, D>, dim3(pl.grid), PM_THREADS, PmSmem<D>::TOTAL + 1024, st, args);
+    } else if (pl.splits) {
         const int items = (a.rows * p.g + 15) / 16 * a.n_head_kv * pl.splits;
         r = launch_pdl((const void *) k_pa_pieces<T, D, false, false>, dim3(std::min(items, 148 * 16)), PA_WARPS * 32,
                        (size_t) PA_WARPS * 16 * (D + 4) * 4, st, args);
@@ -600,14 +628,16 @@ cudaError_t launch_pa_t(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
 }
 template <typename T>
 cudaError_t raise_pa(int device) {
-    static SmemLimit lim;
+    static SmemLimit lim, lim2;
     return lim.raise(device,
                      { (const void *) k_pa_direct<T, 64, true>, (const void *) k_pa_direct<T, 64, false>,
                        (const void *) k_pa_direct<T, 128, true>, (const void *) k_pa_direct<T, 128, false>,
                        (const void *) k_pa_pieces<T, 64, false, false>, (const void *) k_pa_pieces<T, 128, false, false>,
                        (const void *) k_pa_pieces<T, 64, true, true>, (const void *) k_pa_pieces<T, 64, false, true>,
                        (const void *) k_pa_pieces<T, 128, true, true>, (const void *) k_pa_pieces<T, 128, false, true> },
-                     96 * 1024);
+                     96 * 1024) == cudaSuccess
+               ? lim2.raise(device, { (const void *) k_pa_mma<T, 64>, (const void *) k_pa_mma<T, 128> }, (int) std::max(PmSmem<64>::TOTAL, PmSmem<128>::TOTAL) + 1024)
+               : cudaErrorUnknown;
 }
 
 }  // namespace
@@ -656,6 +686,11 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
     p.sl2 = a->scale * 1.44269504088896340736f;
     p.pre_splits = pl.splits;
     p.pre_len = pl.len;
+    p.mma = pl.mma;
+    p.pair = pl.pair;
+    p.tiles = pl.tiles;
+    p.per = pl.per;
+    p.rtiles = pl.rtiles;
     p.off = (int *) a->work;
     const size_t slots = pl.pre_slots + pl.own_slots;
     p.pml = (float2 *) ((uint8_t *) a->work + pl.off_bytes);

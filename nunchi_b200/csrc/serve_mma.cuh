@@ -1,0 +1,410 @@
+// The shared prompt on the 5th-generation tensor cores (part of serve_attn.cu, inside its namespace): S = Q K^T and O += P V by
+// tcgen05.mma with S, P and O in tensor memory, for many query rows on one list of positions.
+//
+// Rows are (conversation, head) pairs of one kv head, 128 to a tile; a CTA runs two streams of them against the same tiles of
+// 128 positions (or, with at most 128 rows in all, one row tile against alternate position tiles), so that one stream's
+// softmax overlaps the other's products. A thread of a softmax warp owns a row (a TMEM lane): no exchange between threads.
+// P takes the place of S's first half (two 16-bit values per column) and is the product's A operand from there; O stays in
+// TMEM, and is rescaled only when a row's maximum has risen by more than 2^8 since the reference it was last scaled to (so a
+// P is at most 2^8, which fp16 holds, and l is summed in 32 bits).
+//   warps 0..3   K and V rows from their pages by 16-byte asynchronous copies into rings of tiles (128-byte swizzle, rows of a
+//                page that does not exist or beyond the prompt's end zero-filled)
+//   warps 4..7   softmax of stream 0, warps 8..11 of stream 1
+//   warp 12      issues the products: QK(j+1) of a stream directly behind PV(j), which reads the P that it overwrites (products
+//                of one thread run in the order of issue)
+// K is [position][dimension], the B operand with K = dimension contiguous; V is the B operand with N = dimension contiguous.
+// Bound by the exponentials: 16 per clock and SM, 2,048 clocks for two streams' tile; the products of head_dim 64 take half that.
+#pragma once
+
+constexpr int PM_M = 128, PM_N = 128, PM_ROWS = 2 * PM_M;
+constexpr int PM_MIN_ROWS = 16;        // query rows of a kv head up to which k_pa_pieces takes the prompt
+constexpr int PM_MIN_TILES = 2;        // position tiles of a piece at least
+constexpr int PM_MAX_TILES = 256;      // and at most (its page numbers are held in shared memory)
+constexpr int PM_THREADS = 13 * 32;
+constexpr float PM_RISE = 8.0f;
+
+template <int D> struct PmSmem {
+    static constexpr int TILE = PM_N * D * 2, NK = D == 64 ? 4 : 2, NV = D == 64 ? 4 : 2;
+    static constexpr int Q = 0, K = Q + 2 * PM_M * D * 2, V = K + NK * TILE, IDS = V + NV * TILE,
+                         BAR = IDS + PM_MAX_TILES * (PM_N / 16) * 4, TOTAL = BAR + 256;
+};
+
+__device__ __forceinline__ void pm_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((int) acc)
+                 : "memory");
+}
+__device__ __forceinline__ void pm_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"((int) acc)
+                 : "memory");
+}
+__device__ __forceinline__ void pm_commit(uint64_t *b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ void pm_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ void pm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// a matrix descriptor with the 128-byte swizzle (layout 2 at bit 61, version 1 at bit 46); lbo and sbo in bytes
+__device__ __forceinline__ uint64_t pm_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t) ((saddr >> 4) & 0x3FFF) | ((uint64_t) ((lbo >> 4) & 0x3FFF) << 16) | ((uint64_t) ((sbo >> 4) & 0x3FFF) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// kind::f16: D f32 (1 at bit 4), A and B both fp16 (0) or both bf16 (1) at bits 7 and 10, B with N contiguous: bit 16
+template <typename T>
+__device__ constexpr uint32_t pm_idesc(int m, int n, bool b_mn) {
+    const uint32_t t = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (m >> 4) << 24);
+}
+__device__ __forceinline__ void pm_ld32(uint32_t t, float (&v)[32]) {
+    uint32_t *u = (uint32_t *) v;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+          "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]),
+          "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
+          "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(t));
+}
+__device__ __forceinline__ void pm_st32(uint32_t t, const float (&v)[32]) {
+    const uint32_t *u = (const uint32_t *) v;
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+        "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]),
+        "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]),
+        "r"(u[31])
+        : "memory");
+}
+__device__ __forceinline__ void pm_st16(uint32_t t, const uint32_t (&u)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
+                 "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+                 "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+                 : "memory");
+}
+__device__ __forceinline__ void pm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 16 bytes to shared memory, or 16 zero bytes
+__device__ __forceinline__ void pm_copy(uint32_t dst, const void *src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant__ PaArgs p) {
+    extern __shared__ __align__(1024) uint8_t sm_raw[];
+    using L = PmSmem<D>;
+    constexpr int NK = L::NK, NV = L::NV, CH = D / 8;
+    constexpr uint32_t TM_S = 0, TM_O = 2 * PM_N;             // TMEM columns: S (and P) of both streams, O of both
+    const imi_cuda_prefix_attn_args &a = p.a;
+    uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
+    int *ids = (int *) (sm + L::IDS);
+    uint64_t *k_full = (uint64_t *) (sm + L::BAR), *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV,
+             *s_full = v_free + NV, *p_full = s_full + 2, *o_full = p_full + 2, *fin = o_full + 2;
+    __shared__ uint32_t tmem_at;
+    __shared__ int stop;
+    __shared__ int low_of;                                     // the lowest position that a row of the unit sees
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < NK; i++) { mbar_init(&k_full[i], 128); mbar_init(&k_free[i], 1); }
+        for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], 128); mbar_init(&v_free[i], 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
+        mbar_init(fin, 1);
+        stop = 0;
+        fence_barrier_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pm_fence_before();
+    __syncthreads();
+    pm_fence_after();
+    const uint32_t tmem = tmem_at;
+    pdl_wait();
+    pdl_trigger();
+
+    auto wait = [&](uint64_t *b, uint32_t parity) -> bool {    // bounded: about a second, then the CTA gives up
+        if (mbar_try_wait(b, parity)) return true;
+        if (*(volatile int *) &stop) return false;
+        if (mbar_wait(b, parity)) return true;
+        stop = 1;
+        if (a.status) atomicMax(a.status, IMI_DEV_WAIT);
+        return false;
+    };
+    const int qrows = a.rows * p.g;
+    const long long ps = (long long) a.n_head_kv * a.page * D;
+    const float sl2 = fabsf(p.sl2);                            // a negative scale turns q around
+    const bool turn = p.sl2 < 0.0f;
+    const long long line = (long long) p.rtiles * a.n_head_kv * p.tiles;
+    long long at = (long long) blockIdx.x * p.per;
+    const long long end = min(line, at + p.per);
+    int nk = 0, nv = 0, ns = 0;                                // tiles gone through the rings, S tiles of this thread's stream
+    int no = 0;                                                // units done
+    int pn[2] = { 0, 0 }, kn = 0, vn = 0;                      // MMA warp: P tiles of the streams, tiles of the rings
+    while (at < end) {
+        // one unit's part: position tiles [t0, t1)
+        const int unit = (int) (at / p.tiles), piece = (int) (blockIdx.x - (long long) unit * p.tiles / p.per);
+        int t0 = (int) (at - (long long) unit * p.tiles);
+        const int t1 = (int) min((long long) p.tiles, t0 + (end - at));
+        at += t1 - t0;
+        const int kvh = unit / p.rtiles, row0 = (unit % p.rtiles) * (p.pair ? PM_M : PM_ROWS);
+        if (__syncthreads_or(*(volatile int *) &stop)) break;  // the unit before is done with shared memory
+        if (tid == 0) low_of = INT32_MAX;
+        __syncthreads();
+        // the queries, and what their rows see
+        int fr = -1, lo = 0;
+        if (warp >= 4 && warp < 12) {
+            const int x = tid - 128;
+            fr = row0 + (p.pair ? x % PM_M : x);
+            if (fr >= qrows) fr = -1;
+            if (fr >= 0 && a.window > 0) lo = seen_of(p, fr / p.g).plo;
+            const int least = __reduce_min_sync(~0u, fr >= 0 ? lo : INT32_MAX);
+            if (lane == 0) atomicMin(&low_of, least);
+            if (!p.pair || x < PM_M) {
+                uint8_t *dst = sm + L::Q + (x / PM_M) * (PM_M * D * 2);
+                const int r = x % PM_M;
+                const T *q = fr >= 0 ? (const T *) a.q + fr / p.g * a.q_stride + ((long long) kvh * p.g + fr % p.g) * D : nullptr;
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    uint4 v = q ? ldg16(q + 8 * c) : make_uint4(0, 0, 0, 0);
+                    if (turn) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
+                    *(uint4 *) (dst + (c / 8) * (PM_M * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                }
+            }
+            fence_proxy_async();
+        } else if (warp < 4) {                                 // the pages of this part, -1 for one that does not exist
+            const int first = (t0 * PM_N) >> p.shift, n = ((min(a.prefix_len, t1 * PM_N) - 1) >> p.shift) - first + 1;
+            for (int i = tid; i < n; i += 128) {
+                int id = __ldg(a.prefix + first + i);
+                if ((unsigned) id >= (unsigned) a.n_pages) {
+                    id = -1;
+                    if (a.status) atomicMax(a.status, IMI_DEV_PAGE);
+                }
+                ids[i] = id;
+            }
+        }
+        __syncthreads();
+        const int page0 = (t0 * PM_N) >> p.shift;
+        t0 = max(t0, min(t1, low_of / PM_N));               // tiles that no row sees
+        const int tiles = t1 - t0, n0 = p.pair ? (tiles + 1) / 2 : tiles, n1 = p.pair ? tiles / 2 : tiles;
+        // the page of a position (a multiple of 16) of this part
+        auto id_at = [&](int pos) { return ids[(pos >> p.shift) - page0]; };
+
+        if (warp < 4) {
+            // ---------------- copies ----------------
+            const T *kb = (const T *) a.k_pages + (long long) kvh * a.page * D, *vb = (const T *) a.v_pages + (long long) kvh * a.page * D;
+            constexpr int RP = 128 / CH;                       // rows per pass
+            const int c = tid % CH, r0 = tid / CH;
+            uint64_t *pending[3];
+            int np = 0;
+            auto flush = [&]() {                               // everything issued has landed: say so
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async();
+                for (int i = 0; i < np; i++) pm_arrive(pending[i]);
+                np = 0;
+            };
+            auto load = [&](const T *base, int tile, uint32_t dst, uint64_t *full) {
+#pragma unroll
+                for (int i = 0; i < PM_N / RP; i++) {
+                    const int r = r0 + i * RP, pos = tile * PM_N + r;
+                    const bool in = pos < a.prefix_len;
+                    const int id = in ? id_at(pos) : -1;
+                    const T *src = base + (id >= 0 ? id : 0) * ps + (long long) (pos & (a.page - 1)) * D + 8 * c;
+                    pm_copy(dst + (c / 8) * (PM_N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, id >= 0);
+                }
+                if (np == 2) {                                 // two tiles in flight: the older one is awaited
+                    asm volatile("cp.async.commit_group;\n cp.async.wait_group 2;" ::: "memory");
+                    fence_proxy_async();
+                    pm_arrive(pending[0]);
+                    pending[0] = pending[1];
+                    np = 1;
+                } else {
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                }
+                pending[np++] = full;
+            };
+            bool ok = true;
+            for (int t = t0; t < t1 && ok; t++) {
+                const int ks = nk % NK, vs = nv % NV;
+                if (!mbar_try_wait(&k_free[ks], ((nk / NK) & 1) ^ 1)) {
+                    flush();                                   // nothing landed may be held back while this waits
+                    ok = wait(&k_free[ks], ((nk / NK) & 1) ^ 1);
+                    if (!ok) break;
+                }
+                load(kb, t, smem_u32(sm + L::K + ks * L::TILE), &k_full[ks]);
+                nk++;
+                if (!mbar_try_wait(&v_free[vs], ((nv / NV) & 1) ^ 1)) {
+                    flush();
+                    ok = wait(&v_free[vs], ((nv / NV) & 1) ^ 1);
+                    if (!ok) break;
+                }
+                load(vb, t, smem_u32(sm + L::V + vs * L::TILE), &v_full[vs]);
+                nv++;
+            }
+            flush();
+        } else if (warp == 12) {
+            // ---------------- products ----------------
+            const uint32_t qk = pm_idesc<T>(PM_M, PM_N, false), pv = pm_idesc<T>(PM_M, D, true);
+            bool ok = true;
+            auto issue_qk = [&](int st, int j) {
+                const int n = kn + (p.pair ? 2 * j + st : j), ks = n % NK;
+                ok = ok && __all_sync(~0u, wait(&k_full[ks], (n / NK) & 1));
+                if (!ok) return;
+                pm_fence_after();
+                if (lane == 0) {
+                    const uint32_t q = smem_u32(sm + L::Q) + (p.pair ? 0 : st) * (PM_M * D * 2), k = smem_u32(sm + L::K + ks * L::TILE);
+#pragma unroll
+                    for (int x = 0; x < D / 16; x++) {
+                        const uint32_t o = (x / 4) * (PM_N * 128) + (x % 4) * 32;
+                        pm_mma_ss(tmem + TM_S + st * PM_N, pm_desc(q + o, 16, 1024), pm_desc(k + o, 16, 1024), qk, x > 0);
+                    }
+                    pm_commit(&s_full[st]);
+                    if (p.pair || st == 1) pm_commit(&k_free[ks]);
+                }
+                __syncwarp();
+            };
+            auto issue_pv = [&](int st, int j, bool last) {
+                const int n = vn + (p.pair ? 2 * j + st : j), vs = n % NV;
+                ok = ok && __all_sync(~0u, wait(&v_full[vs], (n / NV) & 1));
+                ok = ok && __all_sync(~0u, wait(&p_full[st], (pn[st] & 1)));
+                pn[st]++;
+                if (!ok) return;
+                pm_fence_after();
+                if (lane == 0) {
+                    const uint32_t v = smem_u32(sm + L::V + vs * L::TILE);
+#pragma unroll
+                    for (int x = 0; x < PM_N / 16; x++)
+                        pm_mma_ts(tmem + TM_O + st * D, tmem + TM_S + st * PM_N + 8 * x, pm_desc(v + x * 2048, PM_N * 128, 1024), pv,
+                                  j > 0 || x > 0);
+                    if (p.pair || st == 1) pm_commit(&v_free[vs]);
+                    if (last) pm_commit(&o_full[st]);
+                }
+                __syncwarp();
+            };
+            if (n0 > 0) issue_qk(0, 0);
+            if (n1 > 0) issue_qk(1, 0);
+            for (int j = 0; j < n0 && ok; j++) {
+                issue_pv(0, j, j == n0 - 1);
+                if (j + 1 < n0) issue_qk(0, j + 1);
+                if (j < n1) issue_pv(1, j, j == n1 - 1);
+                if (j + 1 < n1) issue_qk(1, j + 1);
+            }
+            kn += tiles;
+            vn += tiles;
+        } else {
+            // ---------------- softmax ----------------
+            const int st = (warp - 4) / 4, n = st ? n1 : n0;
+            const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, S = tmem + TM_S + st * PM_N + lanes, O = tmem + TM_O + st * D + lanes;
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < n; j++, ns++) {
+                const int pos = (t0 + (p.pair ? 2 * j + st : j)) * PM_N;
+                ok = __all_sync(~0u, wait(&s_full[st], ns & 1));
+                if (!ok) break;
+                pm_fence_after();
+                // which of the tile's positions this row sees: from `from` to `to`, but for groups of 16 without a page
+                const int from = lo - pos, to = a.prefix_len - pos;
+                unsigned groups = 0;
+                if (lane < 8 && 16 * lane < to) groups = id_at(pos + 16 * lane) < 0;
+                groups = __ballot_sync(~0u, groups);
+                const bool masked = __any_sync(~0u, from > 0) || to < PM_N || groups;
+                auto hide = [&](float (&v)[32], int c) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const int x = 32 * c + e;
+                        if (x < from || x >= to || (groups >> (x / 16) & 1)) v[e] = -INFINITY;
+                    }
+                };
+                float v[32], top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    pm_ld32(S + 32 * c, v);
+                    pm_wait_ld();
+                    if (masked) hide(v, c);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(v[e], v[e + 1]));
+                }
+                top = top == -INFINITY ? top : top * sl2;
+                const bool raise = top > m + PM_RISE || (m == -INFINITY && top > m);
+                if (__any_sync(~0u, raise) ) {
+                    const float f = raise ? ex2(m - top) : 1.0f;   // m -infinity: 0
+                    l *= f;
+                    if (raise) m = top;
+                    if (j > 0) {
+                        float o[32];
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            pm_ld32(O + 32 * c, o);
+                            pm_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] *= f;
+                            pm_st32(O + 32 * c, o);
+                        }
+                    }
+                }
+                const float u = m == -INFINITY ? 0.0f : -m;
+                const float2 s2 = make_float2(sl2, sl2), u2 = make_float2(u, u);
+                float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    pm_ld32(S + 32 * c, v);
+                    pm_wait_ld();
+                    if (masked) hide(v, c);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float2 x = __ffma2_rn(make_float2(v[2 * e], v[2 * e + 1]), s2, u2);
+                        const float2 y = make_float2(ex2(x.x), ex2(x.y));
+                        sum = __fadd2_rn(sum, y);
+                        pk[e] = Half2<T>::pack(y.x, y.y);
+                    }
+                    pm_st16(S + 16 * c, pk);
+                }
+                l += sum.x + sum.y;
+                pm_wait_st();
+                pm_fence_before();
+                pm_arrive(&p_full[st]);
+            }
+            // this row's piece
+            const int i = fr / p.g, h = kvh * p.g + fr % p.g;
+            const long long slot = ((long long) i * a.n_head + h) * p.pre_splits + (p.pair ? 2 * piece + st : piece);
+            if (n > 0 && ok) {
+                ok = __all_sync(~0u, wait(&o_full[st], no & 1));
+                pm_fence_after();
+            }
+            if (fr >= 0) p.pml[slot] = make_float2(m, l);
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                float o[32];
+                if (n > 0 && ok) {
+                    pm_ld32(O + 32 * c, o);
+                    pm_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0.0f;
+                }
+                if (fr >= 0)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *(float4 *) (p.po + slot * D + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+            pm_fence_before();
+            if (n > 0) no++;
+        }
+    }
+    // products in flight end before their memory goes (bounded); copies have landed
+    __syncthreads();
+    if (warp == 12) {
+        if (lane == 0) {
+            pm_commit(fin);
+            mbar_wait(fin, 0);
+        }
+        __syncwarp();
+        pm_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
