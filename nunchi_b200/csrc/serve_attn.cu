@@ -21,8 +21,9 @@ namespace {
 constexpr int PA_ROWS = 4096;             // conversations at most
 constexpr int PA_WARPS = 4;               // warps of a piece's CTA
 constexpr int PA_STEP = 16;               // positions of a warp's step (a page holds whole steps)
-constexpr int PA_MIN_STEPS = 2 * PA_WARPS;   // steps of an own piece at least
-constexpr int PA_OWN_ITEMS = 1184;        // (piece, kv head) items aimed at for the own positions: 148 SMs x 8
+constexpr int PA_MIN_STEPS = 2 * PA_WARPS;   // steps of a piece of the prompt at least
+constexpr int PO_MIN_STEPS = 4;           // of an own piece, which is one warp's
+constexpr int PO_CTAS = 592, PO_ITEMS = PO_CTAS * PA_WARPS;   // own CTAs: 148 SMs x 4; (piece, kv head) items aimed at: one per warp
 constexpr int PA_PRE_ITEMS = 592;         // (row tile, kv head, piece) items aimed at for the prompt: 148 SMs x 4
 constexpr int PA_DIRECT = 1024;           // positions (prompt and own) up to which one CTA takes a row alone
 constexpr int PA_DWARPS = 8;              // its warps
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(PA_DWARPS * 32) k_pa_direct(const __grid_const
 
 // ---- pieces ----
 // own pieces of every row into off[0..rows] (shared memory): steps of 16 positions, `chunk` steps per piece, chosen so
-// that about PA_OWN_ITEMS (piece, kv head) items come out whatever the lengths are. Every CTA works this out from the
+// that about PO_ITEMS (piece, kv head) items come out whatever the lengths are. Every CTA works this out from the
 // lengths (4 bytes per row from L2). Returns chunk.
 __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     const imi_cuda_prefix_attn_args &a = p.a;
@@ -405,7 +406,7 @@ __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     int total;
     scan(sum, total);
     const long long items = (long long) total * a.n_head_kv;
-    const int chunk = max(PA_MIN_STEPS, (int) ((items + PA_OWN_ITEMS - 1) / PA_OWN_ITEMS));
+    const int chunk = max(PO_MIN_STEPS, (int) ((items + PO_ITEMS - 1) / PO_ITEMS));
     int cnt = 0;
     for (int i = i0; i < i1; i++) cnt += (off[i + 1] + chunk - 1) / chunk;
     int at = scan(cnt, total);
@@ -418,56 +419,22 @@ __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     return chunk;
 }
 
-// the pieces: (piece, row tile, kv head) of the prompt or, OWN, (piece, kv head) of the conversations' own positions
-template <typename T, int D, bool R8, bool OWN>
+// the prompt for few query rows: CTA items are (piece, tile of 16 query rows, kv head)
+template <typename T, int D>
 __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_pieces(const __grid_constant__ PaArgs p) {
-    constexpr int ROWS = R8 ? 8 : 16;
+    constexpr int ROWS = 16;
     extern __shared__ float shf[];
-    __shared__ int tmp[32];
     const imi_cuda_prefix_attn_args &a = p.a;
-    float *sh = shf;
-    int *off = (int *) (shf + PA_WARPS * ROWS * (D + 4));
-    // own pieces behind a launch for the prompt: that launch has let them start when all of its CTAs had done their own wait,
-    // and shares nothing with them; they wait for it at their end, so that k_join, which waits for them, has both
-    const bool early = OWN && a.prefix_len > 0;
-    if (!early) pdl_wait();
+    pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2;
     const long long ps = (long long) a.n_head_kv * a.page * D;
-    int chunk = 0, items;
-    const int qrows = a.rows * p.g, tiles = (qrows + ROWS - 1) / ROWS;
-    if (OWN) {
-        chunk = own_plan(p, off, tmp);
-        items = off[a.rows] * a.n_head_kv;
-        if (blockIdx.x == 0)
-            for (int i = threadIdx.x; i <= a.rows; i += PA_WARPS * 32) p.off[i] = off[i];
-    } else {
-        items = tiles * a.n_head_kv * p.pre_splits;
-    }
+    const int qrows = a.rows * p.g, tiles = (qrows + ROWS - 1) / ROWS, items = tiles * a.n_head_kv * p.pre_splits;
     for (int it = blockIdx.x; it < items; it += gridDim.x) {
-        Pass<T, D, R8> f;
+        Pass<T, D, false> f;
         f.init();
-        int fr0, nr, kvh, piece, row = 0;
-        if (OWN) {
-            kvh = it % a.n_head_kv;
-            const int k = it / a.n_head_kv;
-            int lo = 0, hi = a.rows;   // the row whose pieces hold k
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (off[mid] <= k) lo = mid;
-                else hi = mid;
-            }
-            row = lo;
-            piece = k - off[row];
-            fr0 = row * p.g;
-            nr = p.g;
-        } else {
-            kvh = it % a.n_head_kv;
-            const int k = it / a.n_head_kv, tile = k % tiles;
-            piece = k / tiles;
-            fr0 = tile * ROWS;
-            nr = min(ROWS, qrows - fr0);
-        }
+        const int kvh = it % a.n_head_kv, k = it / a.n_head_kv, tile = k % tiles, piece = k / tiles, fr0 = tile * ROWS,
+                  nr = min(ROWS, qrows - fr0);
         const T *q = (const T *) a.q + (long long) kvh * p.g * D;
         auto qrow = [&](int x) -> const T * {
             if (x >= nr) return nullptr;
@@ -476,81 +443,156 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_pieces(const __grid_consta
         };
         f.load_q(qrow(r), qrow(r + 8));
         const long long head = (long long) kvh * a.page * D;
-        const T *kb = (const T *) a.k_pages + head, *vb = (const T *) a.v_pages + head;
-        if (OWN) {
-            const Seen v = seen_of(p, row);
-            const int s0 = v.olo / PA_STEP + piece * chunk, lo = max(v.olo, s0 * PA_STEP), hi = min(v.len, (s0 + chunk) * PA_STEP);
-            f.run(p, a.table + row * a.table_stride, kb, vb, ps, lo, hi, v.olo, v.olo, warp, PA_WARPS);
-        } else {
-            int lo0 = 0, lo1 = 0, lo = piece * p.pre_len;
-            const int hi = min(a.prefix_len, lo + p.pre_len);
-            if (a.window > 0) {
-                if (r < nr) lo0 = seen_of(p, (fr0 + r) / p.g).plo;
-                if (r + 8 < nr) lo1 = seen_of(p, (fr0 + r + 8) / p.g).plo;
-                lo = max(lo, __reduce_min_sync(~0u, min(r < nr ? lo0 : INT32_MAX, r + 8 < nr ? lo1 : INT32_MAX)));
-            }
-            f.run(p, a.prefix, kb, vb, ps, lo, hi, lo0, lo1, warp, PA_WARPS);
+        int lo0 = 0, lo1 = 0, lo = piece * p.pre_len;
+        const int hi = min(a.prefix_len, lo + p.pre_len);
+        if (a.window > 0) {
+            if (r < nr) lo0 = seen_of(p, (fr0 + r) / p.g).plo;
+            if (r + 8 < nr) lo1 = seen_of(p, (fr0 + r + 8) / p.g).plo;
+            lo = max(lo, __reduce_min_sync(~0u, min(r < nr ? lo0 : INT32_MAX, r + 8 < nr ? lo1 : INT32_MAX)));
         }
+        f.run(p, a.prefix, (const T *) a.k_pages + head, (const T *) a.v_pages + head, ps, lo, hi, lo0, lo1, warp, PA_WARPS);
         f.finish();
         __syncthreads();   // the item before has been read
-        f.put(sh + warp * ROWS * (D + 4));
+        f.put(shf + warp * ROWS * (D + 4));
         __syncthreads();
-        join_warps<D, PA_WARPS, ROWS>(sh, nr, [&](int x, int c, float4 s, float m, float l) {
+        join_warps<D, PA_WARPS, ROWS>(shf, nr, [&](int x, int c, float4 s, float m, float l) {
             const int fr = fr0 + x, i = fr / p.g, h = kvh * p.g + fr % p.g;
-            const long long slot = OWN ? p.own_slot0 + (long long) (off[row] + piece) * a.n_head + h
-                                       : ((long long) i * a.n_head + h) * p.pre_splits + piece;
+            const long long slot = ((long long) i * a.n_head + h) * p.pre_splits + piece;
             *(float4 *) (p.po + slot * D + c) = s;
             if (c == 0) p.pml[slot] = make_float2(m, l);
         });
+    }
+}
+
+// the conversations' own positions: a warp's item is a (piece, kv head), its 16-position steps one after the other. Bound by
+// HBM: every row of K and V is read once, 4 to 8 KB of them on their way per warp.
+template <typename T, int D, bool R8>
+__global__ void __launch_bounds__(PA_WARPS * 32) k_pa_own(const __grid_constant__ PaArgs p) {
+    extern __shared__ int off[];
+    __shared__ int tmp[32];
+    const imi_cuda_prefix_attn_args &a = p.a;
+    // behind a launch for the prompt: that launch has let these CTAs start when all of its own had done their wait, and shares
+    // nothing with them; they wait for it at their end, so that k_join, which waits for them, has both
+    const bool early = a.prefix_len > 0;
+    if (!early) pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
+    const long long ps = (long long) a.n_head_kv * a.page * D;
+    const int chunk = own_plan(p, off, tmp), items = off[a.rows] * a.n_head_kv;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i <= a.rows; i += PA_WARPS * 32) p.off[i] = off[i];
+    for (int it = blockIdx.x * PA_WARPS + warp; it < items; it += gridDim.x * PA_WARPS) {
+        const int kvh = it % a.n_head_kv, k = it / a.n_head_kv;
+        int row = 0, up = a.rows;   // the row whose pieces hold k
+        while (up - row > 1) {
+            const int mid = (row + up) >> 1;
+            if (off[mid] <= k) row = mid;
+            else up = mid;
+        }
+        const int piece = k - off[row];
+        const T *q = (const T *) a.q + row * a.q_stride + (long long) kvh * p.g * D;
+        Pass<T, D, R8> f;
+        f.init();
+        f.load_q(r < p.g ? q + r * D : nullptr, r + 8 < p.g ? q + (r + 8) * D : nullptr);
+        const long long head = (long long) kvh * a.page * D;
+        const Seen v = seen_of(p, row);
+        const int s0 = v.olo / PA_STEP + piece * chunk, lo = max(v.olo, s0 * PA_STEP), hi = min(v.len, (s0 + chunk) * PA_STEP);
+        f.run(p, a.table + row * a.table_stride, (const T *) a.k_pages + head, (const T *) a.v_pages + head, ps, lo, hi, v.olo, v.olo, 0, 1);
+        f.finish();
+        const long long slot0 = p.own_slot0 + (long long) k * a.n_head + kvh * p.g;
+#pragma unroll
+        for (int x = 0; x < (R8 ? 1 : 2); x++)
+            if (r + 8 * x < p.g) {
+                float *o = p.po + (slot0 + r + 8 * x) * D;
+#pragma unroll
+                for (int h = 0; h < D / 64; h++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++)   // column n of the products: dimensions 64 h + 8 (2t + n) + 0..7
+#pragma unroll
+                        for (int j = 0; j < 8; j += 4)
+                            *(float4 *) (o + 64 * h + 16 * t + 8 * n + j) =
+                                make_float4(f.o[8 * h + j][2 * x + n], f.o[8 * h + j + 1][2 * x + n], f.o[8 * h + j + 2][2 * x + n],
+                                            f.o[8 * h + j + 3][2 * x + n]);
+                if (t == 0) p.pml[slot0 + r + 8 * x] = make_float2(x ? f.m1 : f.m0, x ? f.l1 : f.l0);
+            }
     }
     if (early) pdl_wait();
 }
 
 #include "serve_mma.cuh"
 
-// out and lse of every (row, head) from its pieces: one warp each
+// out and lse of every (row, head) from its pieces: `ways` (1, 2, 4 or 8) warps each, more where the pieces are many
 template <int D>
-__global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p) {
+__global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, int ways) {
+    __shared__ float sh[8][D + 4];
     const imi_cuda_prefix_attn_args &a = p.a;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31;
-    const long long x = blockIdx.x * 8LL + (threadIdx.x >> 5);
-    if (x >= (long long) a.rows * a.n_head) return;
-    const int i = (int) (x / a.n_head), h = (int) (x % a.n_head);
-    if (a.length[i] < 0) return;
-    int np = p.pre_splits;   // the prompt's pieces of this row
-    if (p.mma) {
-        const long long u0 = (long long) (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.tiles;
-        np = (int) (((u0 + p.tiles - 1) / p.per - u0 / p.per + 1) * (p.pair ? 2 : 1));
-    }
-    const int o0 = p.off[i], on = p.off[i + 1] - o0, n = np + on;
-    auto slot_of = [&](int k) -> long long {
-        return k < np ? x * p.pre_splits + k : p.own_slot0 + (long long) (o0 + k - np) * a.n_head + h;
-    };
-    float m = -INFINITY;
-    for (int k = lane; k < n; k += 32) m = fmaxf(m, p.pml[slot_of(k)].x);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    const float u = m == -INFINITY ? 0.0f : m;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, way = warp % ways;
+    const int x = blockIdx.x * (8 / ways) + warp / ways, i = x / a.n_head, h = x % a.n_head;
+    const bool live = i < a.rows && a.length[min(i, a.rows - 1)] >= 0;
+    float m = -INFINITY, l = 0.0f;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     // D / 4 lanes hold four dimensions each; at D 64 the warp's halves take every other piece
     constexpr int G = 32 / (D / 4);
     const int part = lane / (D / 4), c = lane % (D / 4) * 4;
-    float l = 0.0f;
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = part; k < n; k += G) {
-        const long long slot = slot_of(k);
-        const float2 ml = p.pml[slot];
-        const float f = ex2(ml.x - u);
-        const float4 v = *(const float4 *) (p.po + slot * D + c);
-        l = fmaf(f, ml.y, l);
-        s.x = fmaf(f, v.x, s.x); s.y = fmaf(f, v.y, s.y); s.z = fmaf(f, v.z, s.z); s.w = fmaf(f, v.w, s.w);
+    if (live) {
+        int np = p.pre_splits;   // the prompt's pieces of this row
+        if (p.mma) {
+            const int u0 = (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.tiles;
+            np = ((u0 + p.tiles - 1) / p.per - u0 / p.per + 1) * (p.pair ? 2 : 1);
+        }
+        const int o0 = p.off[i], n = np + p.off[i + 1] - o0;
+        auto slot_of = [&](int k) -> long long {
+            return k < np ? (long long) x * p.pre_splits + k : p.own_slot0 + (long long) (o0 + k - np) * a.n_head + h;
+        };
+        for (int k0 = way * G; k0 < n; k0 += 4 * G * ways) {   // four pieces' values on their way
+            float2 ml[4];
+            float4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int k = k0 + e * G * ways + part;
+                const long long slot = slot_of(min(k, n - 1));
+                ml[e] = k < n ? p.pml[slot] : make_float2(-INFINITY, 0.0f);
+                v[e] = *(const float4 *) (p.po + slot * D + c);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float top = fmaxf(m, ml[e].x), u = top == -INFINITY ? 0.0f : top, f = ex2(m - u), g = ex2(ml[e].x - u);
+                l = fmaf(l, f, g * ml[e].y);
+                // a piece that saw nothing adds nothing, whatever its sums hold
+                if (ml[e].x > -INFINITY) {
+                    s.x = fmaf(s.x, f, g * v[e].x); s.y = fmaf(s.y, f, g * v[e].y);
+                    s.z = fmaf(s.z, f, g * v[e].z); s.w = fmaf(s.w, f, g * v[e].w);
+                }
+                m = top;
+            }
+        }
+        if (G == 2) {
+            const float om = __shfl_xor_sync(~0u, m, 16), top = fmaxf(m, om), u = top == -INFINITY ? 0.0f : top, f = ex2(m - u);
+            l *= f;
+            s.x *= f; s.y *= f; s.z *= f; s.w *= f;
+            l += __shfl_xor_sync(~0u, l, 16);
+            s.x += __shfl_xor_sync(~0u, s.x, 16); s.y += __shfl_xor_sync(~0u, s.y, 16);
+            s.z += __shfl_xor_sync(~0u, s.z, 16); s.w += __shfl_xor_sync(~0u, s.w, 16);
+            m = top;
+        }
     }
-    if (G == 2) {
-        l += __shfl_xor_sync(~0u, l, 16);
-        s.x += __shfl_xor_sync(~0u, s.x, 16); s.y += __shfl_xor_sync(~0u, s.y, 16);
-        s.z += __shfl_xor_sync(~0u, s.z, 16); s.w += __shfl_xor_sync(~0u, s.w, 16);
+    if (ways > 1) {
+        if (part == 0) *(float4 *) &sh[warp][c] = s;
+        if (lane == 0) { sh[warp][D] = m; sh[warp][D + 1] = l; }
+        __syncthreads();
+        if (way) return;
+        for (int w = 1; w < ways; w++) {
+            const float *q = sh[warp + w];
+            const float4 v = *(const float4 *) (q + c);
+            const float om = q[D], top = fmaxf(m, om), u = top == -INFINITY ? 0.0f : top, f = ex2(m - u), g = ex2(om - u);
+            l = fmaf(l, f, g * q[D + 1]);
+            s.x = fmaf(s.x, f, g * v.x); s.y = fmaf(s.y, f, g * v.y); s.z = fmaf(s.z, f, g * v.z); s.w = fmaf(s.w, f, g * v.w);
+            m = top;
+        }
     }
+    if (!live) return;
     if (part == 0) put_out(a, i * a.out_stride + (long long) h * D + c, scaled(s, l));
     if (lane == 0 && a.lse) a.lse[x] = lse_of(m, l);
 }
@@ -584,7 +626,7 @@ PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len
         p.splits = (prefix_len + p.len - 1) / p.len;
     }
     p.pre_slots = (size_t) rows * n_head * p.splits;
-    p.own_slots = ((size_t) rows + (PA_OWN_ITEMS + n_head_kv - 1) / n_head_kv) * n_head;
+    p.own_slots = ((size_t) rows + (PO_ITEMS + n_head_kv - 1) / n_head_kv) * n_head;
     p.off_bytes = ((size_t) (rows + 1) * 4 + 255) / 256 * 256;
     const size_t slots = p.pre_slots + p.own_slots;
     p.bytes = p.off_bytes + (slots * 8 + 255) / 256 * 256 + slots * head_dim * 4;
@@ -610,14 +652,18 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
         r = launch_pdl((const void *) k_pa_mma<T, D>, dim3(pl.grid), PM_THREADS, PmSmem<D>::TOTAL + 1024, st, args);
     } else if (pl.splits) {
         const int items = (a.rows * p.g + 15) / 16 * a.n_head_kv * pl.splits;
-        r = launch_pdl((const void *) k_pa_pieces<T, D, false, false>, dim3(std::min(items, 148 * 16)), PA_WARPS * 32,
+        r = launch_pdl((const void *) k_pa_pieces<T, D>, dim3(std::min(items, 148 * 16)), PA_WARPS * 32,
                        (size_t) PA_WARPS * 16 * (D + 4) * 4, st, args);
     }
     if (r == cudaSuccess)
-        r = launch_pdl((const void *) k_pa_pieces<T, D, R8, true>, dim3(PA_OWN_ITEMS), PA_WARPS * 32,
-                       (size_t) PA_WARPS * ROWS * (D + 4) * 4 + (a.rows + 1) * 4, st, args);
-    if (r == cudaSuccess)
-        r = launch_pdl((const void *) k_join<D>, dim3((a.rows * a.n_head + 7) / 8), 256, 0, st, args);
+        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(PO_CTAS), PA_WARPS * 32, (size_t) (a.rows + 1) * 4, st, args);
+    if (r == cudaSuccess) {
+        // warps per (row, head): one up to 16 pieces, and while there are few of both
+        int ways = 1;
+        while (ways < 8 && (pl.splits > 16 * ways || (a.rows * a.n_head * ways < 1184 && pl.splits > 2 * ways))) ways *= 2;
+        void *jargs[] = { &p, &ways };
+        r = launch_pdl((const void *) k_join<D>, dim3((a.rows * a.n_head * ways + 7) / 8), 256, 0, st, jargs);
+    }
     return r;
 }
 template <typename T>
@@ -632,9 +678,7 @@ cudaError_t raise_pa(int device) {
     return lim.raise(device,
                      { (const void *) k_pa_direct<T, 64, true>, (const void *) k_pa_direct<T, 64, false>,
                        (const void *) k_pa_direct<T, 128, true>, (const void *) k_pa_direct<T, 128, false>,
-                       (const void *) k_pa_pieces<T, 64, false, false>, (const void *) k_pa_pieces<T, 128, false, false>,
-                       (const void *) k_pa_pieces<T, 64, true, true>, (const void *) k_pa_pieces<T, 64, false, true>,
-                       (const void *) k_pa_pieces<T, 128, true, true>, (const void *) k_pa_pieces<T, 128, false, true> },
+                       (const void *) k_pa_pieces<T, 64>, (const void *) k_pa_pieces<T, 128> },
                      96 * 1024) == cudaSuccess
                ? lim2.raise(device, { (const void *) k_pa_mma<T, 64>, (const void *) k_pa_mma<T, 128> }, (int) std::max(PmSmem<64>::TOTAL, PmSmem<128>::TOTAL) + 1024)
                : cudaErrorUnknown;
@@ -661,6 +705,8 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
     if (a->n_pages < 0 || a->window < 0) return set_error(IMI_E_ARG, "prefix_attn: negative n_pages or window");
     if (!std::isfinite(a->scale)) return set_error(IMI_E_ARG, "prefix_attn: scale is not finite");
     if (a->rows == 0) return IMI_OK;
+    if ((int64_t) a->rows * a->n_head / PM_ROWS * ((int64_t) a->prefix_len / PM_N + 1) > INT32_MAX / 4)
+        return set_error(IMI_E_ARG, "prefix_attn: the prompt is too long for so many rows");
     if (!a->q || !a->out || !a->length || !a->work) return set_error(IMI_E_ARG, "prefix_attn: null argument");
     if ((a->prefix_len && !a->prefix) || (a->width && !a->table)) return set_error(IMI_E_ARG, "prefix_attn: no page list");
     if ((a->prefix_len || a->width) && (!a->k_pages || !a->v_pages || a->n_pages < 1))

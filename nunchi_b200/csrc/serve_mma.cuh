@@ -4,14 +4,16 @@
 // Rows are (conversation, head) pairs of one kv head, 128 to a tile; a CTA runs two streams of them against the same tiles of
 // 128 positions (or, with at most 128 rows in all, one row tile against alternate position tiles), so that one stream's
 // softmax overlaps the other's products. A thread of a softmax warp owns a row (a TMEM lane): no exchange between threads.
-// P takes the place of S's first half (two 16-bit values per column) and is the product's A operand from there; O stays in
-// TMEM, and is rescaled only when a row's maximum has risen by more than 2^8 since the reference it was last scaled to (so a
-// P is at most 2^8, which fp16 holds, and l is summed in 32 bits).
-//   warps 0..3   K and V rows from their pages by 16-byte asynchronous copies into rings of tiles (128-byte swizzle, rows of a
+// P (two 16-bit values per column) is the product's A operand from TMEM; O stays in TMEM, and is rescaled only when a row's
+// maximum has risen by more than 2^8 since the reference it was last scaled to (so a P is at most 2^8, which fp16 holds, and l
+// is summed in 32 bits). At head_dim 64 S, P and O of both streams fill the 512 columns: QK(j+1) is issued as soon as S(j) is in
+// the softmax's registers. At 128 P takes S's place, and QK(j+1) goes directly behind PV(j), which reads it (products of one
+// thread run in the order of issue).
+//   warps 0..2   K and V rows from their pages by 16-byte asynchronous copies into rings of tiles (128-byte swizzle, rows of a
 //                page that does not exist or beyond the prompt's end zero-filled)
-//   warps 4..7   softmax of stream 0, warps 8..11 of stream 1
-//   warp 12      issues the products: QK(j+1) of a stream directly behind PV(j), which reads the P that it overwrites (products
-//                of one thread run in the order of issue)
+//   warp 3       issues the products
+//   warps 4..7   softmax of stream 0, warps 8..11 of stream 1, with the registers that the others give up: a thread holds its
+//                row's 128 scores
 // K is [position][dimension], the B operand with K = dimension contiguous; V is the B operand with N = dimension contiguous.
 // Bound by the exponentials: 16 per clock and SM, 2,048 clocks for two streams' tile; the products of head_dim 64 take half that.
 #pragma once
@@ -20,7 +22,8 @@ constexpr int PM_M = 128, PM_N = 128, PM_ROWS = 2 * PM_M;
 constexpr int PM_MIN_ROWS = 16;        // query rows of a kv head up to which k_pa_pieces takes the prompt
 constexpr int PM_MIN_TILES = 2;        // position tiles of a piece at least
 constexpr int PM_MAX_TILES = 256;      // and at most (its page numbers are held in shared memory)
-constexpr int PM_THREADS = 13 * 32;
+constexpr int PM_COPY = 96, PM_THREADS = 12 * 32;
+constexpr int PM_REGS = 168, PM_REGS_FEW = 80, PM_REGS_MANY = 208;   // 4 x 80 + 8 x 208 <= 12 x 168
 constexpr float PM_RISE = 8.0f;
 
 template <int D> struct PmSmem {
@@ -44,6 +47,12 @@ __device__ __forceinline__ void pm_commit(uint64_t *b) {
 }
 __device__ __forceinline__ void pm_arrive(uint64_t *b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+// true in one thread of the warp
+__device__ __forceinline__ bool pm_elect() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void pm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -98,32 +107,36 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     extern __shared__ __align__(1024) uint8_t sm_raw[];
     using L = PmSmem<D>;
     constexpr int NK = L::NK, NV = L::NV, CH = D / 8;
-    constexpr uint32_t TM_S = 0, TM_O = 2 * PM_N;             // TMEM columns: S (and P) of both streams, O of both
+    constexpr bool APART = D == 64;                            // P beside S, not over it
+    constexpr uint32_t TM_S = 0, TM_P = APART ? 2 * PM_N : 0, TM_O = APART ? 3 * PM_N : 2 * PM_N;   // TMEM columns, both streams'
+    constexpr uint32_t P_STEP = APART ? PM_N / 2 : PM_N;       // from stream 0's P to stream 1's
     const imi_cuda_prefix_attn_args &a = p.a;
     uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
     int *ids = (int *) (sm + L::IDS);
     uint64_t *k_full = (uint64_t *) (sm + L::BAR), *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV,
-             *s_full = v_free + NV, *p_full = s_full + 2, *o_full = p_full + 2, *fin = o_full + 2;
+             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *fin = o_full + 2;
     __shared__ uint32_t tmem_at;
     __shared__ int stop;
     __shared__ int low_of;                                     // the lowest position that a row of the unit sees
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // what a warp's threads agree on goes through a shuffle, so that the compiler keeps it, and the products' operands made of
+    // it, in uniform registers: moved there for every product, issuing them took 2.5 us of a tile instead of 1
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
     if (tid == 0) {
-        for (int i = 0; i < NK; i++) { mbar_init(&k_full[i], 128); mbar_init(&k_free[i], 1); }
-        for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], 128); mbar_init(&v_free[i], 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
+        for (int i = 0; i < NK; i++) { mbar_init(&k_full[i], PM_COPY); mbar_init(&k_free[i], 1); }
+        for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], PM_COPY); mbar_init(&v_free[i], 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&s_read[i], 128); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
         mbar_init(fin, 1);
         stop = 0;
         fence_barrier_init();
     }
-    if (warp == 12) {
+    if (warp == 3) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     pm_fence_before();
     __syncthreads();
     pm_fence_after();
-    const uint32_t tmem = tmem_at;
+    const uint32_t tmem = __shfl_sync(~0u, tmem_at, 0);
     pdl_wait();
     pdl_trigger();
 
@@ -139,35 +152,36 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     const long long ps = (long long) a.n_head_kv * a.page * D;
     const float sl2 = fabsf(p.sl2);                            // a negative scale turns q around
     const bool turn = p.sl2 < 0.0f;
-    const long long line = (long long) p.rtiles * a.n_head_kv * p.tiles;
-    long long at = (long long) blockIdx.x * p.per;
-    const long long end = min(line, at + p.per);
-    int nk = 0, nv = 0, ns = 0;                                // tiles gone through the rings, S tiles of this thread's stream
-    int no = 0;                                                // units done
-    int pn[2] = { 0, 0 }, kn = 0, vn = 0;                      // MMA warp: P tiles of the streams, tiles of the rings
-    while (at < end) {
-        // one unit's part: position tiles [t0, t1)
-        const int unit = (int) (at / p.tiles), piece = (int) (blockIdx.x - (long long) unit * p.tiles / p.per);
-        int t0 = (int) (at - (long long) unit * p.tiles);
-        const int t1 = (int) min((long long) p.tiles, t0 + (end - at));
-        at += t1 - t0;
-        const int kvh = unit / p.rtiles, row0 = (unit % p.rtiles) * (p.pair ? PM_M : PM_ROWS);
-        if (__syncthreads_or(*(volatile int *) &stop)) break;  // the unit before is done with shared memory
+    const int line = p.rtiles * a.n_head_kv * p.tiles, end = min(line, ((int) blockIdx.x + 1) * p.per);
+    int at = (int) blockIdx.x * p.per;
+    struct Unit {
+        int kvh, row0, piece, page0, t0, t1, n0, n1;           // position tiles [t0, t1), of them the streams'
+    };
+    // the next unit's part, after the CTA is done with the one before: false where there is none
+    int fr = -1, lo = 0;                                       // softmax: the thread's row, and what it sees from
+    auto next = [&](Unit &w) -> bool {
+        if (__syncthreads_or(at >= end || *(volatile int *) &stop)) return false;
         if (tid == 0) low_of = INT32_MAX;
+        const int unit = at / p.tiles;
+        w.piece = (int) blockIdx.x - unit * p.tiles / p.per;
+        w.t0 = at - unit * p.tiles;
+        w.t1 = min(p.tiles, w.t0 + (end - at));
+        at += w.t1 - w.t0;
+        w.kvh = unit / p.rtiles;
+        w.row0 = (unit % p.rtiles) * (p.pair ? PM_M : PM_ROWS);
+        w.page0 = (w.t0 * PM_N) >> p.shift;
         __syncthreads();
-        // the queries, and what their rows see
-        int fr = -1, lo = 0;
-        if (warp >= 4 && warp < 12) {
+        if (warp >= 4) {                                       // the queries, and what their rows see
             const int x = tid - 128;
-            fr = row0 + (p.pair ? x % PM_M : x);
+            fr = w.row0 + (p.pair ? x % PM_M : x);
             if (fr >= qrows) fr = -1;
-            if (fr >= 0 && a.window > 0) lo = seen_of(p, fr / p.g).plo;
+            lo = fr >= 0 && a.window > 0 ? seen_of(p, fr / p.g).plo : 0;
             const int least = __reduce_min_sync(~0u, fr >= 0 ? lo : INT32_MAX);
             if (lane == 0) atomicMin(&low_of, least);
             if (!p.pair || x < PM_M) {
                 uint8_t *dst = sm + L::Q + (x / PM_M) * (PM_M * D * 2);
                 const int r = x % PM_M;
-                const T *q = fr >= 0 ? (const T *) a.q + fr / p.g * a.q_stride + ((long long) kvh * p.g + fr % p.g) * D : nullptr;
+                const T *q = fr >= 0 ? (const T *) a.q + fr / p.g * a.q_stride + ((long long) w.kvh * p.g + fr % p.g) * D : nullptr;
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
                     uint4 v = q ? ldg16(q + 8 * c) : make_uint4(0, 0, 0, 0);
@@ -176,10 +190,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                 }
             }
             fence_proxy_async();
-        } else if (warp < 4) {                                 // the pages of this part, -1 for one that does not exist
-            const int first = (t0 * PM_N) >> p.shift, n = ((min(a.prefix_len, t1 * PM_N) - 1) >> p.shift) - first + 1;
+        } else {                                               // the pages of this part, -1 for one that does not exist
+            const int n = ((min(a.prefix_len, w.t1 * PM_N) - 1) >> p.shift) - w.page0 + 1;
             for (int i = tid; i < n; i += 128) {
-                int id = __ldg(a.prefix + first + i);
+                int id = __ldg(a.prefix + w.page0 + i);
                 if ((unsigned) id >= (unsigned) a.n_pages) {
                     id = -1;
                     if (a.status) atomicMax(a.status, IMI_DEV_PAGE);
@@ -188,121 +202,146 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
             }
         }
         __syncthreads();
-        const int page0 = (t0 * PM_N) >> p.shift;
-        t0 = max(t0, min(t1, low_of / PM_N));               // tiles that no row sees
-        const int tiles = t1 - t0, n0 = p.pair ? (tiles + 1) / 2 : tiles, n1 = p.pair ? tiles / 2 : tiles;
-        // the page of a position (a multiple of 16) of this part
-        auto id_at = [&](int pos) { return ids[(pos >> p.shift) - page0]; };
+        w.t0 = max(w.t0, min(w.t1, __shfl_sync(~0u, low_of, 0) / PM_N));            // tiles that no row sees
+        const int tiles = w.t1 - w.t0;
+        w.n0 = p.pair ? (tiles + 1) / 2 : tiles;
+        w.n1 = p.pair ? tiles / 2 : tiles;
+        return true;
+    };
+    Unit w = {};
+    // the page of a position (a multiple of 16, or in its group of 16) of the part
+    auto id_at = [&](int pos) { return ids[(pos >> p.shift) - w.page0]; };
 
-        if (warp < 4) {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PM_REGS_FEW));
+        if (warp < 3) {
             // ---------------- copies ----------------
-            const T *kb = (const T *) a.k_pages + (long long) kvh * a.page * D, *vb = (const T *) a.v_pages + (long long) kvh * a.page * D;
-            constexpr int RP = 128 / CH;                       // rows per pass
-            const int c = tid % CH, r0 = tid / CH;
+            int nk = 0, nv = 0;                                    // tiles gone through the rings
             uint64_t *pending[3];
             int np = 0;
-            auto flush = [&]() {                               // everything issued has landed: say so
+            auto flush = [&]() {                                   // everything issued has landed: say so
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_proxy_async();
                 for (int i = 0; i < np; i++) pm_arrive(pending[i]);
                 np = 0;
             };
-            auto load = [&](const T *base, int tile, uint32_t dst, uint64_t *full) {
-#pragma unroll
-                for (int i = 0; i < PM_N / RP; i++) {
-                    const int r = r0 + i * RP, pos = tile * PM_N + r;
-                    const bool in = pos < a.prefix_len;
-                    const int id = in ? id_at(pos) : -1;
-                    const T *src = base + (id >= 0 ? id : 0) * ps + (long long) (pos & (a.page - 1)) * D + 8 * c;
-                    pm_copy(dst + (c / 8) * (PM_N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, id >= 0);
-                }
-                if (np == 2) {                                 // two tiles in flight: the older one is awaited
-                    asm volatile("cp.async.commit_group;\n cp.async.wait_group 2;" ::: "memory");
-                    fence_proxy_async();
-                    pm_arrive(pending[0]);
-                    pending[0] = pending[1];
-                    np = 1;
-                } else {
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                }
-                pending[np++] = full;
-            };
-            bool ok = true;
-            for (int t = t0; t < t1 && ok; t++) {
-                const int ks = nk % NK, vs = nv % NV;
-                if (!mbar_try_wait(&k_free[ks], ((nk / NK) & 1) ^ 1)) {
-                    flush();                                   // nothing landed may be held back while this waits
-                    ok = wait(&k_free[ks], ((nk / NK) & 1) ^ 1);
-                    if (!ok) break;
-                }
-                load(kb, t, smem_u32(sm + L::K + ks * L::TILE), &k_full[ks]);
-                nk++;
-                if (!mbar_try_wait(&v_free[vs], ((nv / NV) & 1) ^ 1)) {
-                    flush();
-                    ok = wait(&v_free[vs], ((nv / NV) & 1) ^ 1);
-                    if (!ok) break;
-                }
-                load(vb, t, smem_u32(sm + L::V + vs * L::TILE), &v_full[vs]);
-                nv++;
-            }
-            flush();
-        } else if (warp == 12) {
-            // ---------------- products ----------------
-            const uint32_t qk = pm_idesc<T>(PM_M, PM_N, false), pv = pm_idesc<T>(PM_M, D, true);
-            bool ok = true;
-            auto issue_qk = [&](int st, int j) {
-                const int n = kn + (p.pair ? 2 * j + st : j), ks = n % NK;
-                ok = ok && __all_sync(~0u, wait(&k_full[ks], (n / NK) & 1));
-                if (!ok) return;
-                pm_fence_after();
-                if (lane == 0) {
-                    const uint32_t q = smem_u32(sm + L::Q) + (p.pair ? 0 : st) * (PM_M * D * 2), k = smem_u32(sm + L::K + ks * L::TILE);
-#pragma unroll
-                    for (int x = 0; x < D / 16; x++) {
-                        const uint32_t o = (x / 4) * (PM_N * 128) + (x % 4) * 32;
-                        pm_mma_ss(tmem + TM_S + st * PM_N, pm_desc(q + o, 16, 1024), pm_desc(k + o, 16, 1024), qk, x > 0);
+            while (next(w)) {
+                const T *kb = (const T *) a.k_pages + (long long) w.kvh * a.page * D, *vb = (const T *) a.v_pages + (long long) w.kvh * a.page * D;
+                auto load = [&](const T *base, int tile, uint32_t dst, uint64_t *full) {
+    #pragma unroll 4
+                    for (int x = tid; x < PM_N * CH; x += PM_COPY) {
+                        const int r = x / CH, c = x % CH, pos = tile * PM_N + r;
+                        const bool in = pos < a.prefix_len;
+                        const int id = in ? id_at(pos) : -1;
+                        const T *src = base + (id >= 0 ? id : 0) * ps + (long long) (pos & (a.page - 1)) * D + 8 * c;
+                        pm_copy(dst + (c / 8) * (PM_N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, id >= 0);
                     }
-                    pm_commit(&s_full[st]);
-                    if (p.pair || st == 1) pm_commit(&k_free[ks]);
+                    if (np == 2) {                                 // two tiles in flight: the older one is awaited
+                        asm volatile("cp.async.commit_group;\n cp.async.wait_group 2;" ::: "memory");
+                        fence_proxy_async();
+                        pm_arrive(pending[0]);
+                        pending[0] = pending[1];
+                        np = 1;
+                    } else {
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                    }
+                    pending[np++] = full;
+                };
+                auto room = [&](uint64_t *b, uint32_t parity) -> bool {
+                    if (mbar_try_wait(b, parity)) return true;
+                    flush();                                       // nothing landed may be held back while this waits
+                    return wait(b, parity);
+                };
+                for (int t = w.t0; t < w.t1; t++) {
+                    const int ks = nk % NK, vs = nv % NV;
+                    if (!room(&k_free[ks], ((nk / NK) & 1) ^ 1)) break;
+                    load(kb, t, smem_u32(sm + L::K + ks * L::TILE), &k_full[ks]);
+                    nk++;
+                    if (!room(&v_free[vs], ((nv / NV) & 1) ^ 1)) break;
+                    load(vb, t, smem_u32(sm + L::V + vs * L::TILE), &v_full[vs]);
+                    nv++;
                 }
-                __syncwarp();
-            };
-            auto issue_pv = [&](int st, int j, bool last) {
-                const int n = vn + (p.pair ? 2 * j + st : j), vs = n % NV;
-                ok = ok && __all_sync(~0u, wait(&v_full[vs], (n / NV) & 1));
-                ok = ok && __all_sync(~0u, wait(&p_full[st], (pn[st] & 1)));
-                pn[st]++;
-                if (!ok) return;
-                pm_fence_after();
-                if (lane == 0) {
-                    const uint32_t v = smem_u32(sm + L::V + vs * L::TILE);
-#pragma unroll
-                    for (int x = 0; x < PM_N / 16; x++)
-                        pm_mma_ts(tmem + TM_O + st * D, tmem + TM_S + st * PM_N + 8 * x, pm_desc(v + x * 2048, PM_N * 128, 1024), pv,
-                                  j > 0 || x > 0);
-                    if (p.pair || st == 1) pm_commit(&v_free[vs]);
-                    if (last) pm_commit(&o_full[st]);
-                }
-                __syncwarp();
-            };
-            if (n0 > 0) issue_qk(0, 0);
-            if (n1 > 0) issue_qk(1, 0);
-            for (int j = 0; j < n0 && ok; j++) {
-                issue_pv(0, j, j == n0 - 1);
-                if (j + 1 < n0) issue_qk(0, j + 1);
-                if (j < n1) issue_pv(1, j, j == n1 - 1);
-                if (j + 1 < n1) issue_qk(1, j + 1);
+                flush();
             }
-            kn += tiles;
-            vn += tiles;
-        } else {
-            // ---------------- softmax ----------------
-            const int st = (warp - 4) / 4, n = st ? n1 : n0;
-            const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, S = tmem + TM_S + st * PM_N + lanes, O = tmem + TM_O + st * D + lanes;
+        } else if (warp == 3) {
+            // ---------------- products ----------------
+            int pn[2] = { 0, 0 }, rn[2] = { 0, 0 }, kn = 0, vn = 0;   // P and S tiles of the streams, tiles of the rings
+            const uint32_t qk = pm_idesc<T>(PM_M, PM_N, false), pv = pm_idesc<T>(PM_M, D, true);
+            // descriptors of the first tiles; the others' differ in the address alone (16-byte units, in the low bits)
+            const uint64_t qd = pm_desc(smem_u32(sm + L::Q), 16, 1024), kd = pm_desc(smem_u32(sm + L::K), 16, 1024),
+                           vd = pm_desc(smem_u32(sm + L::V), PM_N * 128, 1024);
+            while (next(w)) {
+                const int n0 = w.n0, n1 = w.n1;
+                bool ok = true;
+                auto issue_qk = [&](int st, int j) {
+                    const int n = kn + (p.pair ? 2 * j + st : j), ks = n % NK;
+                    ok = ok && __all_sync(~0u, wait(&k_full[ks], (n / NK) & 1));
+                    if (!ok) return;
+                    pm_fence_after();
+                    if (pm_elect()) {
+                        const uint64_t q = qd + (p.pair ? 0 : st) * (PM_M * D * 2 >> 4), k = kd + ks * (L::TILE >> 4);
+#pragma unroll
+                        for (int x = 0; x < D / 16; x++) {
+                            const uint32_t o = ((x / 4) * (PM_N * 128) + (x % 4) * 32) >> 4;
+                            pm_mma_ss(tmem + TM_S + st * PM_N, q + o, k + o, qk, x > 0);
+                        }
+                        pm_commit(&s_full[st]);
+                        if (p.pair || st == 1) pm_commit(&k_free[ks]);
+                    }
+                    __syncwarp();
+                };
+                auto issue_pv = [&](int st, int j, bool last) {
+                    const int n = vn + (p.pair ? 2 * j + st : j), vs = n % NV;
+                    ok = ok && __all_sync(~0u, wait(&v_full[vs], (n / NV) & 1));
+                    ok = ok && __all_sync(~0u, wait(&p_full[st], (pn[st] & 1)));
+                    pn[st]++;
+                    if (!ok) return;
+                    pm_fence_after();
+                    if (pm_elect()) {
+                        const uint64_t v = vd + vs * (L::TILE >> 4);
+#pragma unroll
+                        for (int x = 0; x < PM_N / 16; x++)
+                            pm_mma_ts(tmem + TM_O + st * D, tmem + TM_P + st * P_STEP + 8 * x, v + x * (2048 >> 4), pv, j > 0 || x > 0);
+                        if (p.pair || st == 1) pm_commit(&v_free[vs]);
+                        if (APART || last) pm_commit(&o_full[st]);
+                    }
+                    __syncwarp();
+                };
+                auto read = [&](int st) {                          // S is in the softmax's registers
+                    ok = ok && __all_sync(~0u, wait(&s_read[st], rn[st] & 1));
+                    rn[st]++;
+                };
+                if (n0 > 0) issue_qk(0, 0);
+                if (n1 > 0) issue_qk(1, 0);
+                for (int j = 0; j < n0 && ok; j++) {
+                    if (APART) {
+                        read(0);
+                        if (j + 1 < n0) issue_qk(0, j + 1);
+                        if (j < n1) read(1);
+                        if (j + 1 < n1) issue_qk(1, j + 1);
+                    }
+                    issue_pv(0, j, j == n0 - 1);
+                    if (!APART && j + 1 < n0) issue_qk(0, j + 1);
+                    if (j < n1) issue_pv(1, j, j == n1 - 1);
+                    if (!APART && j + 1 < n1) issue_qk(1, j + 1);
+                }
+                kn += w.t1 - w.t0;
+                vn += w.t1 - w.t0;
+            }
+        }
+    } else {
+        // ---------------- softmax ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PM_REGS_MANY));
+        const int st = (warp - 4) / 4;
+        const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, S = tmem + TM_S + st * PM_N + lanes,
+                       P = tmem + TM_P + st * P_STEP + lanes, O = tmem + TM_O + st * D + lanes;
+        int ns = 0, no = 0;                                    // S tiles, and O's commits, of this stream
+        while (next(w)) {
+            const int n = st ? w.n1 : w.n0;
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
             for (int j = 0; j < n; j++, ns++) {
-                const int pos = (t0 + (p.pair ? 2 * j + st : j)) * PM_N;
+                const int pos = (w.t0 + (p.pair ? 2 * j + st : j)) * PM_N;
                 ok = __all_sync(~0u, wait(&s_full[st], ns & 1));
                 if (!ok) break;
                 pm_fence_after();
@@ -312,25 +351,35 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                 if (lane < 8 && 16 * lane < to) groups = id_at(pos + 16 * lane) < 0;
                 groups = __ballot_sync(~0u, groups);
                 const bool masked = __any_sync(~0u, from > 0) || to < PM_N || groups;
-                auto hide = [&](float (&v)[32], int c) {
+                float v[PM_N];
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int x = 32 * c + e;
-                        if (x < from || x >= to || (groups >> (x / 16) & 1)) v[e] = -INFINITY;
-                    }
-                };
-                float v[32], top = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    pm_ld32(S + 32 * c, v);
-                    pm_wait_ld();
-                    if (masked) hide(v, c);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(v[e], v[e + 1]));
+                for (int c = 0; c < 4; c++) pm_ld32(S + 32 * c, *(float (*)[32]) (v + 32 * c));
+                pm_wait_ld();
+                if (APART) {
+                    pm_fence_before();
+                    pm_arrive(&s_read[st]);
                 }
+                if (masked)
+#pragma unroll
+                    for (int x = 0; x < PM_N; x++)
+                        if (x < from || x >= to || (groups >> (x / 16) & 1)) v[x] = -INFINITY;
+                float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+#pragma unroll
+                for (int x = 0; x < PM_N; x += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) t4[e] = fmaxf(t4[e], fmaxf(v[x + e], v[x + e + 4]));
+                float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
                 top = top == -INFINITY ? top : top * sl2;
                 const bool raise = top > m + PM_RISE || (m == -INFINITY && top > m);
-                if (__any_sync(~0u, raise) ) {
+                const bool any = __any_sync(~0u, raise);
+                // the product of the tile before reads P and adds to O: done before either is written
+                if (APART && j > 0) {
+                    ok = __all_sync(~0u, wait(&o_full[st], no & 1));
+                    no++;
+                    if (!ok) break;
+                    pm_fence_after();
+                }
+                if (any) {
                     const float f = raise ? ex2(m - top) : 1.0f;   // m -infinity: 0
                     l *= f;
                     if (raise) m = top;
@@ -348,30 +397,27 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                 }
                 const float u = m == -INFINITY ? 0.0f : -m;
                 const float2 s2 = make_float2(sl2, sl2), u2 = make_float2(u, u);
-                float2 sum = make_float2(0.0f, 0.0f);
+                float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    pm_ld32(S + 32 * c, v);
-                    pm_wait_ld();
-                    if (masked) hide(v, c);
                     uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const float2 x = __ffma2_rn(make_float2(v[2 * e], v[2 * e + 1]), s2, u2);
+                        const float2 x = __ffma2_rn(make_float2(v[32 * c + 2 * e], v[32 * c + 2 * e + 1]), s2, u2);
                         const float2 y = make_float2(ex2(x.x), ex2(x.y));
-                        sum = __fadd2_rn(sum, y);
+                        sum[e & 1] = __fadd2_rn(sum[e & 1], y);
                         pk[e] = Half2<T>::pack(y.x, y.y);
                     }
-                    pm_st16(S + 16 * c, pk);
+                    pm_st16(P + 16 * c, pk);
                 }
-                l += sum.x + sum.y;
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 pm_wait_st();
                 pm_fence_before();
                 pm_arrive(&p_full[st]);
             }
             // this row's piece
-            const int i = fr / p.g, h = kvh * p.g + fr % p.g;
-            const long long slot = ((long long) i * a.n_head + h) * p.pre_splits + (p.pair ? 2 * piece + st : piece);
+            const int i = fr / p.g, h = w.kvh * p.g + fr % p.g;
+            const long long slot = ((long long) i * a.n_head + h) * p.pre_splits + (p.pair ? 2 * w.piece + st : w.piece);
             if (n > 0 && ok) {
                 ok = __all_sync(~0u, wait(&o_full[st], no & 1));
                 pm_fence_after();
@@ -398,7 +444,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     }
     // products in flight end before their memory goes (bounded); copies have landed
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 3) {
         if (lane == 0) {
             pm_commit(fin);
             mbar_wait(fin, 0);
