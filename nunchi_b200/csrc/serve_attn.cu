@@ -11,6 +11,7 @@
 #include "serve.h"
 
 #include <cuda_bf16.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cmath>
@@ -639,6 +640,30 @@ bool pa_shape_ok(int rows, int n_head, int n_head_kv, int head_dim, int prefix_l
            (int64_t) width * page + prefix_len + page <= INT32_MAX;
 }
 
+// the pages of K (or V) as rows of head_dim values, copied in boxes of up to 128 rows x 64 values with the 128-byte swizzle
+cudaError_t page_map_of(const imi_cuda_prefix_attn_args &a, const void *pages, CUtensorMap *out) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    static std::mutex mu;
+    {
+        std::lock_guard<std::mutex> g(mu);
+        if (!encode) {
+            void *fn = nullptr;
+            cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+            const cudaError_t r = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q);
+            if (r != cudaSuccess) return r;
+            if (q != cudaDriverEntryPointSuccess || !fn) return cudaErrorNotSupported;
+            encode = (PFN_cuTensorMapEncodeTiled_v12000) fn;
+        }
+    }
+    const cuuint64_t dims[2] = { (cuuint64_t) a.head_dim, (cuuint64_t) a.n_pages * a.n_head_kv * a.page },
+                     strides[1] = { (cuuint64_t) a.head_dim * 2 };
+    const cuuint32_t box[2] = { 64, (cuuint32_t) std::min(a.page, PM_N) }, es[2] = { 1, 1 };
+    const CUresult c = encode(out, a.type == IMI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                              (void *) pages, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return c == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <typename T, int D, bool R8>
 cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
     const imi_cuda_prefix_attn_args &a = p.a;
@@ -649,7 +674,10 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
                           (size_t) PA_DWARPS * ROWS * (D + 4) * 4, st, args);
     cudaError_t r = cudaSuccess;
     if (pl.mma) {
-        r = launch_pdl((const void *) k_pa_mma<T, D>, dim3(pl.grid), PM_THREADS, PmSmem<D>::TOTAL + 1024, st, args);
+        CUtensorMap km, vm;
+        if ((r = page_map_of(a, a.k_pages, &km)) != cudaSuccess || (r = page_map_of(a, a.v_pages, &vm)) != cudaSuccess) return r;
+        void *margs[] = { &p, &km, &vm };
+        r = launch_pdl((const void *) k_pa_mma<T, D>, dim3(pl.grid), PM_THREADS, PmSmem<D>::TOTAL + 1024, st, margs);
     } else if (pl.splits) {
         const int items = (a.rows * p.g + 15) / 16 * a.n_head_kv * pl.splits;
         r = launch_pdl((const void *) k_pa_pieces<T, D>, dim3(std::min(items, 148 * 16)), PA_WARPS * 32,
@@ -705,6 +733,7 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
     if (a->n_pages < 0 || a->window < 0) return set_error(IMI_E_ARG, "prefix_attn: negative n_pages or window");
     if (!std::isfinite(a->scale)) return set_error(IMI_E_ARG, "prefix_attn: scale is not finite");
     if (a->rows == 0) return IMI_OK;
+    if (((int64_t) a->n_pages * a->n_head_kv + 1) * a->page > INT32_MAX) return set_error(IMI_E_ARG, "prefix_attn: too many pages");
     if ((int64_t) a->rows * a->n_head / PM_ROWS * ((int64_t) a->prefix_len / PM_N + 1) > INT32_MAX / 4)
         return set_error(IMI_E_ARG, "prefix_attn: the prompt is too long for so many rows");
     if (!a->q || !a->out || !a->length || !a->work) return set_error(IMI_E_ARG, "prefix_attn: null argument");

@@ -9,8 +9,9 @@
 // is summed in 32 bits). At head_dim 64 S, P and O of both streams fill the 512 columns: QK(j+1) is issued as soon as S(j) is in
 // the softmax's registers. At 128 P takes S's place, and QK(j+1) goes directly behind PV(j), which reads it (products of one
 // thread run in the order of issue).
-//   warps 0..2   K and V rows from their pages by 16-byte asynchronous copies into rings of tiles (128-byte swizzle, rows of a
-//                page that does not exist or beyond the prompt's end zero-filled)
+//   warp 0       K and V rows from their pages by tensor copies of up to 128 rows x 128 bytes into rings of tiles (128-byte
+//                swizzle; the rows of a page that does not exist are read beyond the tensor's end, as zeros)
+//   warp 1       zeroes V's rows beyond the prompt's end in its last tile: what a page holds there may be anything
 //   warp 3       issues the products
 //   warps 4..7   softmax of stream 0, warps 8..11 of stream 1, with the registers that the others give up: a thread holds its
 //                row's 128 scores
@@ -22,7 +23,7 @@ constexpr int PM_M = 128, PM_N = 128, PM_ROWS = 2 * PM_M;
 constexpr int PM_MIN_ROWS = 16;        // query rows of a kv head up to which k_pa_pieces takes the prompt
 constexpr int PM_MIN_TILES = 2;        // position tiles of a piece at least
 constexpr int PM_MAX_TILES = 256;      // and at most (its page numbers are held in shared memory)
-constexpr int PM_COPY = 96, PM_THREADS = 12 * 32;
+constexpr int PM_THREADS = 12 * 32;
 constexpr int PM_REGS = 168, PM_REGS_FEW = 80, PM_REGS_MANY = 208;   // 4 x 80 + 8 x 208 <= 12 x 168
 constexpr float PM_RISE = 8.0f;
 
@@ -97,13 +98,9 @@ __device__ __forceinline__ void pm_st16(uint32_t t, const uint32_t (&u)[16]) {
 }
 __device__ __forceinline__ void pm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 16 bytes to shared memory, or 16 zero bytes
-__device__ __forceinline__ void pm_copy(uint32_t dst, const void *src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-
 template <typename T, int D>
-__global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant__ PaArgs p) {
+__global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant__ PaArgs p, const __grid_constant__ CUtensorMap k_map,
+                                                          const __grid_constant__ CUtensorMap v_map) {
     extern __shared__ __align__(1024) uint8_t sm_raw[];
     using L = PmSmem<D>;
     constexpr int NK = L::NK, NV = L::NV, CH = D / 8;
@@ -114,7 +111,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
     int *ids = (int *) (sm + L::IDS);
     uint64_t *k_full = (uint64_t *) (sm + L::BAR), *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV,
-             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *fin = o_full + 2;
+             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *v_raw = o_full + 2, *fin = v_raw + 1;
     __shared__ uint32_t tmem_at;
     __shared__ int stop;
     __shared__ int low_of;                                     // the lowest position that a row of the unit sees
@@ -122,9 +119,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     // it, in uniform registers: moved there for every product, issuing them took 2.5 us of a tile instead of 1
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
     if (tid == 0) {
-        for (int i = 0; i < NK; i++) { mbar_init(&k_full[i], PM_COPY); mbar_init(&k_free[i], 1); }
-        for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], PM_COPY); mbar_init(&v_free[i], 1); }
+        for (int i = 0; i < NK; i++) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], 1); }
+        for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
         for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&s_read[i], 128); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
+        mbar_init(v_raw, 1);
         mbar_init(fin, 1);
         stop = 0;
         fence_barrier_init();
@@ -149,7 +147,6 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         return false;
     };
     const int qrows = a.rows * p.g;
-    const long long ps = (long long) a.n_head_kv * a.page * D;
     const float sl2 = fabsf(p.sl2);                            // a negative scale turns q around
     const bool turn = p.sl2 < 0.0f;
     const int line = p.rtiles * a.n_head_kv * p.tiles, end = min(line, ((int) blockIdx.x + 1) * p.per);
@@ -214,55 +211,59 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PM_REGS_FEW));
-        if (warp < 3) {
+        if (warp == 0) {
             // ---------------- copies ----------------
-            int nk = 0, nv = 0;                                    // tiles gone through the rings
-            uint64_t *pending[3];
-            int np = 0;
-            auto flush = [&]() {                                   // everything issued has landed: say so
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_proxy_async();
-                for (int i = 0; i < np; i++) pm_arrive(pending[i]);
-                np = 0;
+            const int box = min(a.page, PM_N), boxes = PM_N / box, none = a.n_pages * a.n_head_kv * a.page;
+            int nk = 0, nv = 0;                                // tiles gone through the rings
+            auto load = [&](const CUtensorMap &map, int tile, uint8_t *dst, uint64_t *full) {
+                if (lane == 0) mbar_expect_tx(full, (uint32_t) L::TILE);
+                __syncwarp();
+                if (lane < boxes * (D / 64)) {                 // a box each: its rows, and which 64 dimensions
+                    const int b = lane % boxes, half = lane / boxes, pos = tile * PM_N + b * box;
+                    const int id = pos < a.prefix_len ? id_at(pos) : -1;
+                    const int y = id >= 0 ? (id * a.n_head_kv + w.kvh) * a.page + (pos & (a.page - 1)) : none;
+                    tma_load_2d(dst + half * (PM_N * 128) + b * box * 128, &map, 64 * half, y, full);
+                }
+                __syncwarp();
             };
             while (next(w)) {
-                const T *kb = (const T *) a.k_pages + (long long) w.kvh * a.page * D, *vb = (const T *) a.v_pages + (long long) w.kvh * a.page * D;
-                auto load = [&](const T *base, int tile, uint32_t dst, uint64_t *full) {
-    #pragma unroll 4
-                    for (int x = tid; x < PM_N * CH; x += PM_COPY) {
-                        const int r = x / CH, c = x % CH, pos = tile * PM_N + r;
-                        const bool in = pos < a.prefix_len;
-                        const int id = in ? id_at(pos) : -1;
-                        const T *src = base + (id >= 0 ? id : 0) * ps + (long long) (pos & (a.page - 1)) * D + 8 * c;
-                        pm_copy(dst + (c / 8) * (PM_N * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, id >= 0);
-                    }
-                    if (np == 2) {                                 // two tiles in flight: the older one is awaited
-                        asm volatile("cp.async.commit_group;\n cp.async.wait_group 2;" ::: "memory");
-                        fence_proxy_async();
-                        pm_arrive(pending[0]);
-                        pending[0] = pending[1];
-                        np = 1;
-                    } else {
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                    }
-                    pending[np++] = full;
-                };
-                auto room = [&](uint64_t *b, uint32_t parity) -> bool {
-                    if (mbar_try_wait(b, parity)) return true;
-                    flush();                                       // nothing landed may be held back while this waits
-                    return wait(b, parity);
-                };
-                for (int t = w.t0; t < w.t1; t++) {
+                bool ok = true;
+                for (int t = w.t0; t < w.t1 && ok; t++) {
                     const int ks = nk % NK, vs = nv % NV;
-                    if (!room(&k_free[ks], ((nk / NK) & 1) ^ 1)) break;
-                    load(kb, t, smem_u32(sm + L::K + ks * L::TILE), &k_full[ks]);
+                    ok = __all_sync(~0u, wait(&k_free[ks], ((nk / NK) & 1) ^ 1));
+                    if (!ok) break;
+                    load(k_map, t, sm + L::K + ks * L::TILE, &k_full[ks]);
                     nk++;
-                    if (!room(&v_free[vs], ((nv / NV) & 1) ^ 1)) break;
-                    load(vb, t, smem_u32(sm + L::V + vs * L::TILE), &v_full[vs]);
+                    ok = __all_sync(~0u, wait(&v_free[vs], ((nv / NV) & 1) ^ 1));
+                    if (!ok) break;
+                    load(v_map, t, sm + L::V + vs * L::TILE, (t + 1) * PM_N > a.prefix_len ? v_raw : &v_full[vs]);
                     nv++;
                 }
-                flush();
+                if (!ok) {                                     // copies in flight land before the memory goes (bounded)
+                    for (int i = 0; i < NK && i < nk; i++) mbar_wait(&k_full[(nk - 1 - i) % NK], ((nk - 1 - i) / NK) & 1);
+                    for (int i = 0; i < NV && i < nv; i++) mbar_wait(&v_full[(nv - 1 - i) % NV], ((nv - 1 - i) / NV) & 1);
+                }
             }
+        } else if (warp == 1) {
+            // ---------------- the prompt's end ----------------
+            int nv = 0, nr = 0;
+            while (next(w)) {
+                if (w.t1 > w.t0 && w.t1 * PM_N > a.prefix_len) {
+                    const int vs = (nv + w.t1 - 1 - w.t0) % NV, rows = a.prefix_len - (w.t1 - 1) * PM_N;
+                    if (__all_sync(~0u, wait(v_raw, nr & 1))) {
+                        uint8_t *v = sm + L::V + vs * L::TILE;
+                        for (int half = 0; half < D / 64; half++)
+                            for (int x = rows * 8 + lane; x < PM_N * 8; x += 32) *(uint4 *) (v + half * (PM_N * 128) + x * 16) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) pm_arrive(&v_full[vs]);
+                    }
+                    nr++;
+                }
+                nv += w.t1 - w.t0;
+            }
+        } else if (warp == 2) {
+            while (next(w)) {}
         } else if (warp == 3) {
             // ---------------- products ----------------
             int pn[2] = { 0, 0 }, rn[2] = { 0, 0 }, kn = 0, vn = 0;   // P and S tiles of the streams, tiles of the rings
