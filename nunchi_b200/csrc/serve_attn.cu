@@ -24,9 +24,11 @@ constexpr int PA_WARPS = 4;               // warps of a piece's CTA
 constexpr int PA_STEP = 16;               // positions of a warp's step (a page holds whole steps)
 constexpr int PA_MIN_STEPS = 2 * PA_WARPS;   // steps of a piece of the prompt at least
 constexpr int PO_MIN_STEPS = 4;           // of an own piece, which is one warp's
-constexpr int PO_CTAS = 592, PO_ITEMS = PO_CTAS * PA_WARPS;   // own CTAs: 148 SMs x 4; (piece, kv head) items aimed at: one per warp
+constexpr int PO_CTAS = 592;              // own CTAs at most: 148 SMs x 4. One (piece, kv head) item per warp is aimed at
 constexpr int PA_PRE_ITEMS = 592;         // (row tile, kv head, piece) items aimed at for the prompt: 148 SMs x 4
-constexpr int PA_DIRECT = 1024;           // positions (prompt and own) up to which one CTA takes a row alone
+constexpr int PA_DIRECT = 1024;           // positions (prompt and own) up to which one CTA takes a row alone: with few
+constexpr int PA_DIRECT_CTAS = 296;       // (row, kv head)s; with more only
+constexpr int PA_DIRECT_ALL = 256;        // up to these
 constexpr int PA_DWARPS = 8;              // its warps
 
 struct PaArgs {
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(PA_DWARPS * 32) k_pa_direct(const __grid_const
 
 // ---- pieces ----
 // own pieces of every row into off[0..rows] (shared memory): steps of 16 positions, `chunk` steps per piece, chosen so
-// that about PO_ITEMS (piece, kv head) items come out whatever the lengths are. Every CTA works this out from the
+// that about one (piece, kv head) item per warp comes out whatever the lengths are. Every CTA works this out from the
 // lengths (4 bytes per row from L2). Returns chunk.
 __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     const imi_cuda_prefix_attn_args &a = p.a;
@@ -407,7 +409,7 @@ __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     int total;
     scan(sum, total);
     const long long items = (long long) total * a.n_head_kv;
-    const int chunk = max(PO_MIN_STEPS, (int) ((items + PO_ITEMS - 1) / PO_ITEMS));
+    const int warps = gridDim.x * PA_WARPS, chunk = max(PO_MIN_STEPS, (int) ((items + warps - 1) / warps));
     int cnt = 0;
     for (int i = i0; i < i1; i++) cnt += (off[i + 1] + chunk - 1) / chunk;
     int at = scan(cnt, total);
@@ -627,7 +629,7 @@ PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len
         p.splits = (prefix_len + p.len - 1) / p.len;
     }
     p.pre_slots = (size_t) rows * n_head * p.splits;
-    p.own_slots = ((size_t) rows + (PO_ITEMS + n_head_kv - 1) / n_head_kv) * n_head;
+    p.own_slots = ((size_t) rows + (PO_CTAS * PA_WARPS + n_head_kv - 1) / n_head_kv) * n_head;
     p.off_bytes = ((size_t) (rows + 1) * 4 + 255) / 256 * 256;
     const size_t slots = p.pre_slots + p.own_slots;
     p.bytes = p.off_bytes + (slots * 8 + 255) / 256 * 256 + slots * head_dim * 4;
@@ -669,7 +671,8 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
     const imi_cuda_prefix_attn_args &a = p.a;
     constexpr int ROWS = R8 ? 8 : 16;
     void *args[] = { &p };
-    if ((long long) a.prefix_len + ((long long) a.width << p.shift) <= PA_DIRECT)
+    const long long most = (long long) a.prefix_len + ((long long) a.width << p.shift);
+    if (most <= PA_DIRECT_ALL || (most <= PA_DIRECT && a.rows * a.n_head_kv <= PA_DIRECT_CTAS))
         return launch_pdl((const void *) k_pa_direct<T, D, R8>, dim3(a.rows * a.n_head_kv), PA_DWARPS * 32,
                           (size_t) PA_DWARPS * ROWS * (D + 4) * 4, st, args);
     cudaError_t r = cudaSuccess;
@@ -684,7 +687,8 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
                        (size_t) PA_WARPS * 16 * (D + 4) * 4, st, args);
     }
     if (r == cudaSuccess)
-        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(PO_CTAS), PA_WARPS * 32, (size_t) (a.rows + 1) * 4, st, args);
+        // own CTAs do not fit an SM beside one of k_pa_mma's: where those are few, the others' SMs are enough
+        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(pl.mma && pl.grid <= 74 ? (148 - pl.grid) * 4 : PO_CTAS), PA_WARPS * 32, (size_t) (a.rows + 1) * 4, st, args);
     if (r == cudaSuccess) {
         // warps per (row, head): one up to 16 pieces, and while there are few of both
         int ways = 1;

@@ -27,10 +27,12 @@ constexpr int PM_THREADS = 12 * 32;
 constexpr int PM_REGS = 168, PM_REGS_FEW = 80, PM_REGS_MANY = 208;   // 4 x 80 + 8 x 208 <= 12 x 168
 constexpr float PM_RISE = 8.0f;
 
+constexpr int PM_OROW = 80;            // bytes from row to row where a warp turns its part of O around: 16 values and padding
+
 template <int D> struct PmSmem {
     static constexpr int TILE = PM_N * D * 2, NK = D == 64 ? 4 : 2, NV = D == 64 ? 4 : 2;
     static constexpr int Q = 0, K = Q + 2 * PM_M * D * 2, V = K + NK * TILE, IDS = V + NV * TILE,
-                         BAR = IDS + PM_MAX_TILES * (PM_N / 16) * 4, TOTAL = BAR + 256;
+                         OUT = IDS + PM_MAX_TILES * (PM_N / 16) * 4, BAR = OUT + 8 * 32 * PM_OROW, TOTAL = BAR + 256;
 };
 
 __device__ __forceinline__ void pm_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
     int *ids = (int *) (sm + L::IDS);
     uint64_t *k_full = (uint64_t *) (sm + L::BAR), *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV,
-             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *v_raw = o_full + 2, *fin = v_raw + 1;
+             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *v_raw = o_full + 2, *q_full = v_raw + 1, *fin = q_full + 1;
     __shared__ uint32_t tmem_at;
     __shared__ int stop;
     __shared__ int low_of;                                     // the lowest position that a row of the unit sees
@@ -123,6 +125,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
         for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&s_read[i], 128); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
         mbar_init(v_raw, 1);
+        mbar_init(q_full, 256);
         mbar_init(fin, 1);
         stop = 0;
         fence_barrier_init();
@@ -154,11 +157,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     struct Unit {
         int kvh, row0, piece, page0, t0, t1, n0, n1;           // position tiles [t0, t1), of them the streams'
     };
-    // the next unit's part, after the CTA is done with the one before: false where there is none
+    // the next unit's part, after the CTA is done with the one before: false where there is none. The page numbers are there
+    // for warps 0..3 when it returns; the queries when q_full says so (the copies need not wait for them)
     int fr = -1, lo = 0;                                       // softmax: the thread's row, and what it sees from
     auto next = [&](Unit &w) -> bool {
         if (__syncthreads_or(at >= end || *(volatile int *) &stop)) return false;
-        if (tid == 0) low_of = INT32_MAX;
         const int unit = at / p.tiles;
         w.piece = (int) blockIdx.x - unit * p.tiles / p.per;
         w.t0 = at - unit * p.tiles;
@@ -167,27 +170,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         w.kvh = unit / p.rtiles;
         w.row0 = (unit % p.rtiles) * (p.pair ? PM_M : PM_ROWS);
         w.page0 = (w.t0 * PM_N) >> p.shift;
-        __syncthreads();
-        if (warp >= 4) {                                       // the queries, and what their rows see
-            const int x = tid - 128;
-            fr = w.row0 + (p.pair ? x % PM_M : x);
-            if (fr >= qrows) fr = -1;
-            lo = fr >= 0 && a.window > 0 ? seen_of(p, fr / p.g).plo : 0;
-            const int least = __reduce_min_sync(~0u, fr >= 0 ? lo : INT32_MAX);
-            if (lane == 0) atomicMin(&low_of, least);
-            if (!p.pair || x < PM_M) {
-                uint8_t *dst = sm + L::Q + (x / PM_M) * (PM_M * D * 2);
-                const int r = x % PM_M;
-                const T *q = fr >= 0 ? (const T *) a.q + fr / p.g * a.q_stride + ((long long) w.kvh * p.g + fr % p.g) * D : nullptr;
-#pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    uint4 v = q ? ldg16(q + 8 * c) : make_uint4(0, 0, 0, 0);
-                    if (turn) { v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u; }
-                    *(uint4 *) (dst + (c / 8) * (PM_M * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-                }
-            }
-            fence_proxy_async();
-        } else {                                               // the pages of this part, -1 for one that does not exist
+        if (warp < 4) {                                        // the pages of this part, -1 for one that does not exist
             const int n = ((min(a.prefix_len, w.t1 * PM_N) - 1) >> p.shift) - w.page0 + 1;
             for (int i = tid; i < n; i += 128) {
                 int id = __ldg(a.prefix + w.page0 + i);
@@ -197,9 +180,39 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                 }
                 ids[i] = id;
             }
+        } else {                                               // the queries
+            const int x = tid - 128;
+            fr = w.row0 + (p.pair ? x % PM_M : x);
+            if (fr >= qrows) fr = -1;
+            if (!p.pair || x < PM_M) {
+                uint8_t *dst = sm + L::Q + (x / PM_M) * (PM_M * D * 2);
+                const int r = x % PM_M;
+                const T *q = fr >= 0 ? (const T *) a.q + fr / p.g * a.q_stride + ((long long) w.kvh * p.g + fr % p.g) * D : nullptr;
+                uint4 v[CH];
+#pragma unroll
+                for (int c = 0; c < CH; c++) v[c] = q ? ldg16(q + 8 * c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    if (turn) { v[c].x ^= 0x80008000u; v[c].y ^= 0x80008000u; v[c].z ^= 0x80008000u; v[c].w ^= 0x80008000u; }
+                    *(uint4 *) (dst + (c / 8) * (PM_M * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[c];
+                }
+            }
+            fence_proxy_async();
+            pm_arrive(q_full);
         }
-        __syncthreads();
-        w.t0 = max(w.t0, min(w.t1, __shfl_sync(~0u, low_of, 0) / PM_N));            // tiles that no row sees
+        if (a.window > 0) {                                    // what the rows see: tiles that none does are left out
+            if (tid == 0) low_of = INT32_MAX;
+            __syncthreads();
+            if (warp >= 4) {
+                lo = fr >= 0 ? seen_of(p, fr / p.g).plo : 0;
+                const int least = __reduce_min_sync(~0u, fr >= 0 ? lo : INT32_MAX);
+                if (lane == 0) atomicMin(&low_of, least);
+            }
+            __syncthreads();
+            w.t0 = max(w.t0, min(w.t1, __shfl_sync(~0u, low_of, 0) / PM_N));
+        } else if (warp < 4) {
+            asm volatile("bar.sync 1, 128;" ::: "memory");     // the page numbers
+        }
         const int tiles = w.t1 - w.t0;
         w.n0 = p.pair ? (tiles + 1) / 2 : tiles;
         w.n1 = p.pair ? tiles / 2 : tiles;
@@ -266,14 +279,14 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
             while (next(w)) {}
         } else if (warp == 3) {
             // ---------------- products ----------------
-            int pn[2] = { 0, 0 }, rn[2] = { 0, 0 }, kn = 0, vn = 0;   // P and S tiles of the streams, tiles of the rings
+            int units = 0, pn[2] = { 0, 0 }, rn[2] = { 0, 0 }, kn = 0, vn = 0;   // P and S tiles of the streams, tiles of the rings
             const uint32_t qk = pm_idesc<T>(PM_M, PM_N, false), pv = pm_idesc<T>(PM_M, D, true);
             // descriptors of the first tiles; the others' differ in the address alone (16-byte units, in the low bits)
             const uint64_t qd = pm_desc(smem_u32(sm + L::Q), 16, 1024), kd = pm_desc(smem_u32(sm + L::K), 16, 1024),
                            vd = pm_desc(smem_u32(sm + L::V), PM_N * 128, 1024);
             while (next(w)) {
                 const int n0 = w.n0, n1 = w.n1;
-                bool ok = true;
+                bool ok = __all_sync(~0u, wait(q_full, units++ & 1));
                 auto issue_qk = [&](int st, int j) {
                     const int n = kn + (p.pair ? 2 * j + st : j), ks = n % NK;
                     ok = ok && __all_sync(~0u, wait(&k_full[ks], (n / NK) & 1));
@@ -312,8 +325,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                     ok = ok && __all_sync(~0u, wait(&s_read[st], rn[st] & 1));
                     rn[st]++;
                 };
-                if (n0 > 0) issue_qk(0, 0);
-                if (n1 > 0) issue_qk(1, 0);
+                if (n0 > 0 && ok) issue_qk(0, 0);
+                if (n1 > 0 && ok) issue_qk(1, 0);
                 for (int j = 0; j < n0 && ok; j++) {
                     if (APART) {
                         read(0);
@@ -424,6 +437,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                 pm_fence_after();
             }
             if (fr >= 0) p.pml[slot] = make_float2(m, l);
+            // O by 16 dimensions through shared memory, so that four threads write a row's 64 bytes: a row per thread, every store
+            // would touch 32 lines (2.1 us of a piece against 0.5)
+            uint8_t *out = sm + L::OUT + (warp - 4) * 32 * PM_OROW;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 float o[32];
@@ -434,10 +450,22 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 32; e++) o[e] = 0.0f;
                 }
-                if (fr >= 0)
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *(float4 *) (p.po + slot * D + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                for (int h = 0; h < 2; h++) {
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        *(float4 *) (out + lane * PM_OROW + 16 * e) =
+                            make_float4(o[16 * h + 4 * e], o[16 * h + 4 * e + 1], o[16 * h + 4 * e + 2], o[16 * h + 4 * e + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int r = 8 * e + lane / 4;
+                        const long long s0 = __shfl_sync(~0u, fr >= 0 ? slot : -1ll, r);
+                        if (s0 >= 0)
+                            *(float4 *) (p.po + s0 * D + 32 * c + 16 * h + 4 * (lane % 4)) = *(const float4 *) (out + r * PM_OROW + 16 * (lane % 4));
+                    }
+                }
             }
             pm_fence_before();
             if (n > 0) no++;
