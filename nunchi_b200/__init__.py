@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -82,7 +83,7 @@ def lib():
         L.imi_cuda_bench_matvec.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_float),
                                             C.POINTER(C.c_size_t)]
         for f in ("page_map", "page_write", "prefix_attn", "sample"):
-            getattr(L, "imi_cuda_" + f).argtypes = [C.c_int, _vp, _vp]
+            getattr(L, "imi_cuda_" + f).argtypes = [C.c_int, C.c_char_p, _vp]
         L.imi_cuda_prefix_attn_work.argtypes = [C.c_int] * 7
         L.imi_cuda_prefix_attn_work.restype = C.c_size_t
         _L = L
@@ -339,106 +340,119 @@ def bench_matvec(rows: int, cols: int, ncol: int, reps: int = 20, device: int = 
     return float(ms.value), int(b.value)
 
 
-# ---- serving operators on device buffers (imi_cuda.h; arrays with data_ptr(), as torch tensors have) ----
-def _struct(name, fields):
-    return type(name, (C.Structure,), {"_fields_": fields})
+# ---- serving operators on device buffers (imi_cuda.h; torch tensors, or arrays that answer like them) ----
+# the argument blocks as C lays them out: pointers P, int i, int64 q, float f, size_t N
+_PAGE_MAP = struct.Struct("@PPiPqiPiPiiiiPPPPPP0P")
+_PAGE_WRITE = struct.Struct("@PPiqqiPiiPPiiiP0P")
+_PREFIX_ATTN = struct.Struct("@PiqiiiiPPiiPiPqiPfiPiqPPNP0P")
+_SAMPLE = struct.Struct("@PiqiiPPPPPPPP0P")
+_TYPE = {}   # torch's types to imi_cuda_type, filled when the first operator is called
+_F32 = _F16 = _BF16 = _I32 = _stream_of = None
 
 
-_I, _L64 = C.c_int, C.c_int64
-_PageMapArgs = _struct("_PageMapArgs", [
-    ("held", _vp), ("add", _vp), ("n", _I), ("table", _vp), ("table_stride", _L64), ("width", _I), ("free_pages", _vp),
-    ("free_cap", _I), ("n_free", _vp), ("page", _I), ("n_pages", _I), ("pos0", _I), ("cap", _I), ("start", _vp), ("length", _vp),
-    ("slots", _vp), ("pos", _vp), ("n_free_out", _vp), ("status", _vp)])
-_PageWriteArgs = _struct("_PageWriteArgs", [
-    ("k", _vp), ("v", _vp), ("type", _I), ("row_stride", _L64), ("head_stride", _L64), ("rows", _I), ("slots", _vp),
-    ("n_head_kv", _I), ("head_dim", _I), ("k_pages", _vp), ("v_pages", _vp), ("page_type", _I), ("page", _I), ("n_pages", _I),
-    ("status", _vp)])
-_PrefixAttnArgs = _struct("_PrefixAttnArgs", [
-    ("q", _vp), ("type", _I), ("q_stride", _L64), ("rows", _I), ("n_head", _I), ("n_head_kv", _I), ("head_dim", _I),
-    ("k_pages", _vp), ("v_pages", _vp), ("page", _I), ("n_pages", _I), ("prefix", _vp), ("prefix_len", _I), ("table", _vp),
-    ("table_stride", _L64), ("width", _I), ("length", _vp), ("scale", C.c_float), ("window", _I), ("out", _vp), ("out_type", _I),
-    ("out_stride", _L64), ("lse", _vp), ("work", _vp), ("work_bytes", C.c_size_t), ("status", _vp)])
-_SampleArgs = _struct("_SampleArgs", [
-    ("scores", _vp), ("type", _I), ("stride", _L64), ("n", _I), ("vocab", _I), ("u", _vp), ("temperature", _vp), ("top_k", _vp),
-    ("top_p", _vp), ("min_p", _vp), ("ids", _vp), ("logprob", _vp), ("kept", _vp)])
-_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+def _types():
+    global _F32, _F16, _BF16, _I32, _stream_of
+    import torch
+    _F32, _F16, _BF16, _I32 = torch.float32, torch.float16, torch.bfloat16, torch.int32
+    _TYPE.update({_F32: 0, _F16: 1, _BF16: 2})
+    # the current stream's handle; the call that gives it without a Stream object where this torch has one
+    _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def _bad(msg):
+    return ImiError(1, msg)
 
 
 def _type(t, name):
-    ty = _TYPES.get(str(t.dtype))
+    ty = _TYPE.get(t.dtype)
     if ty is None:
-        raise ImiError(1, f"{name}: type {t.dtype} is not float32, float16 or bfloat16")
+        raise _bad(f"{name}: type {t.dtype} is not float32, float16 or bfloat16")
     return ty
 
 
-def _vec(t, name, n, dtype="torch.int32"):
+def _vec(t, name, n, dtype):
     """The pointer of a contiguous array of at least n elements (None: null)."""
     if t is None:
-        return None
-    if str(t.dtype) != dtype or t.numel() < n or not t.is_contiguous():
-        raise ImiError(1, f"{name}: a contiguous {dtype} array of at least {n} elements is wanted")
+        return 0
+    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous():
+        raise _bad(f"{name}: a contiguous {dtype} array of at least {n} elements is wanted")
     return t.data_ptr()
 
 
 def _rows(t, name, dims):
-    """Checks that t has `dims` dimensions with its last one contiguous."""
-    if t.dim() != dims or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise ImiError(1, f"{name}: {dims} dimensions are wanted, the last one contiguous")
-    return t
+    """The strides of an array that has `dims` dimensions, the last one contiguous."""
+    st = t.stride()
+    if len(st) != dims or (st[-1] != 1 and t.shape[-1] > 1):
+        raise _bad(f"{name}: {dims} dimensions are wanted, the last one contiguous")
+    return st
+
+
+def _table(t, name, n):
+    st = _rows(t, name, 2)
+    rows, width = t.shape
+    if rows < n or t.dtype is not _I32:
+        raise _bad(f"{name}: an int32 row for each of {n} requests is wanted")
+    return t.data_ptr(), st[0] if rows > 1 else width, width
 
 
 def _pages(k, v):
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous():
-        raise ImiError(1, "k_pages, v_pages: two contiguous arrays [n_pages][n_head_kv][page][head_dim] are wanted")
-    return k.shape
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or k.dtype is not v.dtype or not k.is_contiguous() or not v.is_contiguous():
+        raise _bad("k_pages, v_pages: two contiguous arrays [n_pages][n_head_kv][page][head_dim] are wanted")
+    return shape
 
 
-def _launch(fn, like, args, stream):
+def _call(fn, like, args, stream):
     """Calls the operator on like's device, on `stream` (a torch stream or a handle; None: torch's current one)."""
-    dev = like.device.index
-    if like.device.type != "cuda":
-        raise ImiError(1, "the serving operators work on device arrays")
+    dev = like.get_device()
+    if dev < 0:
+        raise _bad("the serving operators work on device arrays")
     if stream is None:
-        import torch
-        stream = torch.cuda.current_stream(dev).cuda_stream
-    _check(fn(dev, C.addressof(args), getattr(stream, "cuda_stream", stream)))
+        stream = _stream_of(dev)
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    st = fn(dev, args, stream)
+    if st:
+        _check(st)
 
 
 def page_map(held, add, table, free_pages, n_free, *, page, n_pages, start, length, slots, pos, n_free_out, status, pos0=0,
              stream=None):
     """Block tables and slot maps from the requests' lengths (imi_cuda_page_map): all arrays int32 on one device, table
     [n][width]; writes table's new entries, start, length, slots, pos and n_free_out."""
-    n, cap = held.shape[0], slots.numel()
-    _rows(table, "table", 2)
-    if table.shape[0] < n or str(table.dtype) != "torch.int32":
-        raise ImiError(1, "table: an int32 row for every request is wanted")
-    a = _PageMapArgs(_vec(held, "held", n), _vec(add, "add", n), n, table.data_ptr(), table.stride(0), table.shape[1],
-                     _vec(free_pages, "free_pages", 0), free_pages.numel(), _vec(n_free, "n_free", 1), page, n_pages, pos0, cap,
-                     _vec(start, "start", n + 1), _vec(length, "length", n), _vec(slots, "slots", cap), _vec(pos, "pos", cap),
-                     _vec(n_free_out, "n_free_out", 1), _vec(status, "status", 2))
-    _launch(lib().imi_cuda_page_map, held, a, stream)
+    if not _TYPE:
+        _types()
+    i32, n, cap = _I32, held.shape[0], slots.numel()
+    tp, ts, width = _table(table, "table", n)
+    _call(lib().imi_cuda_page_map, held, _PAGE_MAP.pack(
+        _vec(held, "held", n, i32), _vec(add, "add", n, i32), n, tp, ts, width, _vec(free_pages, "free_pages", 0, i32),
+        free_pages.numel(), _vec(n_free, "n_free", 1, i32), page, n_pages, pos0, cap, _vec(start, "start", n + 1, i32),
+        _vec(length, "length", n, i32), _vec(slots, "slots", cap, i32), _vec(pos, "pos", cap, i32),
+        _vec(n_free_out, "n_free_out", 1, i32), _vec(status, "status", 2, i32)), stream)
 
 
 def page_write(k, v, slots, k_pages, v_pages, *, status=None, stream=None):
     """K and V rows [rows][n_head_kv][head_dim] (any row and head strides, the same for both) to the slots' places in the
     pages [n_pages][n_head_kv][page][head_dim] (imi_cuda_page_write)."""
+    if not _TYPE:
+        _types()
     n_pages, kv, page, d = _pages(k_pages, v_pages)
-    _rows(k, "k", 3)
-    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or tuple(k.shape[1:]) != (kv, d):
-        raise ImiError(1, "k, v: rows of the pages' heads, with the same type and strides, are wanted")
-    a = _PageWriteArgs(k.data_ptr(), v.data_ptr(), _type(k, "k"), k.stride(0), k.stride(1), k.shape[0],
-                       _vec(slots, "slots", k.shape[0]), kv, d, k_pages.data_ptr(), v_pages.data_ptr(), _type(k_pages, "k_pages"), page,
-                       n_pages, _vec(status, "status", 1))
-    _launch(lib().imi_cuda_page_write, k_pages, a, stream)
+    st = _rows(k, "k", 3)
+    rows, h, dd = k.shape
+    if k.shape != v.shape or v.stride() != st or k.dtype is not v.dtype or h != kv or dd != d:
+        raise _bad("k, v: rows of the pages' heads, with the same type and strides, are wanted")
+    _call(lib().imi_cuda_page_write, k_pages, _PAGE_WRITE.pack(
+        k.data_ptr(), v.data_ptr(), _type(k, "k"), st[0], st[1], rows, _vec(slots, "slots", rows, _I32), kv, d, k_pages.data_ptr(),
+        v_pages.data_ptr(), _type(k_pages, "k_pages"), page, n_pages, _vec(status, "status", 1, _I32)), stream)
 
 
 def prefix_attn_work(q, k_pages, prefix_len, table):
     """A workspace for prefix_attn calls of these shapes (imi_cuda_prefix_attn_work bytes)."""
+    import torch
     _, kv, page, d = k_pages.shape
     n = lib().imi_cuda_prefix_attn_work(q.shape[0], q.shape[1], kv, d, prefix_len, table.shape[1], page)
     if n == 0:
-        raise ImiError(1, "prefix_attn: unsupported shape")
-    import torch
+        raise _bad("prefix_attn: unsupported shape")
     return torch.empty(n, dtype=torch.uint8, device=q.device)
 
 
@@ -447,35 +461,38 @@ def prefix_attn(q, k_pages, v_pages, prefix, prefix_len, table, length, *, out, 
     """Attention of one token per conversation, q [rows][n_head][head_dim], over the prompt in the pages `prefix` and each
     conversation's own pages table[rows][width], length[rows] positions of them (imi_cuda_prefix_attn); writes out
     [rows][n_head][head_dim] and lse [rows][n_head]. scale None: head_dim ** -0.5."""
+    if not _TYPE:
+        _types()
     n_pages, kv, page, d = _pages(k_pages, v_pages)
-    rows, heads = _rows(q, "q", 3).shape[:2]
-    for t, name in ((q, "q"), (_rows(out, "out", 3), "out")):
-        if t.shape != (rows, heads, d) or (heads > 1 and t.stride(1) != d):
-            raise ImiError(1, f"{name}: [rows][n_head][head_dim] with contiguous heads is wanted")
-    if q.dtype != k_pages.dtype:
-        raise ImiError(1, "q and the pages have one type")
-    _rows(table, "table", 2)
-    if table.shape[0] < rows or str(table.dtype) != "torch.int32":
-        raise ImiError(1, "table: an int32 row for every conversation is wanted")
-    span = heads * d   # the stride of a single row does not matter
-    a = _PrefixAttnArgs(q.data_ptr(), _type(q, "q"), q.stride(0) if rows > 1 else span, rows, heads, kv, d, k_pages.data_ptr(),
-                        v_pages.data_ptr(), page, n_pages, _vec(prefix, "prefix", (prefix_len + page - 1) // page) or None, prefix_len,
-                        table.data_ptr() or None, table.stride(0) if rows > 1 else table.shape[1], table.shape[1],
-                        _vec(length, "length", rows), d ** -0.5 if scale is None else scale, window, out.data_ptr(), _type(out, "out"),
-                        out.stride(0) if rows > 1 else span, _vec(lse, "lse", rows * heads, "torch.float32"), work.data_ptr(),
-                        work.numel() * work.element_size(), _vec(status, "status", 1))
-    _launch(lib().imi_cuda_prefix_attn, q, a, stream)
+    qs, os_ = _rows(q, "q", 3), _rows(out, "out", 3)
+    shape = q.shape
+    rows, heads, dd = shape
+    if dd != d or out.shape != shape or (heads > 1 and (qs[1] != d or os_[1] != d)):
+        raise _bad("q, out: [rows][n_head][head_dim] with contiguous heads of the pages' size are wanted")
+    if q.dtype is not k_pages.dtype:
+        raise _bad("q and the pages have one type")
+    tp, ts, width = _table(table, "table", rows)
+    one = heads * d if rows <= 1 else 0   # the stride of a single row does not matter
+    _call(lib().imi_cuda_prefix_attn, q, _PREFIX_ATTN.pack(
+        q.data_ptr(), _type(q, "q"), one or qs[0], rows, heads, kv, d, k_pages.data_ptr(), v_pages.data_ptr(), page, n_pages,
+        _vec(prefix, "prefix", (prefix_len + page - 1) // page, _I32), prefix_len, tp, ts, width, _vec(length, "length", rows, _I32),
+        d ** -0.5 if scale is None else scale, window, out.data_ptr(), _type(out, "out"), one or os_[0],
+        _vec(lse, "lse", rows * heads, _F32), work.data_ptr(), work.numel() * work.element_size(), _vec(status, "status", 1, _I32)),
+        stream)
 
 
 def sample(scores, u, *, ids, temperature=None, top_k=None, top_p=None, min_p=None, logprob=None, kept=None, stream=None):
     """A word per row of scores [n][vocab] by temperature, top-k, top-p and min-p (arrays of n, None: off) from the uniform
     numbers u[n] (imi_cuda_sample); writes ids (and logprob, kept)."""
-    n, vocab = _rows(scores, "scores", 2).shape
-    f = "torch.float32"
-    a = _SampleArgs(scores.data_ptr(), _type(scores, "scores"), scores.stride(0), n, vocab, _vec(u, "u", n, f),
-                    _vec(temperature, "temperature", n, f), _vec(top_k, "top_k", n), _vec(top_p, "top_p", n, f),
-                    _vec(min_p, "min_p", n, f), _vec(ids, "ids", n), _vec(logprob, "logprob", n, f), _vec(kept, "kept", n))
-    _launch(lib().imi_cuda_sample, scores, a, stream)
+    if not _TYPE:
+        _types()
+    f, i32 = _F32, _I32
+    st = _rows(scores, "scores", 2)
+    n, vocab = scores.shape
+    _call(lib().imi_cuda_sample, scores, _SAMPLE.pack(
+        scores.data_ptr(), _type(scores, "scores"), st[0], n, vocab, _vec(u, "u", n, f), _vec(temperature, "temperature", n, f),
+        _vec(top_k, "top_k", n, i32), _vec(top_p, "top_p", n, f), _vec(min_p, "min_p", n, f), _vec(ids, "ids", n, i32),
+        _vec(logprob, "logprob", n, f), _vec(kept, "kept", n, i32)), stream)
 
 
 class Seoul:

@@ -533,7 +533,8 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, 
     pdl_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, way = warp % ways;
     const int x = blockIdx.x * (8 / ways) + warp / ways, i = x / a.n_head, h = x % a.n_head;
-    const bool live = i < a.rows && a.length[min(i, a.rows - 1)] >= 0;
+    const int ic = min(i, a.rows - 1), len = a.length[ic], o0 = p.off[ic], o1 = p.off[ic + 1];
+    const bool live = i < a.rows && len >= 0;
     float m = -INFINITY, l = 0.0f;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     // D / 4 lanes hold four dimensions each; at D 64 the warp's halves take every other piece
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, 
             const int u0 = (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.tiles;
             np = ((u0 + p.tiles - 1) / p.per - u0 / p.per + 1) * (p.pair ? 2 : 1);
         }
-        const int o0 = p.off[i], n = np + p.off[i + 1] - o0;
+        const int n = np + o1 - o0;
         auto slot_of = [&](int k) -> long long {
             return k < np ? (long long) x * p.pre_splits + k : p.own_slot0 + (long long) (o0 + k - np) * a.n_head + h;
         };

@@ -26,13 +26,15 @@ constexpr int PM_MAX_TILES = 256;      // and at most (its page numbers are held
 constexpr int PM_THREADS = 12 * 32;
 constexpr int PM_REGS = 168, PM_REGS_FEW = 80, PM_REGS_MANY = 208;   // 4 x 80 + 8 x 208 <= 12 x 168
 constexpr float PM_RISE = 8.0f;
+constexpr int PM_HAND = 2;              // of four parts of a tile's exponentials, the one behind which the other stream begins
+constexpr int PM_POLY = 4;              // every PM_POLY-th pair's exponentials by the FMA units
 
 constexpr int PM_OROW = 80;            // bytes from row to row where a warp turns its part of O around: 16 values and padding
 
 template <int D> struct PmSmem {
     static constexpr int TILE = PM_N * D * 2, NK = D == 64 ? 4 : 2, NV = D == 64 ? 4 : 2;
     static constexpr int Q = 0, K = Q + 2 * PM_M * D * 2, V = K + NK * TILE, IDS = V + NV * TILE,
-                         OUT = IDS + PM_MAX_TILES * (PM_N / 16) * 4, BAR = OUT + 8 * 32 * PM_OROW, TOTAL = BAR + 256;
+                         OUT = IDS + PM_MAX_TILES * (PM_N / 16) * 4, BAR = OUT + 8 * 32 * PM_OROW, TOTAL = BAR + 512;
 };
 
 __device__ __forceinline__ void pm_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
@@ -100,6 +102,21 @@ __device__ __forceinline__ void pm_st16(uint32_t t, const uint32_t (&u)[16]) {
 }
 __device__ __forceinline__ void pm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 2^x for a pair by the FMA units: n the nearest integer, 2^(x - n) by the polynomial through its values at 6 Chebyshev nodes
+// (relative error below 2^-21, ex2.approx's is 2^-22), n into the exponent. Below 2^-126: about 2^-126
+__device__ __forceinline__ float2 pm_exp2(float2 x) {
+    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+    const float2 b = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f)),   // 1.5 * 2^23: n in the low bits
+                 n = __fadd2_rn(b, make_float2(-12582912.0f, -12582912.0f)), f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
+    float2 e = __ffma2_rn(f, make_float2(0.0013390863f, 0.0013390863f), make_float2(0.009676032f, 0.009676032f));
+    e = __ffma2_rn(f, e, make_float2(0.05550357f, 0.05550357f));
+    e = __ffma2_rn(f, e, make_float2(0.24022107f, 0.24022107f));
+    e = __ffma2_rn(f, e, make_float2(0.6931472f, 0.6931472f));
+    e = __ffma2_rn(f, e, make_float2(1.0f, 1.0f));
+    return make_float2(__int_as_float(__float_as_int(e.x) + (__float_as_int(b.x) << 23)),
+                       __int_as_float(__float_as_int(e.y) + (__float_as_int(b.y) << 23)));
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant__ PaArgs p, const __grid_constant__ CUtensorMap k_map,
                                                           const __grid_constant__ CUtensorMap v_map) {
@@ -113,7 +130,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
     int *ids = (int *) (sm + L::IDS);
     uint64_t *k_full = (uint64_t *) (sm + L::BAR), *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV,
-             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *v_raw = o_full + 2, *q_full = v_raw + 1, *fin = q_full + 1;
+             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *v_raw = o_full + 2, *q_full = v_raw + 1, *fin = q_full + 1,
+             *turn_of = fin + 1;                               // [stream][warp]: the warp may begin its exponentials
     __shared__ uint32_t tmem_at;
     __shared__ int stop;
     __shared__ int low_of;                                     // the lowest position that a row of the unit sees
@@ -124,6 +142,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         for (int i = 0; i < NK; i++) { mbar_init(&k_full[i], 1); mbar_init(&k_free[i], 1); }
         for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
         for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&s_read[i], 128); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
+        for (int i = 0; i < 8; i++) mbar_init(&turn_of[i], 1);
         mbar_init(v_raw, 1);
         mbar_init(q_full, 256);
         mbar_init(fin, 1);
@@ -349,7 +368,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         const int st = (warp - 4) / 4;
         const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16, S = tmem + TM_S + st * PM_N + lanes,
                        P = tmem + TM_P + st * P_STEP + lanes, O = tmem + TM_O + st * D + lanes;
-        int ns = 0, no = 0;                                    // S tiles, and O's commits, of this stream
+        // The two warps of a scheduler, one of each stream, begin their exponentials in turn: in step, both would wait for the
+        // same unit and then both for their products. With a quarter of them on the FMA units, 1.77 us of two streams' tile went to
+        // 1.53 at head_dim 64; at 128, which waits for its products (P over S), neither made a difference, and both are left out
+        uint64_t *my_turn = &turn_of[4 * st + (warp & 3)], *their_turn = &turn_of[4 * (1 - st) + (warp & 3)];
+        int ns = 0, no = 0, nt = 0;                            // S tiles, O's commits, and turns, of this stream
         while (next(w)) {
             const int n = st ? w.n1 : w.n0;
             float m = -INFINITY, l = 0.0f;
@@ -409,6 +432,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                         }
                     }
                 }
+                if (APART && (st == 1 || j > 0)) {
+                    ok = __all_sync(~0u, wait(my_turn, nt & 1));
+                    nt++;
+                    if (!ok) break;
+                }
                 const float u = m == -INFINITY ? 0.0f : -m;
                 const float2 s2 = make_float2(sl2, sl2), u2 = make_float2(u, u);
                 float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
@@ -418,11 +446,12 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const float2 x = __ffma2_rn(make_float2(v[32 * c + 2 * e], v[32 * c + 2 * e + 1]), s2, u2);
-                        const float2 y = make_float2(ex2(x.x), ex2(x.y));
+                        const float2 y = APART && e % PM_POLY == PM_POLY - 1 ? pm_exp2(x) : make_float2(ex2(x.x), ex2(x.y));
                         sum[e & 1] = __fadd2_rn(sum[e & 1], y);
                         pk[e] = Half2<T>::pack(y.x, y.y);
                     }
                     pm_st16(P + 16 * c, pk);
+                    if (APART && c == PM_HAND && lane == 0 && (st == 0 ? j < w.n1 : j + 1 < w.n0)) pm_arrive(their_turn);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 pm_wait_st();

@@ -1,6 +1,8 @@
 """The serving operators' refusals on the host: every bad argument is IMI_E_ARG with a message before any device work, and
 good ones without a device are IMI_E_NODEV. No GPU needed (the pointers are never followed)."""
-import ctypes as C
+import os
+import struct
+import subprocess
 
 import pytest
 
@@ -9,9 +11,9 @@ import nunchi_b200 as nb
 P = 0x10000   # an aligned address that is never read
 
 
-def call(name, cls, good, **bad):
-    a = cls(**{**good, **bad})
-    st = getattr(nb.lib(), name)(0, C.addressof(a), None)
+def call(name, block, good, device=0, **bad):
+    a = block.pack(*(v or 0 for v in {**good, **bad}.values()))
+    st = getattr(nb.lib(), "imi_cuda_" + name)(device, a, None)
     return st, nb.lib().imi_cuda_error().decode()
 
 
@@ -31,7 +33,7 @@ SAMPLE = dict(scores=P, type=0, stride=1000, n=3, vocab=1000, u=P, temperature=P
     dict(n_pages=0), dict(n_pages=1 << 28), dict(width=0), dict(table_stride=7), dict(cap=-1), dict(free_cap=-1), dict(free_pages=None),
     dict(pos0=-1), dict(pos0=2 ** 31 - 10), dict(held=P + 2), dict(status=P + 1)])
 def test_page_map_refuses(bad):
-    st, msg = call("imi_cuda_page_map", nb._PageMapArgs, MAP, **bad)
+    st, msg = call("page_map", nb._PAGE_MAP, MAP, **bad)
     assert st == 1 and "page_map" in msg
 
 
@@ -40,7 +42,7 @@ def test_page_map_refuses(bad):
     dict(head_dim=264), dict(page=48), dict(n_pages=0), dict(k=None), dict(v=None), dict(slots=None), dict(k_pages=None), dict(v_pages=None),
     dict(row_stride=-1), dict(head_stride=-1), dict(k=P + 2), dict(k_pages=P + 8), dict(slots=P + 2)])
 def test_page_write_refuses(bad):
-    st, msg = call("imi_cuda_page_write", nb._PageWriteArgs, WRITE, **bad)
+    st, msg = call("page_write", nb._PAGE_WRITE, WRITE, **bad)
     assert st == 1 and "page_write" in msg
 
 
@@ -52,7 +54,7 @@ def test_page_write_refuses(bad):
     dict(q_stride=2052), dict(out_stride=2040), dict(out_stride=2050), dict(q=P + 8), dict(k_pages=P + 2), dict(out=P + 4), dict(work=P + 8),
     dict(lse=P + 2), dict(work_bytes=100), dict(prefix_len=2 ** 31 - 1)])
 def test_prefix_attn_refuses(bad):
-    st, msg = call("imi_cuda_prefix_attn", nb._PrefixAttnArgs, ATTN, **bad)
+    st, msg = call("prefix_attn", nb._PREFIX_ATTN, ATTN, **bad)
     assert st == 1 and "prefix_attn" in msg
 
 
@@ -71,7 +73,7 @@ def test_prefix_attn_work():
     dict(n=-1), dict(n=65536), dict(vocab=0), dict(vocab=262145, stride=300000), dict(type=3), dict(scores=None), dict(u=None), dict(ids=None),
     dict(stride=999), dict(scores=P + 2), dict(top_k=P + 1), dict(kept=P + 2)])
 def test_sample_refuses(bad):
-    st, msg = call("imi_cuda_sample", nb._SampleArgs, SAMPLE, **bad)
+    st, msg = call("sample", nb._SAMPLE, SAMPLE, **bad)
     assert st == 1 and "sample" in msg
 
 
@@ -81,8 +83,28 @@ def test_null_argument_blocks():
 
 
 def test_no_such_device():
-    for name, cls, good in (("imi_cuda_page_map", nb._PageMapArgs, MAP), ("imi_cuda_page_write", nb._PageWriteArgs, WRITE),
-                            ("imi_cuda_prefix_attn", nb._PrefixAttnArgs, ATTN), ("imi_cuda_sample", nb._SampleArgs, SAMPLE)):
-        a = cls(**good)
+    for name, block, good in (("page_map", nb._PAGE_MAP, MAP), ("page_write", nb._PAGE_WRITE, WRITE), ("prefix_attn", nb._PREFIX_ATTN, ATTN),
+                              ("sample", nb._SAMPLE, SAMPLE)):
         for device in (-1, 4096):
-            assert getattr(nb.lib(), name)(device, C.addressof(a), None) == 8
+            assert call(name, block, good, device)[0] == 8
+
+
+def test_argument_blocks_match_the_header(tmp_path):
+    """The blocks that the Python binding packs are laid out as the C compiler lays the header's out: every field at its place."""
+    names = {"page_map": (nb._PAGE_MAP, MAP), "page_write": (nb._PAGE_WRITE, WRITE), "prefix_attn": (nb._PREFIX_ATTN, ATTN), "sample": (nb._SAMPLE, SAMPLE)}
+    src = '#include "imi_cuda.h"\n#include <stddef.h>\n#include <stdio.h>\nint main(void) {\n'
+    for n, (_, good) in names.items():
+        src += f'printf("%zu", sizeof(imi_cuda_{n}_args));\n'
+        src += "".join(f'printf(" %zu", offsetof(imi_cuda_{n}_args, {f}));\n' for f in good) + 'puts("");\n'
+    c, exe = tmp_path / "t.c", tmp_path / "t"
+    c.write_text(src + "return 0; }\n")
+    inc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I", inc, str(c), "-o", str(exe)], check=True)
+    lines = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+    for line, (n, (block, good)) in zip(lines, names.items()):
+        size, *offsets = map(int, line.split())
+        assert block.size == size, n
+        fmt, at = block.format[1:-2], []
+        for k in range(len(fmt)):
+            at.append(struct.calcsize("@" + fmt[:k] + "0" + fmt[k]))
+        assert at == offsets, n
