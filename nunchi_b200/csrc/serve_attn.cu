@@ -24,7 +24,8 @@ constexpr int PA_WARPS = 4;               // warps of a piece's CTA
 constexpr int PA_STEP = 16;               // positions of a warp's step (a page holds whole steps)
 constexpr int PA_MIN_STEPS = 2 * PA_WARPS;   // steps of a piece of the prompt at least
 constexpr int PO_MIN_STEPS = 4;           // of an own piece, which is one warp's
-constexpr int PO_CTAS = 592;              // own CTAs at most: 148 SMs x 4. One (piece, kv head) item per warp is aimed at
+constexpr int PO_ITEM_COST = 4, PO_ROUNDS = 3;   // own_plan
+constexpr int PO_CTAS(int d) { return d == 64 ? 592 : 296; }   // own CTAs: as many as 148 SMs hold (4 and 2: registers)
 constexpr int PA_PRE_ITEMS = 592;         // (row tile, kv head, piece) items aimed at for the prompt: 148 SMs x 4
 constexpr int PA_DIRECT = 1024;           // positions (prompt and own) up to which one CTA takes a row alone: with few
 constexpr int PA_DIRECT_CTAS = 296;       // (row, kv head)s; with more only
@@ -374,45 +375,55 @@ __global__ void __launch_bounds__(PA_DWARPS * 32) k_pa_direct(const __grid_const
 }
 
 // ---- pieces ----
-// own pieces of every row into off[0..rows] (shared memory): steps of 16 positions, `chunk` steps per piece, chosen so
-// that about one (piece, kv head) item per warp comes out whatever the lengths are. Every CTA works this out from the
-// lengths (4 bytes per row from L2). Returns chunk.
+// own pieces of every row into off[0..rows] (shared memory): steps of 16 positions, `chunk` steps per piece. A warp takes one
+// (piece, kv head) item after the other, so the time is rounds x (chunk + what an item costs beside its steps, about
+// PO_ITEM_COST). Either a chunk so long that one round does, or PO_ROUNDS rounds of short ones, which the rows' last pieces and
+// their different lengths do less harm. Every CTA works this out from the lengths (4 bytes per row from L2). Returns chunk.
 __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     const imi_cuda_prefix_attn_args &a = p.a;
-    const int tid = threadIdx.x, nt = blockDim.x, per = (a.rows + nt - 1) / nt, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
-    int sum = 0;
+    const int tid = threadIdx.x, nt = PA_WARPS * 32, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.rows + nt - 1) / nt, i0 = min(a.rows, tid * per), i1 = min(a.rows, i0 + per);
+    int sum = 0, most = 0, live = 0;
     for (int i = i0; i < i1; i++) {
         const Seen v = seen_of(p, i);
         const int steps = v.len > v.olo ? (v.len + PA_STEP - 1) / PA_STEP - v.olo / PA_STEP : 0;
         off[i + 1] = steps;
         sum += steps;
+        most = max(most, steps);
+        live += steps > 0;
     }
-    auto scan = [&](int x, int &total) {   // exclusive sum over the threads
-        const int lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
-        int y = x;
+    sum = __reduce_add_sync(~0u, sum);
+    most = __reduce_max_sync(~0u, most);
+    live = __reduce_add_sync(~0u, live);
+    if (lane == 0) { tmp[3 * warp] = sum; tmp[3 * warp + 1] = most; tmp[3 * warp + 2] = live; }
+    __syncthreads();
+    sum = most = live = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(~0u, y, o);
-            if (lane >= o) y += z;
-        }
-        __syncthreads();
-        if (lane == 31) tmp[warp] = y;
-        __syncthreads();
-        int before = 0;
-        total = 0;
-        for (int w = 0; w < nw; w++) {
-            if (w < warp) before += tmp[w];
-            total += tmp[w];
-        }
-        return before + y - x;
-    };
-    int total;
-    scan(sum, total);
-    const long long items = (long long) total * a.n_head_kv;
-    const int warps = gridDim.x * PA_WARPS, chunk = max(PO_MIN_STEPS, (int) ((items + warps - 1) / warps));
+    for (int w = 0; w < PA_WARPS; w++) {
+        sum += tmp[3 * w];
+        most = max(most, tmp[3 * w + 1]);
+        live += tmp[3 * w + 2];
+    }
+    const long long warps = (long long) gridDim.x * PA_WARPS, work = (long long) sum * a.n_head_kv, rows = (long long) live * a.n_head_kv;
+    // one round: at most work / chunk + rows items
+    const int one = rows < warps ? (int) min((long long) max(1, most), (work + warps - rows - 1) / (warps - rows)) : INT32_MAX;
+    int chunk = max(PO_MIN_STEPS, (int) ((work + PO_ROUNDS * warps - 1) / (PO_ROUNDS * warps)));
+    const long long rounds = (work / chunk + rows + warps - 1) / warps;
+    if (one < INT32_MAX && one + PO_ITEM_COST <= rounds * (chunk + PO_ITEM_COST)) chunk = max(PO_MIN_STEPS, one);
     int cnt = 0;
     for (int i = i0; i < i1; i++) cnt += (off[i + 1] + chunk - 1) / chunk;
-    int at = scan(cnt, total);
+    int at = cnt;   // exclusive sums over the threads
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(~0u, at, o);
+        if (lane >= o) at += z;
+    }
+    if (lane == 31) tmp[16 + warp] = at;
+    __syncthreads();
+    at -= cnt;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; w++)
+        if (w < warp) at += tmp[16 + w];
     for (int i = i0; i < i1; i++) {
         at += (off[i + 1] + chunk - 1) / chunk;
         off[i + 1] = at;
@@ -630,7 +641,7 @@ PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len
         p.splits = (prefix_len + p.len - 1) / p.len;
     }
     p.pre_slots = (size_t) rows * n_head * p.splits;
-    p.own_slots = ((size_t) rows + (PO_CTAS * PA_WARPS + n_head_kv - 1) / n_head_kv) * n_head;
+    p.own_slots = ((size_t) rows + (PO_ROUNDS * PO_CTAS(head_dim) * PA_WARPS + n_head_kv - 1) / n_head_kv) * n_head;
     p.off_bytes = ((size_t) (rows + 1) * 4 + 255) / 256 * 256;
     const size_t slots = p.pre_slots + p.own_slots;
     p.bytes = p.off_bytes + (slots * 8 + 255) / 256 * 256 + slots * head_dim * 4;
@@ -689,11 +700,11 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
     }
     if (r == cudaSuccess)
         // own CTAs do not fit an SM beside one of k_pa_mma's: where those are few, the others' SMs are enough
-        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(pl.mma && pl.grid <= 74 ? (148 - pl.grid) * 4 : PO_CTAS), PA_WARPS * 32, (size_t) (a.rows + 1) * 4, st, args);
+        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(pl.mma && pl.grid <= 74 ? PO_CTAS(D) / 148 * (148 - pl.grid) : PO_CTAS(D)), PA_WARPS * 32, (size_t) (a.rows + 1) * 4, st, args);
     if (r == cudaSuccess) {
-        // warps per (row, head): one up to 16 pieces, and while there are few of both
+        // warps per (row, head): one up to 16 pieces of the prompt; more while the SMs hold them (148 x 64 warps)
         int ways = 1;
-        while (ways < 8 && (pl.splits > 16 * ways || (a.rows * a.n_head * ways < 1184 && pl.splits > 2 * ways))) ways *= 2;
+        while (ways < 8 && (pl.splits > 16 * ways || a.rows * a.n_head * ways < 4736)) ways *= 2;
         void *jargs[] = { &p, &ways };
         r = launch_pdl((const void *) k_join<D>, dim3((a.rows * a.n_head * ways + 7) / 8), 256, 0, st, jargs);
     }
