@@ -114,6 +114,8 @@ __device__ __forceinline__ Seen seen_of(const PaArgs &p, int i) {
 // positions of one dimension in a register: lane (w = lane / 4, t) loads the 16 bytes 8w..8w+7 of positions 2t, 2t+1,
 // 2t+8, 2t+9 and pairs them with byte permutes; product j then holds dimension 8n + j at its column n. Nothing passes
 // through shared memory. R8: at most 8 query rows (the fragment's upper rows are zero and not kept).
+constexpr int PO_STAGES = 3;              // steps of own positions in a warp's ring
+
 template <typename T, int D, bool R8>
 struct Pass {
     static constexpr int KC = D / 32, NO = D / 8, HV = D / 64, RH = R8 ? 2 : 4;
@@ -142,6 +144,100 @@ struct Pass {
             } else {
                 q[2 * c][0] = x.x; q[2 * c][1] = y.x; q[2 * c][2] = x.y; q[2 * c][3] = y.y;
                 q[2 * c + 1][0] = x.z; q[2 * c + 1][1] = y.z; q[2 * c + 1][2] = x.w; q[2 * c + 1][3] = y.w;
+            }
+        }
+    }
+    // a step's scores c (8 positions x 2, this lane's rows) into probabilities, the running maximum and sums with them
+    __device__ __forceinline__ void soft(float (&c)[2][4], uint32_t (&pa)[4]) {
+        float x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
+        x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 1));
+        x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 2));
+        const float n0 = fmaxf(m0, x0);
+        float n1 = -INFINITY;
+        if constexpr (!R8) {
+            float x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
+            x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 1));
+            x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 2));
+            n1 = fmaxf(m1, x1);
+        }
+        const float u0 = n0 == -INFINITY ? 0.0f : n0, u1 = n1 == -INFINITY ? 0.0f : n1;
+        if (__any_sync(~0u, n0 != m0 || (!R8 && n1 != m1))) {
+            const float f0 = ex2(m0 - u0), f1 = R8 ? 1.0f : ex2(m1 - u1);
+            l0 *= f0;
+            l1 *= f1;
+#pragma unroll
+            for (int j = 0; j < NO; j++) {
+                o[j][0] *= f0; o[j][1] *= f0;
+                if constexpr (!R8) { o[j][2] *= f1; o[j][3] *= f1; }
+            }
+            m0 = n0;
+            m1 = n1;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float e0 = ex2(c[i][0] - u0), e1 = ex2(c[i][1] - u0);
+            l0 += e0 + e1;
+            pa[2 * i] = Half2<T>::pack(e0, e1);
+            if constexpr (R8) pa[2 * i + 1] = 0;
+            else {
+                const float e2 = ex2(c[i][2] - u1), e3 = ex2(c[i][3] - u1);
+                l1 += e2 + e3;
+                pa[2 * i + 1] = Half2<T>::pack(e2, e3);
+            }
+        }
+    }
+    // scores in powers of two; positions outside [lo0 or lo1, hi) masked (`none`: all)
+    __device__ __forceinline__ void mask(float (&c)[2][4], float sl2, int base, int lo0, int lo1, int hi, bool none) {
+        const int t = threadIdx.x & 3;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < RH; e++) c[i][e] *= sl2;
+        if (base < lo0 || base < lo1 || base + PA_STEP > hi || none) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < RH; e++) {
+                    const int at = base + 8 * i + 2 * t + (e & 1);
+                    if (none || at >= hi || at < (e < 2 ? lo0 : lo1)) c[i][e] = -INFINITY;
+                }
+        }
+    }
+    // scores of 8 positions, whose K rows this lane holds in 16-byte pieces
+    __device__ __forceinline__ void score(float (&c)[4], const uint4 (&kr)[KC]) {
+        c[0] = c[1] = c[2] = c[3] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KC; j++) {
+            const uint4 k = kr[j];
+            uint32_t a0[4], a1[4];
+            if constexpr (R8) {
+                a0[0] = q[2 * j][0]; a0[1] = 0; a0[2] = q[2 * j][1]; a0[3] = 0;
+                a1[0] = q[2 * j + 1][0]; a1[1] = 0; a1[2] = q[2 * j + 1][1]; a1[3] = 0;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) { a0[e] = q[2 * j][e]; a1[e] = q[2 * j + 1][e]; }
+            }
+            Half2<T>::mma(c, a0, k.x, k.y);
+            Half2<T>::mma(c, a1, k.z, k.w);
+        }
+    }
+    // sums += P V for a 64-dimension part: vr are this lane's pieces of positions 2t, 2t + 1, 2t + 8, 2t + 9
+    __device__ __forceinline__ void add(int h, const uint32_t (&pa)[4], const uint4 (&vr)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t a = (&vr[0].x)[e], b = (&vr[1].x)[e], c = (&vr[2].x)[e], d = (&vr[3].x)[e];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint32_t sel = k ? 0x7632u : 0x5410u, b0 = __byte_perm(a, b, sel), b1 = __byte_perm(c, d, sel);
+                float (&x)[RH] = o[8 * h + 2 * e + k];
+                if constexpr (R8) {
+                    float y[4] = { x[0], x[1], 0.0f, 0.0f };
+                    Half2<T>::mma(y, pa, b0, b1);
+                    x[0] = y[0];
+                    x[1] = y[1];
+                } else {
+                    Half2<T>::mma(x, pa, b0, b1);
+                }
             }
         }
     }
@@ -181,43 +277,13 @@ struct Pass {
                     for (int h = 0; h < HV; h++) vr[i][h] = ldg16(r + ((i & 1) + 8 * (i >> 1)) * D + 64 * h);
             }
             float c[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.0f;
-#pragma unroll
-                for (int j = 0; j < KC; j++) {
-                    const uint4 k = kr[i][j];
-                    uint32_t a0[4], a1[4];
-                    if constexpr (R8) {
-                        a0[0] = q[2 * j][0]; a0[1] = 0; a0[2] = q[2 * j][1]; a0[3] = 0;
-                        a1[0] = q[2 * j + 1][0]; a1[1] = 0; a1[2] = q[2 * j + 1][1]; a1[3] = 0;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) { a0[e] = q[2 * j][e]; a1[e] = q[2 * j + 1][e]; }
-                    }
-                    Half2<T>::mma(c[i], a0, k.x, k.y);
-                    Half2<T>::mma(c[i], a1, k.z, k.w);
-                }
-            }
+            score(c[0], kr[0]);
+            score(c[1], kr[1]);
             const int base = s * PA_STEP, id_now = id;
             id = id1;
             if (s + stride < end) load_k(s + stride, id);
             id1 = page_at(s + 2 * stride);
-            // the scores in powers of two; positions outside [lo.., hi) masked
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int e = 0; e < RH; e++) c[i][e] *= p.sl2;
-            if (base < lo0 || base < lo1 || base + PA_STEP > hi || id_now < 0) {
-                const int from = id_now < 0 ? hi : 0;
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int e = 0; e < RH; e++) {
-                        const int at = base + 8 * i + 2 * t + (e & 1);
-                        if (at >= hi || at < max(from, e < 2 ? lo0 : lo1)) c[i][e] = -INFINITY;
-                    }
-            }
+            mask(c, p.sl2, base, lo0, lo1, hi, id_now < 0);
             if (base < lo || base + PA_STEP > hi || id_now < 0)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {   // what no row sees may be anything: 0 x NaN must not reach the sums
@@ -226,62 +292,83 @@ struct Pass {
 #pragma unroll
                         for (int h = 0; h < HV; h++) vr[i][h] = make_uint4(0, 0, 0, 0);
                 }
-            float x0 = fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1]));
-            x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 1));
-            x0 = fmaxf(x0, __shfl_xor_sync(~0u, x0, 2));
-            const float n0 = fmaxf(m0, x0);
-            float n1 = -INFINITY;
-            if constexpr (!R8) {
-                float x1 = fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3]));
-                x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 1));
-                x1 = fmaxf(x1, __shfl_xor_sync(~0u, x1, 2));
-                n1 = fmaxf(m1, x1);
-            }
-            const float u0 = n0 == -INFINITY ? 0.0f : n0, u1 = n1 == -INFINITY ? 0.0f : n1;
-            if (__any_sync(~0u, n0 != m0 || (!R8 && n1 != m1))) {
-                const float f0 = ex2(m0 - u0), f1 = R8 ? 1.0f : ex2(m1 - u1);
-                l0 *= f0;
-                l1 *= f1;
-#pragma unroll
-                for (int j = 0; j < NO; j++) {
-                    o[j][0] *= f0; o[j][1] *= f0;
-                    if constexpr (!R8) { o[j][2] *= f1; o[j][3] *= f1; }
-                }
-                m0 = n0;
-                m1 = n1;
-            }
             uint32_t pa[4];
+            soft(c, pa);
+#pragma unroll
+            for (int h = 0; h < HV; h++) {
+                const uint4 v[4] = { vr[0][h], vr[1][h], vr[2][h], vr[3][h] };
+                add(h, pa, v);
+            }
+        }
+    }
+    // the same for a long list of one warp, K and V through a ring of PO_STAGES steps in the warp's shared memory, PO_STAGES - 1 of
+    // them on their way: more bytes in flight than registers hold. 16-byte pieces of a row lie at piece ^ x(row), so that neither
+    // the copies, nor the eight lanes that read K (two rows, four pieces) or V (four rows, two pieces) at once meet in a bank. Lane
+    // w takes V's piece w / 2 + 4 (w % 2): product j then holds dimension 8 t + 32 n + j (+ 64 h) at column 2t + n.
+    static constexpr int STAGE = 2 * PA_STEP * D * 2;
+    static __device__ __forceinline__ uint32_t place(int row, int piece) {
+        return row * (D * 2) + ((piece ^ ((row & 1) << 2 | (row >> 1 & 3))) << 4);
+    }
+    __device__ void run_ring(const PaArgs &p, uint8_t *ring, const int32_t *list, const T *kb, const T *vb, long long ps, int lo, int hi) {
+        const int lane = threadIdx.x & 31, w = lane >> 2, t = lane & 3, end = (hi + PA_STEP - 1) / PA_STEP, s0 = lo / PA_STEP;
+        if (lo >= hi) return;
+        auto page_at = [&](int step) {
+            const int id = step < end ? __ldg(list + (step * PA_STEP >> p.shift)) : 0;
+            if ((unsigned) id < (unsigned) p.a.n_pages) return id;
+            if (p.a.status) atomicMax(p.a.status, IMI_DEV_PAGE);
+            return -1;
+        };
+        constexpr int CH = D / 8, RP = 32 / CH;   // pieces of a row, rows that a warp copies at once
+        const int cr = lane / CH, cc = lane % CH;
+        const uint32_t at = smem_u32(ring);
+        auto copy = [&](int step, int id) {       // rows that nobody sees, and those of a page that does not exist, as zeros
+            if (step < end) {
+                const long long off = max(id, 0) * ps + (long long) (step * PA_STEP & (p.a.page - 1)) * D + 8 * cc;
+                const uint32_t dst = at + (step - s0) % PO_STAGES * STAGE;
+#pragma unroll
+                for (int i = 0; i < PA_STEP / RP; i++) {
+                    const int row = cr + i * RP, pos = step * PA_STEP + row, bytes = id >= 0 && pos >= lo && pos < hi ? 16 : 0;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + place(row, cc)), "l"(kb + off + row * D), "r"(bytes) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + STAGE / 2 + place(row, cc)), "l"(vb + off + row * D), "r"(bytes) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int ids[PO_STAGES];                       // of the steps whose copies come next
+#pragma unroll
+        for (int k = 0; k < PO_STAGES; k++) ids[k] = page_at(s0 + k);
+#pragma unroll
+        for (int k = 0; k < PO_STAGES - 1; k++) copy(s0 + k, ids[k]);
+        int next = ids[PO_STAGES - 1];
+        unsigned gone = 0;                        // pages that do not exist, per step, the one at hand in bit 0
+#pragma unroll
+        for (int k = 0; k < PO_STAGES; k++) gone |= (ids[k] < 0) << k;
+        for (int s = s0; s < end; s++) {
+            copy(s + PO_STAGES - 1, next);
+            next = page_at(s + PO_STAGES);
+            asm volatile("cp.async.wait_group %0;" ::"n"(PO_STAGES - 1) : "memory");
+            __syncwarp();
+            const uint8_t *k = ring + (s - s0) % PO_STAGES * STAGE, *v = k + STAGE / 2;
+            float c[2][4];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float e0 = ex2(c[i][0] - u0), e1 = ex2(c[i][1] - u0);
-                l0 += e0 + e1;
-                pa[2 * i] = Half2<T>::pack(e0, e1);
-                if constexpr (R8) pa[2 * i + 1] = 0;
-                else {
-                    const float e2 = ex2(c[i][2] - u1), e3 = ex2(c[i][3] - u1);
-                    l1 += e2 + e3;
-                    pa[2 * i + 1] = Half2<T>::pack(e2, e3);
-                }
+                uint4 kr[KC];
+#pragma unroll
+                for (int x = 0; x < KC; x++) kr[x] = *(const uint4 *) (k + place(8 * i + w, 4 * x + t));
+                score(c[i], kr);
             }
+            mask(c, p.sl2, s * PA_STEP, lo, lo, hi, gone & 1);
+            uint32_t pa[4];
+            soft(c, pa);
 #pragma unroll
-            for (int h = 0; h < HV; h++)
+            for (int h = 0; h < HV; h++) {
+                uint4 vr[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t a = (&vr[0][h].x)[e], b = (&vr[1][h].x)[e], c2 = (&vr[2][h].x)[e], d = (&vr[3][h].x)[e];
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const uint32_t sel = k ? 0x7632u : 0x5410u, b0 = __byte_perm(a, b, sel), b1 = __byte_perm(c2, d, sel);
-                        float (&x)[RH] = o[8 * h + 2 * e + k];
-                        if constexpr (R8) {
-                            float y[4] = { x[0], x[1], 0.0f, 0.0f };
-                            Half2<T>::mma(y, pa, b0, b1);
-                            x[0] = y[0];
-                            x[1] = y[1];
-                        } else {
-                            Half2<T>::mma(x, pa, b0, b1);
-                        }
-                    }
-                }
+                for (int i = 0; i < 4; i++) vr[i] = *(const uint4 *) (v + place(2 * t + (i & 1) + 8 * (i >> 1), 8 * h + (w >> 1) + 4 * (w & 1)));
+                add(h, pa, vr);
+            }
+            gone = gone >> 1 | (next < 0) << (PO_STAGES - 1);
+            __syncwarp();
         }
     }
     // the sums of the lanes that share a row
@@ -479,11 +566,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_pieces(const __grid_consta
 }
 
 // the conversations' own positions: a warp's item is a (piece, kv head), its 16-position steps one after the other. Bound by
-// HBM: every row of K and V is read once, 4 to 8 KB of them on their way per warp.
+// HBM: every row of K and V is read once.
 template <typename T, int D, bool R8>
 __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_own(const __grid_constant__ PaArgs p) {
-    extern __shared__ int off[];
+    extern __shared__ __align__(128) uint8_t shb[];
     __shared__ int tmp[32];
+    int *off = (int *) (shb + PA_WARPS * PO_STAGES * Pass<T, D, R8>::STAGE);
     const imi_cuda_prefix_attn_args &a = p.a;
     // behind a launch for the prompt: that launch has let these CTAs start when all of its own had done their wait, and shares
     // nothing with them; they wait for it at their end, so that k_join, which waits for them, has both
@@ -511,7 +599,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_own(const __grid_constant_
         const long long head = (long long) kvh * a.page * D;
         const Seen v = seen_of(p, row);
         const int s0 = v.olo / PA_STEP + piece * chunk, lo = max(v.olo, s0 * PA_STEP), hi = min(v.len, (s0 + chunk) * PA_STEP);
-        f.run(p, a.table + row * a.table_stride, (const T *) a.k_pages + head, (const T *) a.v_pages + head, ps, lo, hi, v.olo, v.olo, 0, 1);
+        f.run_ring(p, shb + warp * PO_STAGES * Pass<T, D, R8>::STAGE, a.table + row * a.table_stride, (const T *) a.k_pages + head,
+                   (const T *) a.v_pages + head, ps, lo, hi);
         f.finish();
         const long long slot0 = p.own_slot0 + (long long) k * a.n_head + kvh * p.g;
 #pragma unroll
@@ -521,10 +610,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_own(const __grid_constant_
 #pragma unroll
                 for (int h = 0; h < D / 64; h++)
 #pragma unroll
-                    for (int n = 0; n < 2; n++)   // column n of the products: dimensions 64 h + 8 (2t + n) + 0..7
+                    for (int n = 0; n < 2; n++)
 #pragma unroll
                         for (int j = 0; j < 8; j += 4)
-                            *(float4 *) (o + 64 * h + 16 * t + 8 * n + j) =
+                            *(float4 *) (o + 64 * h + 8 * t + 32 * n + j) =
                                 make_float4(f.o[8 * h + j][2 * x + n], f.o[8 * h + j + 1][2 * x + n], f.o[8 * h + j + 2][2 * x + n],
                                             f.o[8 * h + j + 3][2 * x + n]);
                 if (t == 0) p.pml[slot0 + r + 8 * x] = make_float2(x ? f.m1 : f.m0, x ? f.l1 : f.l0);
@@ -700,7 +789,7 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
     }
     if (r == cudaSuccess)
         // own CTAs do not fit an SM beside one of k_pa_mma's: where those are few, the others' SMs are enough
-        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(pl.mma && pl.grid <= 74 ? PO_CTAS(D) / 148 * (148 - pl.grid) : PO_CTAS(D)), PA_WARPS * 32, (size_t) (a.rows + 1) * 4, st, args);
+        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(pl.mma && pl.grid <= 74 ? PO_CTAS(D) / 148 * (148 - pl.grid) : PO_CTAS(D)), PA_WARPS * 32, (size_t) PA_WARPS * PO_STAGES * Pass<T, D, R8>::STAGE + (a.rows + 1) * 4, st, args);
     if (r == cudaSuccess) {
         // warps per (row, head): one up to 16 pieces of the prompt; more while the SMs hold them (148 x 64 warps)
         int ways = 1;
@@ -722,8 +811,9 @@ cudaError_t raise_pa(int device) {
     return lim.raise(device,
                      { (const void *) k_pa_direct<T, 64, true>, (const void *) k_pa_direct<T, 64, false>,
                        (const void *) k_pa_direct<T, 128, true>, (const void *) k_pa_direct<T, 128, false>,
-                       (const void *) k_pa_pieces<T, 64>, (const void *) k_pa_pieces<T, 128> },
-                     96 * 1024) == cudaSuccess
+                       (const void *) k_pa_pieces<T, 64>, (const void *) k_pa_pieces<T, 128>, (const void *) k_pa_own<T, 64, true>,
+                       (const void *) k_pa_own<T, 64, false>, (const void *) k_pa_own<T, 128, true>, (const void *) k_pa_own<T, 128, false> },
+                     112 * 1024 + PA_ROWS * 4) == cudaSuccess
                ? lim2.raise(device, { (const void *) k_pa_mma<T, 64>, (const void *) k_pa_mma<T, 128> }, (int) std::max(PmSmem<64>::TOTAL, PmSmem<128>::TOTAL) + 1024)
                : cudaErrorUnknown;
 }
