@@ -42,9 +42,9 @@ struct PaArgs {
     int own_slot0;              // the first own slot
     int *off;                   // own pieces in front of each row [rows + 1]
     // the prompt on the 5th-generation tensor cores (k_pa_mma): units of PM_ROWS query rows of a kv head, `tiles` position
-    // tiles each, in one line cut every `per` tiles; pair: both streams of a CTA on one row tile
+    // tiles each, `span` apart in one line cut every `per` tiles; pair: both streams of a CTA on one row tile
     bool mma, pair;
-    int tiles, per, rtiles;
+    int tiles, span, per, rtiles;
 };
 
 template <typename T> struct Half2;
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, 
     if (live) {
         int np = p.pre_splits;   // the prompt's pieces of this row
         if (p.mma) {
-            const int u0 = (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.tiles;
+            const int u0 = (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.span;
             np = ((u0 + p.tiles - 1) / p.per - u0 / p.per + 1) * (p.pair ? 2 : 1);
         }
         const int n = np + o1 - o0;
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, 
 struct PaPlan {
     int splits, len;        // pieces of a query row over the prompt at most; positions of a piece (k_pa_pieces)
     bool mma, pair;
-    int tiles, per, rtiles, grid;
+    int tiles, span, per, rtiles, grid;
     size_t pre_slots, own_slots;
     size_t off_bytes, bytes;
 };
@@ -718,10 +718,15 @@ PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len
         p.pair = rows * g <= PM_M;
         p.rtiles = p.pair ? 1 : (rows * g + PM_ROWS - 1) / PM_ROWS;
         p.tiles = (prefix_len + PM_N - 1) / PM_N;
-        const long long total = (long long) p.rtiles * n_head_kv * p.tiles;
-        p.per = (int) std::max<long long>(PM_MIN_TILES, std::min<long long>(PM_MAX_TILES, (total + 147) / 148));
-        p.grid = (int) ((total + p.per - 1) / p.per);
-        p.splits = ((p.tiles + p.per - 1) / p.per + 1) * (p.pair ? 2 : 1);
+        // 148 CTAs: either a whole number of pieces per unit, or the line cut evenly, whose CTAs may have to begin a unit anew
+        // (about PM_BEGIN tiles' time each)
+        const long long units = (long long) p.rtiles * n_head_kv, total = units * p.tiles;
+        const long long k = std::max(1ll, std::min<long long>(148 / units, p.tiles)), whole = (p.tiles + k - 1) / k, even = (total + 147) / 148;
+        const bool cut = (units * k + 147) / 148 * (whole + PM_BEGIN) > even + PM_BEGIN * (1 + (even + p.tiles - 1) / p.tiles);
+        p.per = (int) std::max<long long>(PM_MIN_TILES, std::min<long long>(PM_MAX_TILES, cut ? even : whole));
+        p.span = cut ? p.tiles : (p.tiles + p.per - 1) / p.per * p.per;
+        p.grid = (int) ((units * p.span + p.per - 1) / p.per);
+        p.splits = ((p.tiles + p.per - 1) / p.per + (cut ? 1 : 0)) * (p.pair ? 2 : 1);
     }
     const int steps = (prefix_len + PA_STEP - 1) / PA_STEP;
     if (!p.mma) p.splits = prefix_len ? std::max(1, std::min(PA_PRE_ITEMS / std::max(1, tiles * n_head_kv), steps / PA_MIN_STEPS)) : 0;
@@ -870,6 +875,7 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
     p.mma = pl.mma;
     p.pair = pl.pair;
     p.tiles = pl.tiles;
+    p.span = pl.span;
     p.per = pl.per;
     p.rtiles = pl.rtiles;
     p.off = (int *) a->work;

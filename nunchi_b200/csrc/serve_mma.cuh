@@ -22,6 +22,7 @@
 constexpr int PM_M = 128, PM_N = 128, PM_ROWS = 2 * PM_M;
 constexpr int PM_MIN_ROWS = 16;        // query rows of a kv head up to which k_pa_pieces takes the prompt
 constexpr int PM_MIN_TILES = 2;        // position tiles of a piece at least
+constexpr int PM_BEGIN = 3;            // what a unit's beginning and end take, in tiles
 constexpr int PM_MAX_TILES = 256;      // and at most (its page numbers are held in shared memory)
 constexpr int PM_THREADS = 12 * 32;
 constexpr int PM_REGS = 168, PM_REGS_FEW = 80, PM_REGS_MANY = 208;   // 4 x 80 + 8 x 208 <= 12 x 168
@@ -82,6 +83,13 @@ __device__ __forceinline__ void pm_ld32(uint32_t t, float (&v)[32]) {
           "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
           "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
         : "r"(t));
+}
+__device__ __forceinline__ void pm_ld16(uint32_t t, float (&v)[16]) {
+    uint32_t *u = (uint32_t *) v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+                   "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+                 : "r"(t));
 }
 __device__ __forceinline__ void pm_st32(uint32_t t, const float (&v)[32]) {
     const uint32_t *u = (const uint32_t *) v;
@@ -171,7 +179,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     const int qrows = a.rows * p.g;
     const float sl2 = fabsf(p.sl2);                            // a negative scale turns q around
     const bool turn = p.sl2 < 0.0f;
-    const int line = p.rtiles * a.n_head_kv * p.tiles, end = min(line, ((int) blockIdx.x + 1) * p.per);
+    const int line = p.rtiles * a.n_head_kv * p.span, end = min(line, ((int) blockIdx.x + 1) * p.per);
     int at = (int) blockIdx.x * p.per;
     struct Unit {
         int kvh, row0, piece, page0, t0, t1, n0, n1;           // position tiles [t0, t1), of them the streams'
@@ -181,11 +189,11 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     int fr = -1, lo = 0;                                       // softmax: the thread's row, and what it sees from
     auto next = [&](Unit &w) -> bool {
         if (__syncthreads_or(at >= end || *(volatile int *) &stop)) return false;
-        const int unit = at / p.tiles;
-        w.piece = (int) blockIdx.x - unit * p.tiles / p.per;
-        w.t0 = at - unit * p.tiles;
+        const int unit = at / p.span;
+        w.piece = (int) blockIdx.x - unit * p.span / p.per;
+        w.t0 = at - unit * p.span;
         w.t1 = min(p.tiles, w.t0 + (end - at));
-        at += w.t1 - w.t0;
+        at += min(p.span - w.t0, end - at);
         w.kvh = unit / p.rtiles;
         w.row0 = (unit % p.rtiles) * (p.pair ? PM_M : PM_ROWS);
         w.page0 = (w.t0 * PM_N) >> p.shift;
@@ -422,7 +430,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                     if (raise) m = top;
                     if (j > 0) {
                         float o[32];
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D / 32; c++) {
                             pm_ld32(O + 32 * c, o);
                             pm_wait_ld();
@@ -467,33 +475,27 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
             }
             if (fr >= 0) p.pml[slot] = make_float2(m, l);
             // O by 16 dimensions through shared memory, so that four threads write a row's 64 bytes: a row per thread, every store
-            // would touch 32 lines (2.1 us of a piece against 0.5)
+            // would touch 32 lines (2.1 us of a piece against 0.5). Not unrolled: run once per piece, it waits for its instructions
             uint8_t *out = sm + L::OUT + (warp - 4) * 32 * PM_OROW;
+            const long long to_row = fr >= 0 ? slot * D : -1;
+            const bool real = n > 0 && ok;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+                float o[16];
+                pm_ld16(O + c, o);
+                pm_wait_ld();
+                __syncwarp();
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {
-                float o[32];
-                if (n > 0 && ok) {
-                    pm_ld32(O + 32 * c, o);
-                    pm_wait_ld();
-                } else {
+                for (int e = 0; e < 16; e += 4)
+                    *(float4 *) (out + lane * PM_OROW + 4 * e) =
+                        real ? make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = 0.0f;
-                }
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        *(float4 *) (out + lane * PM_OROW + 16 * e) =
-                            make_float4(o[16 * h + 4 * e], o[16 * h + 4 * e + 1], o[16 * h + 4 * e + 2], o[16 * h + 4 * e + 3]);
-                    __syncwarp();
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int r = 8 * e + lane / 4;
-                        const long long s0 = __shfl_sync(~0u, fr >= 0 ? slot : -1ll, r);
-                        if (s0 >= 0)
-                            *(float4 *) (p.po + s0 * D + 32 * c + 16 * h + 4 * (lane % 4)) = *(const float4 *) (out + r * PM_OROW + 16 * (lane % 4));
-                    }
+                for (int e = 0; e < 4; e++) {
+                    const int r = 8 * e + lane / 4;
+                    const long long at_row = __shfl_sync(~0u, to_row, r);
+                    if (at_row >= 0)
+                        *(float4 *) (p.po + at_row + c + 4 * (lane % 4)) = *(const float4 *) (out + r * PM_OROW + 16 * (lane % 4));
                 }
             }
             pm_fence_before();
