@@ -91,6 +91,30 @@ imi_cuda_status imi_cuda_step_batch(imi_cuda_state *s, const int32_t *tokens, co
  * Logits of the last step stay readable. */
 imi_cuda_status imi_cuda_greedy(imi_cuda_state *const *s, int n, const int32_t *tokens, int steps, int32_t *ids);
 
+/* Sampling from conversations' latest word scores (imi picks greedily only): the words imi_cuda_sample (below) names for the
+ * uniform numbers u[n], with per-conversation settings (arrays of n, host; NULL: temperature 1, the filters off). ids,
+ * logprob and kept (each may be NULL) receive them. A word becomes its conversation's last pick: what imi_cuda_get_argmax
+ * returns as id, and what a later imi_cuda_greedy or imi_cuda_sampled without tokens reads first. */
+imi_cuda_status imi_cuda_sample_states(imi_cuda_state *const *s, int n, const float *u, const float *temperature,
+                                       const int32_t *top_k, const float *top_p, const float *min_p, int32_t *ids, float *logprob,
+                                       int32_t *kept);
+
+/* imi_cuda_greedy with sampling: `steps` positions for each of n conversations, each step's input being the word sampled
+ * after the step before (the first: tokens[i], or the conversation's last pick when tokens is NULL). u[steps][n] (host): the
+ * uniform number of each word; settings as above, the same for all steps. ids[steps][n] and logprob[steps][n] may be NULL.
+ * Temperature 0 gives what imi_cuda_greedy gives. The words stay on the device from step to step. */
+imi_cuda_status imi_cuda_sampled(imi_cuda_state *const *s, int n, const int32_t *tokens, int steps, const float *u,
+                                 const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                                 int32_t *ids, float *logprob);
+
+/* A conversation's cached keys and values of one attention layer (0..n_attn-1), on the device: IMI_F16, position p of kv
+ * head h at k + p * position_stride + h * head_stride (elements; v alike), positions 0..pos-1. Keys are normed and rotated
+ * as the engine's attention reads them. For imi_cuda_page_write: a prompt the engine has read, into pages. The pointers
+ * stay the conversation's; its steps write further positions on the engine's stream (imi_cuda_stream), so a reader on
+ * another stream waits for that. */
+imi_cuda_status imi_cuda_state_kv(const imi_cuda_state *s, int layer, const void **k, const void **v, int64_t *position_stride,
+                                  int64_t *head_stride);
+
 /* Checkpoint / resume of one conversation (the content of imi_seoul_state, seoul.h:21-26) as a host byte image:
  *   int32 magic 0x53494d49 ("IMIS"), version 1, pos, n_attn, n_ctx, kv_dim, n_conv, d_conv, n_embd, n_vocab, next_pick;
  *   K cache [n_attn][pos][kv_dim] fp16, V cache likewise (positions 0..pos-1 only);

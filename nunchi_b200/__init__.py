@@ -82,6 +82,9 @@ def lib():
         L.imi_cuda_q4_matmul.argtypes = [C.c_int, _vp, C.c_int, C.c_int, _vp, _fp, _fp, C.c_int, _fp]
         L.imi_cuda_bench_matvec.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_float),
                                             C.POINTER(C.c_size_t)]
+        L.imi_cuda_sample_states.argtypes = [_vp, C.c_int, _fp, _fp, _ip, _fp, _fp, _ip, _fp, _ip]
+        L.imi_cuda_sampled.argtypes = [_vp, C.c_int, _ip, C.c_int, _fp, _fp, _ip, _fp, _fp, _ip, _fp]
+        L.imi_cuda_state_kv.argtypes = [_vp, C.c_int, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]
         for f in ("page_map", "page_write", "prefix_attn", "sample"):
             getattr(L, "imi_cuda_" + f).argtypes = [C.c_int, C.c_char_p, _vp]
         L.imi_cuda_prefix_attn_work.argtypes = [C.c_int] * 7
@@ -173,6 +176,14 @@ def trace_step(state: "State", token: int, want_logits: bool = True, max_launche
     return out[: n.value], kinds[: n.value], grids[: n.value]
 
 
+class _DeviceView:
+    """fp16 values of a conversation's device memory, for anything that reads __cuda_array_interface__."""
+
+    def __init__(self, owner, ptr, shape, strides):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": "<f2", "data": (ptr, False), "strides": strides, "version": 3}
+
+
 class State:
     """One conversation on the device (imi_seoul_state, seoul.h:21-26)."""
 
@@ -253,6 +264,14 @@ class State:
         hid = take(E, np.float32, (E,))
         return {"pos": pos, "k": k, "v": v, "conv": conv, "hidden": hid, "next_pick": int(h[10])}
 
+    def kv(self, layer: int):
+        """The cached keys and values of one attention layer, on the device, as two views [pos][n_head_kv][head_dim] of the
+        conversation's own memory (imi_cuda_state_kv): torch.as_tensor(view, device="cuda") shares it."""
+        k, v, ps, hs = _vp(), _vp(), C.c_int64(), C.c_int64()
+        _check(lib().imi_cuda_state_kv(self.h, layer, C.byref(k), C.byref(v), C.byref(ps), C.byref(hs)))
+        e = self.engine
+        return tuple(_DeviceView(self, p.value, (self.pos, e.n_head_kv, e.head_dim), (2 * ps.value, 2 * hs.value, 2)) for p in (k, v))
+
     def argmax(self):
         i, v = C.c_int32(), C.c_float()
         _check(lib().imi_cuda_get_argmax(self.h, C.byref(i), C.byref(v)))
@@ -286,6 +305,36 @@ def greedy(states, steps: int, tokens=None) -> np.ndarray:
     ids = np.zeros((steps, n), np.int32)
     _check(lib().imi_cuda_greedy(_handles(states), n, _ptr(t), steps, _ptr(ids)))
     return ids
+
+
+def _per(x, n, dtype):
+    """A setting of n conversations: None, one value for all, or n of them."""
+    return None if x is None else np.ascontiguousarray(np.broadcast_to(np.asarray(x, dtype), (n,)))
+
+
+def sample_states(states, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """A word per conversation sampled from its latest word scores by the uniform numbers u[n] (imi_cuda_sample_states);
+    settings one value or n of them. Returns (ids, logprobs, kept counts); the words become the last picks."""
+    n = len(states)
+    u = np.ascontiguousarray(np.broadcast_to(np.asarray(u, np.float32), (n,)))
+    a = [_per(x, n, t) for x, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+    ids, lp, kept = np.zeros(n, np.int32), np.zeros(n, np.float32), np.zeros(n, np.int32)
+    _check(lib().imi_cuda_sample_states(_handles(states), n, _ptr(u), *map(_ptr, a), _ptr(ids), _ptr(lp), _ptr(kept)))
+    return ids, lp, kept
+
+
+def sampled(states, steps: int, u, tokens=None, temperature=None, top_k=None, top_p=None, min_p=None):
+    """`steps` sampled positions per conversation on the device (imi_cuda_sampled) by the uniform numbers u[steps][n];
+    returns (ids[steps][n], logprobs[steps][n])."""
+    n = len(states)
+    u = np.ascontiguousarray(u, dtype=np.float32)
+    if u.shape != (steps, n):
+        raise ImiError(1, f"u: {steps} x {n} uniform numbers are wanted")
+    t = None if tokens is None else np.ascontiguousarray(np.broadcast_to(np.asarray(tokens, np.int32), (n,)))
+    a = [_per(x, n, d) for x, d in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+    ids, lp = np.zeros((steps, n), np.int32), np.zeros((steps, n), np.float32)
+    _check(lib().imi_cuda_sampled(_handles(states), n, _ptr(t), steps, _ptr(u), *map(_ptr, a), _ptr(ids), _ptr(lp)))
+    return ids, lp
 
 
 def q8_cut(x, device: int = 0):

@@ -125,6 +125,8 @@ struct imi_cuda_engine {
     cudaEvent_t t0 = nullptr, t1 = nullptr;   // around the last step's graph (imi_cuda_last_step_ms)
     bool timed = false;
     std::map<int, cudaGraphExec_t> graphs;
+    // sampling (allocated by the first call): pinned and device copies of a call's block, SampleBlock
+    uint8_t *smp_d = nullptr, *smp_h = nullptr;
     size_t state_bytes = 0;
     size_t dev_budget = SIZE_MAX, dev_used = 0;   // IMI_CUDA_MAX_DEVICE_BYTES and what the engine + states hold
     uint8_t *qbuf = nullptr;
@@ -165,6 +167,8 @@ imi_cuda_engine::~imi_cuda_engine() {
     cudaFree(cols_d);
     cudaFree(tc_w);
     cudaFree(tc_xb);
+    cudaFree(smp_d);
+    cudaFreeHost(smp_h);
     cudaFreeHost(cols_h);
     cudaFreeHost(embd_h);
     cudaFreeHost(reply_h);
@@ -1963,6 +1967,168 @@ size_t image_bytes(const imi_cuda_engine *e, int pos) {
            (size_t) e->n_embd * 4 + (size_t) e->n_vocab * 4;
 }
 }  // namespace
+
+namespace {
+// one call's sampling data for up to ncmax conversations and SMP_STEPS steps, as it lies in host and device memory: scores'
+// addresses, picks' addresses, settings, then u[step][conversation], ids, logprobs, kept counts
+constexpr int SMP_STEPS = 64;
+struct SampleBlock {
+    size_t rows, picks, temperature, top_k, top_p, min_p, u, ids, logprob, kept, in_bytes, bytes;
+    explicit SampleBlock(int nc) {
+        size_t o = 0;
+        auto take = [&](size_t n) { const size_t r = o; o = (o + n + 15) / 16 * 16; return r; };
+        rows = take((size_t) nc * 8);
+        picks = take((size_t) nc * 8);
+        temperature = take((size_t) nc * 4);
+        top_k = take((size_t) nc * 4);
+        top_p = take((size_t) nc * 4);
+        min_p = take((size_t) nc * 4);
+        u = take((size_t) SMP_STEPS * nc * 4);
+        in_bytes = o;
+        ids = take((size_t) SMP_STEPS * nc * 4);
+        logprob = take((size_t) SMP_STEPS * nc * 4);
+        kept = take((size_t) SMP_STEPS * nc * 4);
+        bytes = o;
+    }
+};
+
+// the settings of n conversations and `steps` rows of u on their way to the device (nothing of an earlier call may be pending)
+imi_cuda_status sample_begin(imi_cuda_state *const *s, int n, int steps, const float *u, int u_stride, const float *temperature,
+                             const int32_t *top_k, const float *top_p, const float *min_p) {
+    imi_cuda_engine *e = s[0]->e;
+    const SampleBlock b(e->ncmax);
+    if (!e->smp_d) {
+        if (!e->smp_h) CK(cudaMallocHost(&e->smp_h, b.bytes));
+        DALLOC(e, e->smp_d, b.bytes);
+    }
+    uint8_t *h = e->smp_h;
+    for (int c = 0; c < n; c++) {
+        ((const void **) (h + b.rows))[c] = s[c]->logits;
+        ((int32_t **) (h + b.picks))[c] = &s[c]->s->next_token;
+        ((float *) (h + b.temperature))[c] = temperature ? temperature[c] : 1.0f;
+        ((int32_t *) (h + b.top_k))[c] = top_k ? top_k[c] : 0;
+        ((float *) (h + b.top_p))[c] = top_p ? top_p[c] : 1.0f;
+        ((float *) (h + b.min_p))[c] = min_p ? min_p[c] : 0.0f;
+        for (int k = 0; k < steps; k++) ((float *) (h + b.u))[(size_t) k * n + c] = u[(size_t) k * u_stride + c];
+    }
+    CK(cudaMemcpyAsync(e->smp_d, h, b.in_bytes, cudaMemcpyHostToDevice, e->stream));
+    return IMI_OK;
+}
+// step k's words of the n conversations from their latest scores, each also the conversation's last pick
+imi_cuda_status sample_step(imi_cuda_engine *e, int n, int k) {
+    const SampleBlock b(e->ncmax);
+    uint8_t *d = e->smp_d;
+    imi_cuda_sample_args a = {};
+    a.type = IMI_F32;
+    a.n = n;
+    a.vocab = e->n_vocab;
+    a.u = (const float *) (d + b.u) + (size_t) k * n;
+    a.temperature = (const float *) (d + b.temperature);
+    a.top_k = (const int32_t *) (d + b.top_k);
+    a.top_p = (const float *) (d + b.top_p);
+    a.min_p = (const float *) (d + b.min_p);
+    a.ids = (int32_t *) (d + b.ids) + (size_t) k * n;
+    a.logprob = (float *) (d + b.logprob) + (size_t) k * n;
+    a.kept = (int32_t *) (d + b.kept) + (size_t) k * n;
+    CK(launch_sample(e->device, a, (const void *const *) (d + b.rows), (int32_t *const *) (d + b.picks), e->stream));
+    e->gen++;   // the conversations' records have changed
+    return IMI_OK;
+}
+// the words (and logprobs, kept counts) of `steps` steps read back into rows `out_stride` apart
+imi_cuda_status sample_end(imi_cuda_engine *e, int n, int steps, int out_stride, int32_t *ids, float *logprob, int32_t *kept) {
+    const SampleBlock b(e->ncmax);
+    CK(cudaMemcpyAsync(e->smp_h + b.ids, e->smp_d + b.ids, b.bytes - b.ids, cudaMemcpyDeviceToHost, e->stream));
+    const imi_cuda_status st = check_err(e);   // waits for the stream
+    if (st != IMI_OK) return st;
+    for (int k = 0; k < steps; k++)
+        for (int c = 0; c < n; c++) {
+            const size_t from = (size_t) k * n + c, to = (size_t) k * out_stride + c;
+            if (ids) ids[to] = ((const int32_t *) (e->smp_h + b.ids))[from];
+            if (logprob) logprob[to] = ((const float *) (e->smp_h + b.logprob))[from];
+            if (kept) kept[to] = ((const int32_t *) (e->smp_h + b.kept))[from];
+        }
+    return IMI_OK;
+}
+imi_cuda_status sample_states_ok(imi_cuda_state *const *s, int n, const float *u) {
+    if (!s || n <= 0 || !s[0] || !u) return fail(IMI_E_ARG, "bad sampling arguments");
+    imi_cuda_engine *e = s[0]->e;
+    for (int i = 0; i < n; i++) {
+        if (!s[i] || s[i]->e != e) return fail(IMI_E_ARG, "states of another engine");
+        for (int j = 0; j < i; j++) if (s[j] == s[i]) return fail(IMI_E_ARG, "a state appears twice");
+    }
+    if (e->n_vocab > IMI_CUDA_SAMPLE_VOCAB) return fail(IMI_E_ARG, "the word table is too large to sample from");
+    return IMI_OK;
+}
+}  // namespace
+
+imi_cuda_status imi_cuda_sample_states(imi_cuda_state *const *s, int n, const float *u, const float *temperature,
+                                       const int32_t *top_k, const float *top_p, const float *min_p, int32_t *ids, float *logprob,
+                                       int32_t *kept) {
+    imi_cuda_status st;
+    if ((st = sample_states_ok(s, n, u)) != IMI_OK) return st;
+    imi_cuda_engine *e = s[0]->e;
+    CK(cudaSetDevice(e->device));
+    for (int i = 0; i < n; i += e->ncmax) {
+        const int m = std::min(e->ncmax, n - i);
+        auto at = [&](auto *p) { return p ? p + i : p; };
+        if ((st = sample_begin(s + i, m, 1, u + i, n, at(temperature), at(top_k), at(top_p), at(min_p))) != IMI_OK) return st;
+        if ((st = sample_step(e, m, 0)) != IMI_OK) return st;
+        if ((st = sample_end(e, m, 1, n, at(ids), at(logprob), at(kept))) != IMI_OK) return st;
+    }
+    return IMI_OK;
+}
+
+imi_cuda_status imi_cuda_sampled(imi_cuda_state *const *s, int n, const int32_t *tokens, int steps, const float *u,
+                                 const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                                 int32_t *ids, float *logprob) {
+    imi_cuda_status st;
+    if (steps <= 0) return fail(IMI_E_ARG, "bad sampling arguments");
+    if ((st = sample_states_ok(s, n, u)) != IMI_OK) return st;
+    imi_cuda_engine *e = s[0]->e;
+    if (n > e->max_batch && n > STEP_COLS) return fail(IMI_E_ARG, "more conversations than max_batch");
+    for (int i = 0; i < n; i++) {
+        if (s[i]->pos + steps > e->n_ctx) return fail(IMI_E_CTX_FULL, "context full (" + std::to_string(e->n_ctx) + ")");
+        if (tokens && (tokens[i] < 0 || tokens[i] >= e->n_vocab)) return fail(IMI_E_ARG, "token out of range");
+    }
+    CK(cudaSetDevice(e->device));
+    for (int i = 0; i < n; i += e->ncmax) {   // groups of ncmax conversations, each group all its steps
+        const int m = std::min(e->ncmax, n - i);
+        auto at = [&](auto *p) { return p ? p + i : p; };
+        for (int k0 = 0; k0 < steps; k0 += SMP_STEPS) {
+            const int ks = std::min(SMP_STEPS, steps - k0);
+            if ((st = sample_begin(s + i, m, ks, u + (size_t) k0 * n + i, n, at(temperature), at(top_k), at(top_p), at(min_p))) != IMI_OK)
+                return st;
+            for (int k = 0; k < ks; k++) {
+                // the columns are uploaded for the first two steps (a given word, then the last pick) and stay for the rest
+                const bool first = k0 + k == 0, fresh = k < 2;
+                if (fresh) {
+                    if ((st = staging_wait(e)) != IMI_OK) return st;
+                    for (int c = 0; c < m; c++) e->cols_h[c] = decode_col(s[i + c], first && tokens ? tokens[i + c] : -2, false, c, true);
+                }
+                if ((st = run_step(e, m, true, K_DECODE, fresh)) != IMI_OK) return st;
+                for (int c = 0; c < m; c++) s[i + c]->pos++;
+                if ((st = sample_step(e, m, k)) != IMI_OK) return st;
+            }
+            if ((st = sample_end(e, m, ks, n, ids ? ids + (size_t) k0 * n + i : nullptr, logprob ? logprob + (size_t) k0 * n + i : nullptr,
+                                 nullptr)) != IMI_OK)
+                return st;
+        }
+    }
+    return IMI_OK;
+}
+
+imi_cuda_status imi_cuda_state_kv(const imi_cuda_state *s, int layer, const void **k, const void **v, int64_t *position_stride,
+                                  int64_t *head_stride) {
+    if (!s || !k || !v || !position_stride || !head_stride) return fail(IMI_E_ARG, "null argument");
+    const imi_cuda_engine *e = s->e;
+    if (layer < 0 || layer >= e->n_attn) return fail(IMI_E_ARG, "no such attention layer");
+    const size_t off = (size_t) layer * e->n_head_kv * e->n_ctx * e->head_dim;
+    *k = s->kc + off;
+    *v = s->vc + off;
+    *position_stride = e->head_dim;
+    *head_stride = (int64_t) e->n_ctx * e->head_dim;
+    return IMI_OK;
+}
 
 imi_cuda_status imi_cuda_state_save(const imi_cuda_state *s, void *buf, size_t cap, size_t *size) {
     if (!s || !size) return fail(IMI_E_ARG, "null argument");

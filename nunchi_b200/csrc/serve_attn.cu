@@ -734,7 +734,13 @@ PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len
         p.len = (steps + p.splits - 1) / p.splits * PA_STEP;
         p.splits = (prefix_len + p.len - 1) / p.len;
     }
-    p.pre_slots = (size_t) rows * n_head * p.splits;
+    // slots for the prompt's pieces: at most this many for any call of no more rows and positions, so that its workspace serves
+    // them. k_pa_mma: 148 CTAs' pieces of PM_ROWS rows, and up to 3 more pieces (those that PM_MAX_TILES ends besides) of every
+    // unit; k_pa_pieces: its items' rows, and one piece of every row
+    const size_t units = (size_t) ((rows * g + PM_ROWS - 1) / PM_ROWS) * n_head_kv, most_tiles = ((size_t) prefix_len + PM_N - 1) / PM_N;
+    p.pre_slots = prefix_len ? std::max((size_t) PM_ROWS * (148 + units * (3 + most_tiles / PM_MAX_TILES)),
+                                        (size_t) R * PA_PRE_ITEMS + (size_t) tiles * R * n_head_kv)
+                             : 0;
     p.own_slots = ((size_t) rows + (PO_ROUNDS * PO_CTAS(head_dim) * PA_WARPS + n_head_kv - 1) / n_head_kv) * n_head;
     p.off_bytes = ((size_t) (rows + 1) * 4 + 255) / 256 * 256;
     const size_t slots = p.pre_slots + p.own_slots;

@@ -52,6 +52,8 @@ typedef unsigned long long u64;
 struct SampleArgs {
     imi_cuda_sample_args a;
     int seg, slice;   // words per warp (a multiple of SM_TILE) and per CTA (SM_NW * seg)
+    const void *const *rows;   // the rows' scores where they do not lie `stride` apart (the engine's conversations)
+    int32_t *const *picks;     // and where each row's word goes besides ids (not if there is none)
 };
 
 // scores as unsigned keys in the same order; NaN is -infinity, whose key no kept word has; the zeros are one
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     const double m = fmin((double) min_p, 1.0), pd = (double) top_p;
 
     // the row as keys; the largest
-    const S *x = (const S *) a.scores + row * a.stride;
+    const S *x = p.rows ? (const S *) p.rows[row] : (const S *) a.scores + row * a.stride;
     const bool vec = ((uintptr_t) (x + base) & (4 * sizeof(S) - 1)) == 0;
     uint32_t mx = 0;
     uint32_t *mine = keys + warp * p.seg + 4 * lane;        // the words of a lane, tile by tile
@@ -366,6 +368,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     uint32_t floor = max(__reduce_min_sync(~0u, lane < C ? s.all_floor[lane] : ~0u), KEY_NONE + 1);
     auto emit = [&](int id, float lp, int kept) {
         a.ids[row] = id;
+        if (p.picks && id >= 0) *p.picks[row] = id;
         if (a.logprob) a.logprob[row] = lp;
         if (a.kept) a.kept[row] = kept;
     };
@@ -988,6 +991,25 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
 size_t sample_smem(int slice) { return (sizeof(SampleShared) + 15) / 16 * 16 + (size_t) slice * 4; }
 
 }  // namespace
+
+// the launch of checked arguments (the engine's sampling calls it too)
+cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void *const *rows, int32_t *const *picks, cudaStream_t st) {
+    const void *fn = a.type == IMI_F32   ? (const void *) k_sample<float>
+                     : a.type == IMI_F16 ? (const void *) k_sample<__half>
+                                          : (const void *) k_sample<__nv_bfloat16>;
+    static SmemLimit lim;
+    cudaError_t r = lim.raise(device, { (const void *) k_sample<float>, (const void *) k_sample<__half>, (const void *) k_sample<__nv_bfloat16> },
+                              (int) sample_smem(SM_SLICE));
+    // CTAs per row: as many as hold the row, more while the rows leave SMs idle and a CTA keeps a tile per warp
+    int C = 1;
+    while (C < SM_MAX_CLUSTER && ((a.vocab + C - 1) / C > SM_SLICE || (a.n * C < 148 && a.vocab > C * SM_NW * SM_TILE))) C *= 2;
+    SampleArgs p = { a, 0, 0, rows, picks };
+    p.seg = ((a.vocab + C * SM_NW - 1) / (C * SM_NW) + SM_TILE - 1) / SM_TILE * SM_TILE;
+    p.slice = p.seg * SM_NW;
+    void *args[] = { &p };
+    if (r == cudaSuccess) r = launch_pdl(fn, dim3(a.n * C), SM_NT, sample_smem(p.slice), st, args, C);
+    return r;
+}
 }  // namespace imi
 
 using namespace imi;
@@ -1008,20 +1030,7 @@ extern "C" imi_cuda_status imi_cuda_sample(int device, const imi_cuda_sample_arg
     if (!on.ok()) return set_error(IMI_E_NODEV, "no CUDA device " + std::to_string(device));
     if (!all_on_device({ a->scores, a->u, a->temperature, a->top_k, a->top_p, a->min_p, a->ids, a->logprob, a->kept }, device))
         return set_error(IMI_E_ARG, "sample: every buffer must be device memory of device " + std::to_string(device));
-    const void *fn = a->type == IMI_F32   ? (const void *) k_sample<float>
-                     : a->type == IMI_F16 ? (const void *) k_sample<__half>
-                                          : (const void *) k_sample<__nv_bfloat16>;
-    static SmemLimit lim;
-    cudaError_t r = lim.raise(device, { (const void *) k_sample<float>, (const void *) k_sample<__half>, (const void *) k_sample<__nv_bfloat16> },
-                              (int) sample_smem(SM_SLICE));
-    // CTAs per row: as many as hold the row, more while the rows leave SMs idle and a CTA keeps a tile per warp
-    int C = 1;
-    while (C < SM_MAX_CLUSTER && ((a->vocab + C - 1) / C > SM_SLICE || (a->n * C < 148 && a->vocab > C * SM_NW * SM_TILE))) C *= 2;
-    SampleArgs p = { *a, 0, 0 };
-    p.seg = ((a->vocab + C * SM_NW - 1) / (C * SM_NW) + SM_TILE - 1) / SM_TILE * SM_TILE;
-    p.slice = p.seg * SM_NW;
-    void *args[] = { &p };
-    if (r == cudaSuccess) r = launch_pdl(fn, dim3(a->n * C), SM_NT, sample_smem(p.slice), (cudaStream_t) stream, args, C);
+    const cudaError_t r = launch_sample(device, *a, nullptr, nullptr, (cudaStream_t) stream);
     if (r != cudaSuccess) return set_error(IMI_E_CUDA, std::string("sample: ") + cudaGetErrorString(r));
     return IMI_OK;
 }

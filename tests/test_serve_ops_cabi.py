@@ -67,6 +67,9 @@ def test_prefix_attn_work():
     for prefix in (0, 1, 100, 5000, 100000):
         sizes = [w(r, 32, 8, 64, prefix, 20, 64) for r in range(0, 300)]
         assert all(x <= sizes[-1] for x in sizes)
+    for rows in (1, 4, 5, 33, 300):
+        sizes = [w(rows, 32, 8, 64, p, 20, 64) for p in range(0, 200000, 997)]
+        assert sizes == sorted(sizes)
 
 
 @pytest.mark.parametrize("bad", [
