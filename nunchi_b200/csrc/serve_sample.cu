@@ -85,11 +85,12 @@ struct SampleShared {
     };
     unsigned wc[SM_NW];               // scans over the CTA
     u64 wm[SM_NW];
+    double2 near[SM_NW];
     // what the cluster reads of this CTA
     unsigned mx, mn, lmin, nvalid, floor, idmin, n_list, n_all, at_lead, part_kept, lo, hi;
     // of every CTA of the cluster, written here by it: read after a barrier, and never by two exchanges in a row
     unsigned all_mx[SM_MAX_CLUSTER], all_floor[SM_MAX_CLUSTER], all_n[SM_MAX_CLUSTER], all_cnt[SM_MAX_CLUSTER], all_kept[SM_MAX_CLUSTER];
-    double all_near[SM_MAX_CLUSTER];
+    double all_near[SM_MAX_CLUSTER], all_listed[SM_MAX_CLUSTER];
     u64 all_mass[SM_MAX_CLUSTER], all_sum[SM_MAX_CLUSTER];
     u64 mass_above;
     int bin;                          // found in a scan: the crossing bin, and what lies above it
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             floor = max(key_of((float) (lo - 1e-6 * (fabs(lo) + fabs((double) xmax) + (double) temp))), KEY_NONE + 1);
         }
         const float c2 = (float) weigh.c;
-        float near = 0.0f;
+        float near = 0.0f, listed = 0.0f;   // the words' mass, and the listed words'
         for (int o = 0; o < p.seg; o += SM_TILE) {
             const uint4 q = *(const uint4 *) (mine + o);
             if (max(max(q.x, q.y), max(q.z, q.w)) >= floor)
@@ -552,27 +553,43 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"(y));
                 }
                 near = __fadd_rn(near, __fadd_rn(__fadd_rn(e[0], e[1]), __fadd_rn(e[2], e[3])));
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if ((&q.x)[i] >= floor) listed = __fadd_rn(listed, e[i]);
             }
         }
-        double near_sum = (double) near;
         if (by_p) {
+            double t = (double) near, l = (double) listed;
 #pragma unroll
-            for (int d = 16; d; d >>= 1) near_sum += __shfl_xor_sync(~0u, near_sum, d);
-            if (lane == 0) s.wm[warp] = (u64) __double_as_longlong(near_sum);
-        }
-        __syncthreads();
-        if (by_p && warp == 0) {
-            double t = lane < SM_NW ? __longlong_as_double((long long) s.wm[lane]) : 0.0;
+            for (int d = 16; d; d >>= 1) {
+                t += __shfl_xor_sync(~0u, t, d);
+                l += __shfl_xor_sync(~0u, l, d);
+            }
+            if (lane == 0) s.near[warp] = make_double2(t, l);
+            __syncthreads();
+            if (warp == 0) {
+                double2 v = lane < SM_NW ? s.near[lane] : make_double2(0.0, 0.0);
 #pragma unroll
-            for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(~0u, t, d);
-            if (lane < C) cl.map_shared_rank(&s, lane)->all_near[rank] = t;   // to every CTA
+                for (int d = 16; d; d >>= 1) {
+                    v.x += __shfl_xor_sync(~0u, v.x, d);
+                    v.y += __shfl_xor_sync(~0u, v.y, d);
+                }
+                if (lane < C) {   // to every CTA
+                    SampleShared &o = *cl.map_shared_rank(&s, lane);
+                    o.all_near[rank] = v.x;
+                    o.all_listed[rank] = v.y;
+                }
+            }
         }
         push_list();
         cl.sync();
         const double nearW = by_p ? sum8(lane < C ? s.all_near[lane] : 0.0) * SM_ONE : 0.0;
+        const double listedW = by_p ? sum8(lane < C ? s.all_listed[lane] : 0.0) * SM_ONE : 0.0;
         const int n = list_length();
+        // certain already to go on below the list
+        const bool below = by_p && listedW * (1.0 + SM_MASS_ERR) < pd * nearW * (1.0 - SM_MASS_ERR);
         if (!by_p && rank != 0 && n <= SM_LIST) return;   // nobody reads this CTA's shared memory any more
-        if (n <= SM_LIST) {
+        if (n <= SM_LIST && !below) {
             if (!by_p) {
                 weigh_list(n);
                 if (n <= SM_SHORT) {
@@ -737,12 +754,25 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 if (by_mass)
 #pragma unroll
                     for (int e = 0; e < 4; e++) wv[e] = weigh((&q.x)[e]);
+                if (by_mass) {   // add64 for four words, the low halves' additions on their way together
+                    int b[4];
+                    unsigned old[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int b = bin_of((&q.x)[e]);
-                    if (b < 0) continue;
-                    if (by_mass) add64(s.mass[b], wv[e]);
-                    else atomicAdd(&s.cnt[b], 1u);
+                    for (int e = 0; e < 4; e++) {
+                        b[e] = bin_of((&q.x)[e]);
+                        if (b[e] >= 0) old[e] = atomicAdd(&s.mass[b[e]][0], (unsigned) wv[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const unsigned wh = (unsigned) (wv[e] >> 32) + (old[e] + (unsigned) wv[e] < old[e]);
+                        if (b[e] >= 0 && wh) atomicAdd(&s.mass[b[e]][1], wh);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int b = bin_of((&q.x)[e]);
+                        if (b >= 0) atomicAdd(&s.cnt[b], 1u);
+                    }
                 }
             }
             cl.sync();
