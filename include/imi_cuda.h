@@ -272,7 +272,7 @@ imi_cuda_status imi_cuda_q4_matvec_static(int device, const uint8_t *q4, int row
  * independent as long as they write different buffers (outputs, workspaces and status words included).
  * What only the device can see (lengths, page numbers, slots) is checked there: nothing outside the buffers is read or
  * written, and the largest IMI_DEV_* code met is left in the call's status word (atomic maximum; a call never clears
- * it: the caller zeroes it when it has read it). */
+ * it: the caller zeroes it when it has read it). Where a call takes no status word, what it met is not reported. */
 typedef enum { IMI_F32 = 0, IMI_F16 = 1, IMI_BF16 = 2 } imi_cuda_type;
 enum {
     IMI_DEV_PAGE = 1,    /* a page number outside 0..n_pages-1, or a slot beyond the last page */

@@ -304,7 +304,65 @@ def test_attn_bad_pages_and_lengths(prefix):
     run_attn(c, status_want=2)
 
 
-def test_attn_offsets_beyond_32_bits():
+@pytest.mark.parametrize("dt,d", [("f16", 64), ("bf16", 128)])
+def test_attn_bad_pages_of_a_prompt_for_many_rows(dt, d):
+    c = attn_case(9, 2, 4, d, dt, 16, 700, [3, 0, 40, 1, 2, 5, 16, 17, 0])
+    for j, bad in ((0, -1), (8, c["k"].shape[0]), (9, 2 ** 31 - 1), (43, -2 ** 31)):   # the first, two in a tile, the last
+        c["prefix"][j] = bad
+    run_attn(c, status_want=1)
+    run_attn(c, status_want=1, window=500)
+
+
+@pytest.mark.parametrize("prefix", [1, 15, 127, 128, 129, 255, 256, 257, 384, 1023])
+@pytest.mark.parametrize("rows,g,d", [(5, 4, 64), (33, 4, 64), (90, 3, 64), (6, 3, 128), (70, 2, 128)])
+def test_attn_tile_borders(prefix, rows, g, d):
+    c = attn_case(rows, 1, g, d, "f16", 16, prefix, [300] + [i % 3 for i in range(rows - 1)])
+    run_attn(c)
+    run_attn(c, window=130)
+
+
+def test_attn_long_prompt_in_many_parts():
+    """A prompt of 90,001 positions whose parts are ended by the number of tiles a part holds (its pages repeat); the
+    restatement on the device, in 64 bits."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    rows, kv, d, page, P = 18, 64, 64, 256, 90001
+    pages = [torch.randn((7, kv, page, d), generator=gen, device="cuda").half() for _ in range(2)]
+    prefix = torch.randint(0, 7, (-(-P // page),), generator=gen, device="cuda", dtype=I32)
+    q = torch.randn((rows, kv, d), generator=gen, device="cuda").half()
+    out, lse = torch.zeros_like(q), torch.zeros((rows, kv), device="cuda")
+    table, length = torch.zeros((rows, 1), dtype=I32, device="cuda"), torch.zeros(rows, dtype=I32, device="cuda")
+    nb.prefix_attn(q, *pages, prefix, P, table, length, out=out, lse=lse, work=nb.prefix_attn_work(q, pages[0], P, table))
+    for h in range(kv):
+        k, v = (p[prefix.long(), h].reshape(-1, d)[:P].double() for p in pages)
+        x = q[:, h].double() @ k.T * d ** -0.5
+        z = torch.logsumexp(x, 1)
+        e = torch.exp(x - z[:, None])
+        o, spread = e @ v, e @ v.abs()
+        reach = (q[:, h].double().abs() @ k.abs().T).amax(1)
+        ds = (d ** -0.5 * reach * (d * 2.0 ** -23 + 2.0 ** -22))[:, None]   # as in check_attn
+        tol = spread * (2 * ds + HALF["f16"] + 2.0 ** -21 + P * 2.0 ** -23) + o.abs() * HALF["f16"] + 2.0 ** -25 + P * 2.0 ** -25 * v.abs().max()
+        assert ((out[:, h].double() - o).abs() <= tol).all()
+        assert ((lse[:, h].double() - z).abs() <= ds[:, 0] + P * 2.0 ** -23 + 2.0 ** -21 + 2.0 ** -22 * z.abs()).all()
+
+
+def test_attn_two_calls_at_once():
+    """Two streams, each with its own workspace and outputs."""
+    cases = [attn_case(40, 2, 4, 64, "f16", 16, 1500, [(13 * i) % 300 for i in range(40)], seed=s) for s in (1, 2)]
+    want = [run_attn(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    works = [nb.prefix_attn_work(c["q"], c["k"], 1500, c["table"]) for c in cases]
+    outs = [(torch.zeros_like(c["q"]), torch.zeros(c["q"].shape[:2], device="cuda")) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, st, w, (o, l) in zip(cases, streams, works, outs):
+            nb.prefix_attn(c["q"], c["k"], c["v"], c["prefix"], 1500, c["table"], c["length"], out=o, lse=l, work=w, stream=st)
+    torch.cuda.synchronize()
+    for (o, l), (wo, wl) in zip(outs, want):
+        assert torch.equal(o, wo) and torch.equal(l, wl)
+
+
+@pytest.mark.parametrize("rows", [2, 7])
+def test_attn_offsets_beyond_32_bits(rows):
     """A cache of 2^32 elements and more: the pages used lie at its start, across 2^31 and 2^32, and at its end."""
     kv, page, d = 8, 256, 64
     n_pages = 2 ** 32 // (kv * page * d) + 9
@@ -313,8 +371,8 @@ def test_attn_offsets_beyond_32_bits():
     for p in pages:
         for u in used:
             p[u].normal_()
-    small = {"q": torch.randn((2, 32, 64), device="cuda").half(), "prefix": dev([5, 1, 2, 3], I32), "prefix_len": 1000,
-             "table": dev([[4, 0], [0, 4]], I32), "length": dev([300, 11], I32), "dt": "f16",
+    small = {"q": torch.randn((rows, 32, 64), device="cuda").half(), "prefix": dev([5, 1, 2, 3], I32), "prefix_len": 1000,
+             "table": dev(([[4, 0], [0, 4]] * rows)[:rows], I32), "length": dev(([300, 11] * rows)[:rows], I32), "dt": "f16",
              "k": pages[0][used].clone(), "v": pages[1][used].clone()}
     want = run_attn(small)
     at = dev(used, I32)
@@ -459,6 +517,17 @@ def test_sample_masked_infinite_and_nan():
         run_sample(far, 0.5, k=k, t=1e6)
         run_sample(far, 0.5, k=k, p=0.5, t=1e7)
     run_sample(far, 0.5, p=0.5, t=1e9)
+
+
+def test_sample_nuclei_that_end_anywhere():
+    """Flat and steep rows, so that nuclei end in the list, near its end and far below it; borders at p times a sum that the
+    32-bit mass only brackets."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rank = torch.arange(60000, device="cuda").float()
+    for steep in (0.0, 0.3, 0.7, 1.0, 1.3, 2.0, 4.0):
+        x = (-steep * torch.log1p(rank) + 0.01 * torch.randn((6, 60000), generator=g, device="cuda"))[:, torch.randperm(60000, generator=g, device="cuda")]
+        for p in (0.01, 0.3, 0.6, 0.9, 0.99, 0.99999):
+            run_sample(x, np.array([0.0, 0.2, 0.4, 0.6, 0.8, 0.999]), p=p, m=0.0 if p < 0.9 else 1e-3)
 
 
 def test_sample_crowded_scores():
