@@ -706,27 +706,53 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, 
 struct PaPlan {
     int splits, len;        // pieces of a query row over the prompt at most; positions of a piece (k_pa_pieces)
     bool mma, pair;
-    int tiles, span, per, rtiles, grid;
+    int tiles, span, per, rtiles, grid, own_sms;
     size_t pre_slots, own_slots;
     size_t off_bytes, bytes;
 };
-PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len) {
+// The prompt's tiles over `sms` CTAs: either a whole number of pieces per unit, or the line cut evenly, whose CTAs may have to
+// begin a unit anew (about PM_BEGIN tiles' time each). Returns the tiles' time of the longest CTA.
+int pm_cut(PaPlan &p, int n_head_kv, int sms) {
+    const long long units = (long long) p.rtiles * n_head_kv, total = units * p.tiles;
+    const long long k = std::max(1ll, std::min<long long>(sms / units, p.tiles)), whole = (p.tiles + k - 1) / k, even = (total + sms - 1) / sms;
+    const long long t_whole = (units * k + sms - 1) / sms * (whole + PM_BEGIN), t_even = even + PM_BEGIN * (1 + (even + p.tiles - 1) / p.tiles);
+    const bool cut = t_whole > t_even;
+    p.per = (int) std::max<long long>(PM_MIN_TILES, std::min<long long>(PM_MAX_TILES, cut ? even : whole));
+    p.span = cut ? p.tiles : (p.tiles + p.per - 1) / p.per * p.per;
+    p.grid = (int) ((units * p.span + p.per - 1) / p.per);
+    p.splits = ((p.tiles + p.per - 1) / p.per + (cut ? 1 : 0)) * (p.pair ? 2 : 1);
+    return (int) std::min<long long>(INT32_MAX, std::max<long long>(std::min(t_whole, t_even), p.per + PM_BEGIN));
+}
+
+// own_most: own positions of a row at most
+PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len, long long own_most) {
     PaPlan p = {};
+    p.own_sms = 148;
     const int g = n_head / n_head_kv, R = 16, tiles = (rows * g + R - 1) / R;
     p.mma = rows * g > PM_MIN_ROWS && prefix_len > 0;
     if (p.mma) {
         p.pair = rows * g <= PM_M;
         p.rtiles = p.pair ? 1 : (rows * g + PM_ROWS - 1) / PM_ROWS;
         p.tiles = (prefix_len + PM_N - 1) / PM_N;
-        // 148 CTAs: either a whole number of pieces per unit, or the line cut evenly, whose CTAs may have to begin a unit anew
-        // (about PM_BEGIN tiles' time each)
-        const long long units = (long long) p.rtiles * n_head_kv, total = units * p.tiles;
-        const long long k = std::max(1ll, std::min<long long>(148 / units, p.tiles)), whole = (p.tiles + k - 1) / k, even = (total + 147) / 148;
-        const bool cut = (units * k + 147) / 148 * (whole + PM_BEGIN) > even + PM_BEGIN * (1 + (even + p.tiles - 1) / p.tiles);
-        p.per = (int) std::max<long long>(PM_MIN_TILES, std::min<long long>(PM_MAX_TILES, cut ? even : whole));
-        p.span = cut ? p.tiles : (p.tiles + p.per - 1) / p.per * p.per;
-        p.grid = (int) ((units * p.span + p.per - 1) / p.per);
-        p.splits = ((p.tiles + p.per - 1) / p.per + (cut ? 1 : 0)) * (p.pair ? 2 : 1);
+        // The prompt's CTAs take a whole SM each, and wait for their exponentials; the own positions wait for HBM. So both run at
+        // once where that is shorter than one after the other, the own ones, taken to be half of what the tables hold, on the SMs
+        // that are left (45 GB/s each). They may be fewer: the prompt is not made slower than by a quarter (and 4 us) for them.
+        // 256 conversations on 16,384 positions with 128 own ones each: 81 us one after the other, 77 at once; 64 on 8,000 with 50: 28, 23.5
+        const double tile = head_dim == 64 ? 1.55 : 1.9, begin = 5.0;
+        const double own = 2.0 * rows * n_head_kv * head_dim * (double) own_most / 45e3;
+        const double alone = begin + tile * pm_cut(p, n_head_kv, 148);
+        double best = own_most ? alone + 3.0 + own / 148 : alone;
+        int sms = 148;
+        for (int x = 144; x >= 8 && own_most; x -= 4) {
+            const double t = begin + tile * pm_cut(p, n_head_kv, x), o = 3.0 + own / (148 - x);
+            if (t > 1.25 * alone + 4.0) break;
+            if (std::max(t, o) < best) {
+                best = std::max(t, o);
+                sms = x;
+            }
+        }
+        pm_cut(p, n_head_kv, sms);
+        if (p.grid <= sms && sms < 148) p.own_sms = 148 - p.grid;
     }
     const int steps = (prefix_len + PA_STEP - 1) / PA_STEP;
     if (!p.mma) p.splits = prefix_len ? std::max(1, std::min(PA_PRE_ITEMS / std::max(1, tiles * n_head_kv), steps / PA_MIN_STEPS)) : 0;
@@ -799,8 +825,7 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
                        (size_t) PA_WARPS * 16 * (D + 4) * 4, st, args);
     }
     if (r == cudaSuccess)
-        // own CTAs do not fit an SM beside one of k_pa_mma's: where those are few, the others' SMs are enough
-        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(pl.mma && pl.grid <= 74 ? PO_CTAS(D) / 148 * (148 - pl.grid) : PO_CTAS(D)), PA_WARPS * 32, (size_t) PA_WARPS * PO_STAGES * Pass<T, D, R8>::STAGE + (a.rows + 1) * 4, st, args);
+        r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(PO_CTAS(D) / 148 * pl.own_sms), PA_WARPS * 32, (size_t) PA_WARPS * PO_STAGES * Pass<T, D, R8>::STAGE + (a.rows + 1) * 4, st, args);
     if (r == cudaSuccess) {
         // warps per (row, head): one up to 16 pieces of the prompt; more while the SMs hold them (148 x 64 warps)
         int ways = 1;
@@ -837,7 +862,7 @@ using namespace imi;
 extern "C" size_t imi_cuda_prefix_attn_work(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len, int width,
                                             int page) {
     if (!pa_shape_ok(rows, n_head, n_head_kv, head_dim, prefix_len, width, page)) return 0;
-    return pa_plan(rows, n_head, n_head_kv, head_dim, prefix_len).bytes;
+    return pa_plan(rows, n_head, n_head_kv, head_dim, prefix_len, (long long) width * page).bytes;
 }
 
 extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefix_attn_args *a, void *stream) {
@@ -864,7 +889,7 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
     if (!aligned(a->q, 16) || !aligned(a->k_pages, 16) || !aligned(a->v_pages, 16) || !aligned(a->out, 16) || !aligned(a->work, 16) ||
         !aligned(a->prefix, 4) || !aligned(a->table, 4) || !aligned(a->length, 4) || !aligned(a->lse, 4) || !aligned(a->status, 4))
         return set_error(IMI_E_ARG, "prefix_attn: a buffer is not aligned (q, pages, out and work: 16 bytes)");
-    const PaPlan pl = pa_plan(a->rows, a->n_head, a->n_head_kv, a->head_dim, a->prefix_len);
+    const PaPlan pl = pa_plan(a->rows, a->n_head, a->n_head_kv, a->head_dim, a->prefix_len, (long long) a->width * a->page);
     if (a->work_bytes < pl.bytes)
         return set_error(IMI_E_ARG, "prefix_attn: the workspace takes " + std::to_string(pl.bytes) + " bytes (imi_cuda_prefix_attn_work)");
     OnDevice on(device);
