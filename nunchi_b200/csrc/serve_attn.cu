@@ -14,6 +14,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace imi {
@@ -844,14 +845,26 @@ cudaError_t launch_pa_t(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
 template <typename T>
 cudaError_t raise_pa(int device) {
     static SmemLimit lim, lim2;
-    return lim.raise(device,
-                     { (const void *) k_pa_direct<T, 64, true>, (const void *) k_pa_direct<T, 64, false>,
-                       (const void *) k_pa_direct<T, 128, true>, (const void *) k_pa_direct<T, 128, false>,
-                       (const void *) k_pa_pieces<T, 64>, (const void *) k_pa_pieces<T, 128>, (const void *) k_pa_own<T, 64, true>,
-                       (const void *) k_pa_own<T, 64, false>, (const void *) k_pa_own<T, 128, true>, (const void *) k_pa_own<T, 128, false> },
-                     112 * 1024 + PA_ROWS * 4) == cudaSuccess
-               ? lim2.raise(device, { (const void *) k_pa_mma<T, 64>, (const void *) k_pa_mma<T, 128> }, (int) std::max(PmSmem<64>::TOTAL, PmSmem<128>::TOTAL) + 1024)
-               : cudaErrorUnknown;
+    cudaError_t r = lim.raise(device,
+                              { (const void *) k_pa_direct<T, 64, true>, (const void *) k_pa_direct<T, 64, false>,
+                                (const void *) k_pa_direct<T, 128, true>, (const void *) k_pa_direct<T, 128, false>,
+                                (const void *) k_pa_pieces<T, 64>, (const void *) k_pa_pieces<T, 128>,
+                                (const void *) k_pa_own<T, 64, true>, (const void *) k_pa_own<T, 64, false>,
+                                (const void *) k_pa_own<T, 128, true>, (const void *) k_pa_own<T, 128, false> },
+                              112 * 1024 + PA_ROWS * 4);
+    if (r != cudaSuccess) return r;
+    r = lim2.raise(device, { (const void *) k_pa_mma<T, 64>, (const void *) k_pa_mma<T, 128> },
+                   (int) std::max(PmSmem<64>::TOTAL, PmSmem<128>::TOTAL) + 1024);
+    if (r != cudaSuccess) return r;
+    static std::atomic<bool> seen{ false };   // a property of the build, the same on every device
+    if (seen) return cudaSuccess;
+    for (const void *f : { (const void *) k_pa_mma<T, 64>, (const void *) k_pa_mma<T, 128> }) {
+        cudaFuncAttributes at;
+        if ((r = cudaFuncGetAttributes(&at, f)) != cudaSuccess) return r;
+        if (at.numRegs < PM_REGS) return cudaErrorLaunchOutOfResources;
+    }
+    seen = true;
+    return cudaSuccess;
 }
 
 }  // namespace

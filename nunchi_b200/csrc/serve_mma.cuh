@@ -25,7 +25,10 @@ constexpr int PM_MIN_TILES = 2;        // position tiles of a piece at least
 constexpr int PM_BEGIN = 3;            // what a unit's beginning and end take, in tiles
 constexpr int PM_MAX_TILES = 256;      // and at most (its page numbers are held in shared memory)
 constexpr int PM_THREADS = 12 * 32;
-constexpr int PM_REGS = 168, PM_REGS_FEW = 80, PM_REGS_MANY = 208;   // 4 x 80 + 8 x 208 <= 12 x 168
+// registers of a thread: at the launch (the host looks before the first one), then of the four warps that feed and the eight
+// of the softmax; what those take has to be among the launch's, or they would wait for it for good
+constexpr int PM_REGS = 168, PM_REGS_FEW = 80, PM_REGS_MANY = 208;
+static_assert(4 * PM_REGS_FEW + 8 * PM_REGS_MANY <= 12 * PM_REGS, "setmaxnreg draws on the launch's own registers");
 constexpr float PM_RISE = 8.0f;
 constexpr int PM_HAND = 2;              // of four parts of a tile's exponentials, the one behind which the other stream begins
 constexpr int PM_POLY = 4;              // every PM_POLY-th pair's exponentials by the FMA units
