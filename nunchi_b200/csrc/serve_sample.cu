@@ -69,7 +69,7 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 struct SampleShared {
     union {
         struct {
-            unsigned cnt[SM_BINS], mass[SM_BINS][2];   // this CTA's histogram; mass: low and high words
+            unsigned cnt[SM_BINS], mass_lo[SM_BINS], mass_hi[SM_BINS];   // this CTA's histogram
         };
         struct {
             u64 list[SM_LIST];               // leading CTA: (key, ~id) of all CTAs' words
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 if (level == 0) return bin0(k);
                 return bin0(k) == in_bin ? (int) ((khi - k) / (uint32_t) width) : -1;
             };
-            for (int b = tid; b < SM_BINS; b += SM_NT) s.cnt[b] = s.mass[b][0] = s.mass[b][1] = 0;
+            for (int b = tid; b < SM_BINS; b += SM_NT) s.cnt[b] = s.mass_lo[b] = s.mass_hi[b] = 0;
             if (tid == 0) { s.bin = -1; s.lo = ~0u; s.hi = 0; s.n_list = s.n_all = 0; }
             __syncthreads();
             for (int o = 0; o < p.seg; o += SM_TILE) {
@@ -760,12 +760,12 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         b[e] = bin_of((&q.x)[e]);
-                        if (b[e] >= 0) old[e] = atomicAdd(&s.mass[b[e]][0], (unsigned) wv[e]);
+                        if (b[e] >= 0) old[e] = atomicAdd(&s.mass_lo[b[e]], (unsigned) wv[e]);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const unsigned wh = (unsigned) (wv[e] >> 32) + (old[e] + (unsigned) wv[e] < old[e]);
-                        if (b[e] >= 0 && wh) atomicAdd(&s.mass[b[e]][1], wh);
+                        if (b[e] >= 0 && wh) atomicAdd(&s.mass_hi[b[e]], wh);
                     }
                 } else {
 #pragma unroll
@@ -788,9 +788,9 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                         cn[0] += v.x;
                         cn[1] += v.y;
                     } else {
-                        const uint4 w = *(const uint4 *) &o.mass[2 * tid][0];
-                        ms[0] += (u64) w.y << 32 | w.x;
-                        ms[1] += (u64) w.w << 32 | w.z;
+                        const uint2 w0 = *(const uint2 *) &o.mass_lo[2 * tid], w1 = *(const uint2 *) &o.mass_hi[2 * tid];
+                        ms[0] += (u64) w1.x << 32 | w0.x;
+                        ms[1] += (u64) w1.y << 32 | w0.y;
                     }
                 }
             unsigned c0 = cn[0] + cn[1], tc;
