@@ -32,6 +32,7 @@ constexpr int PA_DIRECT = 1024;           // positions (prompt and own) up to wh
 constexpr int PA_DIRECT_CTAS = 296;       // (row, kv head)s; with more only
 constexpr int PA_DIRECT_ALL = 256;        // up to these
 constexpr int PA_DWARPS = 8;              // its warps
+constexpr int JOIN_WARPS = 148 * 4 * 8;   // of k_join<, 4>, that the SMs hold at once (registers)
 
 struct PaArgs {
     imi_cuda_prefix_attn_args a;
@@ -625,44 +626,52 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_own(const __grid_constant_
 
 #include "serve_mma.cuh"
 
-// out and lse of every (row, head) from its pieces: `ways` (1, 2, 4 or 8) warps each, more where the pieces are many
-template <int D>
-__global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, int ways) {
+// out and lse of every (row, head) from its pieces: `ways` (1, 2, 4 or 8) warps each, UN pieces' values of each on their way.
+// Bound by latency: the prompt's first pieces are asked for beside the length and the own pieces' place, not behind them.
+template <int D, int UN>
+__global__ void __launch_bounds__(256, UN == 2 ? 7 : UN == 4 ? 4 : 2) k_join(const __grid_constant__ PaArgs p, int ways) {
     __shared__ float sh[8][D + 4];
     const imi_cuda_prefix_attn_args &a = p.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, way = warp % ways;
+    const int x = blockIdx.x * (8 / ways) + warp / ways, i = x / a.n_head, h = x % a.n_head, ic = min(i, a.rows - 1);
+    int np = p.pre_splits;   // the prompt's pieces of this row
+    if (p.mma) {
+        const int u0 = (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.span;
+        np = ((u0 + p.tiles - 1) / p.per - u0 / p.per + 1) * (p.pair ? 2 : 1);
+    }
+    if (i >= a.rows) np = 0;
+    // D / 4 lanes hold four dimensions each; at D 64 the warp's halves take every other piece
+    constexpr int G = 32 / (D / 4);
+    const int part = lane / (D / 4), c = lane % (D / 4) * 4, step = G * ways;
+    const float *po = p.po + c;
+    float2 ml[UN];
+    float4 v[UN];
+    auto load = [&](int e, long long slot) {
+        ml[e] = p.pml[slot];
+        v[e] = *(const float4 *) (po + slot * D);
+    };
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, way = warp % ways;
-    const int x = blockIdx.x * (8 / ways) + warp / ways, i = x / a.n_head, h = x % a.n_head;
-    const int ic = min(i, a.rows - 1), len = a.length[ic], o0 = p.off[ic], o1 = p.off[ic + 1];
+    const int len = a.length[ic], o0 = p.off[ic], o1 = p.off[ic + 1];
+    int k = way * G + part;   // this lane's next piece
+#pragma unroll
+    for (int e = 0; e < UN; e++)
+        if (k + e * step < np) load(e, (long long) x * p.pre_splits + k + e * step);
     const bool live = i < a.rows && len >= 0;
     float m = -INFINITY, l = 0.0f;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    // D / 4 lanes hold four dimensions each; at D 64 the warp's halves take every other piece
-    constexpr int G = 32 / (D / 4);
-    const int part = lane / (D / 4), c = lane % (D / 4) * 4;
     if (live) {
-        int np = p.pre_splits;   // the prompt's pieces of this row
-        if (p.mma) {
-            const int u0 = (h / p.g * p.rtiles + (i * p.g + h % p.g) / (p.pair ? PM_M : PM_ROWS)) * p.span;
-            np = ((u0 + p.tiles - 1) / p.per - u0 / p.per + 1) * (p.pair ? 2 : 1);
-        }
         const int n = np + o1 - o0;
-        auto slot_of = [&](int k) -> long long {
-            return k < np ? (long long) x * p.pre_splits + k : p.own_slot0 + (long long) (o0 + k - np) * a.n_head + h;
-        };
-        for (int k0 = way * G; k0 < n; k0 += 4 * G * ways) {   // four pieces' values on their way
-            float2 ml[4];
-            float4 v[4];
+        const long long own = p.own_slot0 + (long long) (o0 - np) * a.n_head + h;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int k = k0 + e * G * ways + part;
-                const long long slot = slot_of(min(k, n - 1));
-                ml[e] = k < n ? p.pml[slot] : make_float2(-INFINITY, 0.0f);
-                v[e] = *(const float4 *) (p.po + slot * D + c);
-            }
+        for (int e = 0; e < UN; e++) {
+            const int q = k + e * step;
+            if (q >= n) ml[e] = make_float2(-INFINITY, 0.0f);
+            else if (q >= np) load(e, own + (long long) q * a.n_head);
+        }
+        while (true) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
+            for (int e = 0; e < UN; e++) {
                 const float top = fmaxf(m, ml[e].x), u = top == -INFINITY ? 0.0f : top, f = ex2(m - u), g = ex2(ml[e].x - u);
                 l = fmaf(l, f, g * ml[e].y);
                 // a piece that saw nothing adds nothing, whatever its sums hold
@@ -671,6 +680,14 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ PaArgs p, 
                     s.z = fmaf(s.z, f, g * v[e].z); s.w = fmaf(s.w, f, g * v[e].w);
                 }
                 m = top;
+            }
+            k += UN * step;
+            if (k - part >= n) break;
+#pragma unroll
+            for (int e = 0; e < UN; e++) {
+                const int q = k + e * step;
+                if (q < n) load(e, q < np ? (long long) x * p.pre_splits + q : own + (long long) q * a.n_head);
+                else ml[e] = make_float2(-INFINITY, 0.0f);
             }
         }
         if (G == 2) {
@@ -828,11 +845,22 @@ cudaError_t launch_pa(PaArgs &p, const PaPlan &pl, cudaStream_t st) {
     if (r == cudaSuccess)
         r = launch_pdl((const void *) k_pa_own<T, D, R8>, dim3(PO_CTAS(D) / 148 * pl.own_sms), PA_WARPS * 32, (size_t) PA_WARPS * PO_STAGES * Pass<T, D, R8>::STAGE + (a.rows + 1) * 4, st, args);
     if (r == cudaSuccess) {
-        // warps per (row, head): one up to 16 pieces of the prompt; more while the SMs hold them (148 x 64 warps)
+        // warps per (row, head): more while a row's pieces (the prompt's, and about a row's share of the own ones) are not asked
+        // for all at once and the SMs hold all CTAs at once (a second wave begins 4 us behind the first); then more pieces per
+        // warp, where its registers leave one wave too. Where there are more (row, head)s than that, fewer registers for more
+        // CTAs per SM. Whole calls: 64 rows of 32 heads 23.6 us with 4 pieces per warp, 31 with 12; 24 of 8, 80 pieces each,
+        // 20.6 with 12, 24.4 with 4
+        const long long own = 1 + std::min(((long long) a.width << p.shift) / (PO_MIN_STEPS * PA_STEP),
+                                           (long long) PO_ROUNDS * PO_CTAS(D) * PA_WARPS / (a.n_head_kv * a.rows));
+        const long long all = (long long) a.rows * a.n_head, pieces = pl.splits + own;
+        constexpr int G = 128 / D;
         int ways = 1;
-        while (ways < 8 && (pl.splits > 16 * ways || a.rows * a.n_head * ways < 4736)) ways *= 2;
+        while (ways < 8 && pieces > 4 * G * ways && all * ways * 2 <= JOIN_WARPS) ways *= 2;
         void *jargs[] = { &p, &ways };
-        r = launch_pdl((const void *) k_join<D>, dim3((a.rows * a.n_head * ways + 7) / 8), 256, 0, st, jargs);
+        const void *join = all * ways > JOIN_WARPS ? (const void *) k_join<D, 2>
+                           : pieces > 4 * G * ways && all * ways <= JOIN_WARPS / 2 ? (const void *) k_join<D, 12>
+                                                   : (const void *) k_join<D, 4>;
+        r = launch_pdl(join, dim3((unsigned) ((all * ways + 7) / 8)), 256, 0, st, jargs);
     }
     return r;
 }
