@@ -69,7 +69,7 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 struct SampleShared {
     union {
         struct {
-            unsigned cnt[SM_BINS], mass_lo[SM_BINS], mass_hi[SM_BINS];   // this CTA's histogram
+            unsigned bins[3][SM_BINS];   // this CTA's histogram: words, or their masses' 15-bit digits (2^15 words at most)
         };
         struct {
             u64 list[SM_LIST];               // leading CTA: (key, ~id) of all CTAs' words
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 if (level == 0) return bin0(k);
                 return bin0(k) == in_bin ? (int) ((khi - k) / (uint32_t) width) : -1;
             };
-            for (int b = tid; b < SM_BINS; b += SM_NT) s.cnt[b] = s.mass_lo[b] = s.mass_hi[b] = 0;
+            for (int b = tid; b < SM_BINS; b += SM_NT) s.bins[0][b] = s.bins[1][b] = s.bins[2][b] = 0;
             if (tid == 0) { s.bin = -1; s.lo = ~0u; s.hi = 0; s.n_list = s.n_all = 0; }
             __syncthreads();
             for (int o = 0; o < p.seg; o += SM_TILE) {
@@ -754,24 +754,21 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
                 if (by_mass)
 #pragma unroll
                     for (int e = 0; e < 4; e++) wv[e] = weigh((&q.x)[e]);
-                if (by_mass) {   // add64 for four words, the low halves' additions on their way together
-                    int b[4];
-                    unsigned old[4];
+                if (by_mass) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        b[e] = bin_of((&q.x)[e]);
-                        if (b[e] >= 0) old[e] = atomicAdd(&s.mass_lo[b[e]], (unsigned) wv[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const unsigned wh = (unsigned) (wv[e] >> 32) + (old[e] + (unsigned) wv[e] < old[e]);
-                        if (b[e] >= 0 && wh) atomicAdd(&s.mass_hi[b[e]], wh);
+                        const int b = bin_of((&q.x)[e]);
+                        if (b < 0) continue;
+                        const unsigned d0 = (unsigned) wv[e] & 32767, d1 = (unsigned) (wv[e] >> 15) & 32767, d2 = (unsigned) (wv[e] >> 30);
+                        if (d0) atomicAdd(&s.bins[0][b], d0);
+                        if (d1) atomicAdd(&s.bins[1][b], d1);
+                        if (d2) atomicAdd(&s.bins[2][b], d2);
                     }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int b = bin_of((&q.x)[e]);
-                        if (b >= 0) atomicAdd(&s.cnt[b], 1u);
+                        if (b >= 0) atomicAdd(&s.bins[0][b], 1u);
                     }
                 }
             }
@@ -783,14 +780,14 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             for (int r = 0; r < SM_MAX_CLUSTER; r++)
                 if (r < C) {
                     const SampleShared &o = *cl.map_shared_rank(&s, r);
+                    const uint2 v = *(const uint2 *) &o.bins[0][2 * tid];
                     if (!by_mass) {
-                        const uint2 v = *(const uint2 *) &o.cnt[2 * tid];
                         cn[0] += v.x;
                         cn[1] += v.y;
                     } else {
-                        const uint2 w0 = *(const uint2 *) &o.mass_lo[2 * tid], w1 = *(const uint2 *) &o.mass_hi[2 * tid];
-                        ms[0] += (u64) w1.x << 32 | w0.x;
-                        ms[1] += (u64) w1.y << 32 | w0.y;
+                        const uint2 v1 = *(const uint2 *) &o.bins[1][2 * tid], v2 = *(const uint2 *) &o.bins[2][2 * tid];
+                        ms[0] += v.x + ((u64) v1.x << 15) + ((u64) v2.x << 30);
+                        ms[1] += v.y + ((u64) v1.y << 15) + ((u64) v2.y << 30);
                     }
                 }
             unsigned c0 = cn[0] + cn[1], tc;
