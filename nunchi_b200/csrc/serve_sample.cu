@@ -166,7 +166,21 @@ struct Weigher {
     static __device__ __forceinline__ u64 raw(double w) { return (u64) __double_as_longlong(__fma_rn(w, SM_ONE, 4503599627370496.0)); }
     static __device__ __forceinline__ u64 whole(double w) { return raw(w) - RAW; }
     __device__ __forceinline__ u64 operator()(uint32_t k) const { return whole(real(k)); }
-    __device__ __forceinline__ u64 raw4(uint4 q) const { return (raw(real(q.x)) + raw(real(q.y))) + (raw(real(q.z)) + raw(real(q.w))); }
+    // four words' at once, with one branch for all: their chains of operations go side by side
+    __device__ __forceinline__ void four(const uint4 &q, double (&w)[4]) const {
+        if (odd) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = rare((&q.x)[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = real(value_of((&q.x)[e]));
+        }
+    }
+    __device__ __forceinline__ u64 raw4(const uint4 &q) const {
+        double w[4];
+        four(q, w);
+        return (raw(w[0]) + raw(w[1])) + (raw(w[2]) + raw(w[3]));
+    }
     __device__ __forceinline__ float logprob(uint32_t k, u64 total) const {
         const double d = k == kmax ? 0.0 : ((double) value_of(k) - xmax) * c * 0.69314718055994530942;
         return (float) (d - log((double) total / SM_ONE));
@@ -750,16 +764,15 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             __syncthreads();
             for (int o = 0; o < p.seg; o += SM_TILE) {
                 const uint4 q = *(const uint4 *) (mine + o);
-                u64 wv[4];
-                if (by_mass)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) wv[e] = weigh((&q.x)[e]);
                 if (by_mass) {
+                    double w[4];
+                    weigh.four(q, w);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int b = bin_of((&q.x)[e]);
                         if (b < 0) continue;
-                        const unsigned d0 = (unsigned) wv[e] & 32767, d1 = (unsigned) (wv[e] >> 15) & 32767, d2 = (unsigned) (wv[e] >> 30);
+                        const u64 wv = Weigher::whole(w[e]);
+                        const unsigned d0 = (unsigned) wv & 32767, d1 = (unsigned) (wv >> 15) & 32767, d2 = (unsigned) (wv >> 30);
                         if (d0) atomicAdd(&s.bins[0][b], d0);
                         if (d1) atomicAdd(&s.bins[1][b], d1);
                         if (d2) atomicAdd(&s.bins[2][b], d2);
