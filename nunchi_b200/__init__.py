@@ -520,6 +520,8 @@ def prefix_attn(q, k_pages, v_pages, prefix, prefix_len, table, length, *, out, 
         raise _bad("q, out: [rows][n_head][head_dim] with contiguous heads of the pages' size are wanted")
     if q.dtype is not k_pages.dtype:
         raise _bad("q and the pages have one type")
+    if not work.is_contiguous():
+        raise _bad("work: a contiguous array is wanted")
     tp, ts, width = _table(table, "table", rows)
     one = heads * d if rows <= 1 else 0   # the stride of a single row does not matter
     _call(lib().imi_cuda_prefix_attn, q, _PREFIX_ATTN.pack(

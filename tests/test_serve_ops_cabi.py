@@ -111,3 +111,15 @@ def test_argument_blocks_match_the_header(tmp_path):
         for k in range(len(fmt)):
             at.append(struct.calcsize("@" + fmt[:k] + "0" + fmt[k]))
         assert at == offsets, n
+
+
+def test_python_refuses_a_strided_workspace():
+    torch = pytest.importorskip("torch")
+    pages = [torch.zeros(4, 1, 16, 64, dtype=torch.float16) for _ in range(2)]
+    q, out = (torch.zeros(1, 4, 64, dtype=torch.float16) for _ in range(2))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    call = lambda work: nb.prefix_attn(q, *pages, i32(0), 16, i32(1, 2)[None], i32(5), out=out, work=work)
+    with pytest.raises(nb.ImiError, match="contiguous"):
+        call(torch.zeros(1 << 20, dtype=torch.uint8)[::2])
+    with pytest.raises(nb.ImiError, match="device arrays"):
+        call(torch.zeros(1 << 20, dtype=torch.uint8))
