@@ -17,6 +17,8 @@
 //   A nucleus, or a top-k, that goes on below the list: a histogram over 1,024 steps of score, of masses (or counts), is
 // searched, the crossing bin's words listed and searched in turn; a bin too full for a list (scores crowded in few steps,
 // masked words) is cut again, by keys, until it fits or is a single value. Then every CTA sums its kept words by id.
+// Measured on rows of 97,496: one by top-k 50 and top-p 8.0 us; 64 by top-k 50 and top-p 12.4, by top-p 0.9 alone 51 (7 rows below
+// the list; the others are done at 14); 256 of bf16 with mixed settings 76. Bound by the chains of barriers and searches.
 #include "common.cuh"
 #include "serve.h"
 
@@ -43,6 +45,7 @@ constexpr double SM_MASS_ERR = 45 * 0.7 * 2.4e-7 + 2.4e-7 + 3.9e-6;
 constexpr int SM_TILE = 128;             // words of a warp's load: four per lane
 constexpr int SM_MAX_CLUSTER = 8;
 constexpr int SM_SLICE = 32768;          // words a CTA holds at most
+constexpr int SM_FEW(int c) { return c < 4 ? 96 : 48; }   // CTAs of a call, of c per row, below which its rows get twice as many
 constexpr double SM_ONE = 17592186044416.0;   // 2^44
 static_assert((long long) SM_SLICE * SM_MAX_CLUSTER >= IMI_CUDA_SAMPLE_VOCAB, "a row fits a cluster");
 static_assert((long long) IMI_CUDA_SAMPLE_VOCAB <= 1 << 18, "the weights' sum fits 62 bits");
@@ -1040,9 +1043,11 @@ cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void 
     static SmemLimit lim;
     cudaError_t r = lim.raise(device, { (const void *) k_sample<float>, (const void *) k_sample<__half>, (const void *) k_sample<__nv_bfloat16> },
                               (int) sample_smem(SM_SLICE));
-    // CTAs per row: as many as hold the row, more while the rows leave SMs idle and a CTA keeps a tile per warp
+    // CTAs per row: as many as hold the row, more while the call has few (SM_FEW) and a CTA keeps a tile per warp. More CTAs help
+    // the passes over the row (one row of 97,496 by nucleus: 22 us with 8, 25.9 with 4; 16 of 32,000: 15.4 with 4, 38 with 1),
+    // and cost where the short way does (32 rows of 32,000 by top-k: 8.1 us with 4, 15.4 with 8; 64 of 8,000: 7.1 with 2, 8.9 with 4)
     int C = 1;
-    while (C < SM_MAX_CLUSTER && ((a.vocab + C - 1) / C > SM_SLICE || (a.n * C < 148 && a.vocab > C * SM_NW * SM_TILE))) C *= 2;
+    while (C < SM_MAX_CLUSTER && ((a.vocab + C - 1) / C > SM_SLICE || (a.n * C < SM_FEW(C) && a.vocab > C * SM_NW * SM_TILE))) C *= 2;
     SampleArgs p = { a, 0, 0, rows, picks };
     p.seg = ((a.vocab + C * SM_NW - 1) / (C * SM_NW) + SM_TILE - 1) / SM_TILE * SM_TILE;
     p.slice = p.seg * SM_NW;
