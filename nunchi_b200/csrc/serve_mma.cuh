@@ -411,17 +411,21 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                     pm_fence_before();
                     pm_arrive(&s_read[st]);
                 }
-                if (masked)
+                // masked behind the scale: a scale of 0 must not meet the mask's infinity. sc: what the scores still take
+                float sc = sl2;
+                if (masked) {
 #pragma unroll
                     for (int x = 0; x < PM_N; x++)
-                        if (x < from || x >= to || (groups >> (x / 16) & 1)) v[x] = -INFINITY;
+                        v[x] = x < from || x >= to || (groups >> (x / 16) & 1) ? -INFINITY : v[x] * sl2;
+                    sc = 1.0f;
+                }
                 float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
                 for (int x = 0; x < PM_N; x += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) t4[e] = fmaxf(t4[e], fmaxf(v[x + e], v[x + e + 4]));
                 float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                top = top == -INFINITY ? top : top * sl2;
+                top = top == -INFINITY ? top : top * sc;
                 const bool raise = top > m + PM_RISE || (m == -INFINITY && top > m);
                 const bool any = __any_sync(~0u, raise);
                 // the product of the tile before reads P and adds to O: done before either is written
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                     if (!ok) break;
                 }
                 const float u = m == -INFINITY ? 0.0f : -m;
-                const float2 s2 = make_float2(sl2, sl2), u2 = make_float2(u, u);
+                const float2 s2 = make_float2(sc, sc), u2 = make_float2(u, u);
                 float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
