@@ -338,8 +338,9 @@ imi_cuda_status imi_cuda_page_write(int device, const imi_cuda_page_write_args *
  *   out[i][h] = sum_j p_j V_j,  p = softmax(scale * q[i][h] . K_j),  lse[i][h] = log sum_j exp(scale * q . K_j)
  * Head h reads kv head h / (n_head / n_head_kv). The prompt's pages are read once for the whole batch. A conversation
  * that sees nothing gets out 0 and lse -infinity. length[i] < 0: the row is not in use, its out and lse stay as they
- * were. Positions beyond a length may hold anything, NaN included; a NaN or infinity in V at a prompt position that some
- * conversation's window includes may reach the others' outputs too.
+ * were. A score of NaN or +infinity at a position that a conversation sees makes its out and lse NaN. Positions beyond a
+ * length may hold anything, NaN included; a NaN or infinity in V at a prompt position that some conversation's window
+ * includes may reach the others' outputs too.
  * type: IMI_F16 or IMI_BF16, of q and the pages; products, softmax and sums are held in 32 bits, the probabilities
  * rounded to `type` for their product with V. out_type: any imi_cuda_type. head_dim 64 or 128; n_head / n_head_kv at
  * most 16; rows at most 4096; page a power of two, 16..256; q and pages 16-byte aligned, q's and out's rows

@@ -118,9 +118,16 @@ __device__ __forceinline__ void pm_st16(uint32_t t, const uint32_t (&u)[16]) {
 __device__ __forceinline__ void pm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 2^x for a pair by the FMA units: n the nearest integer, 2^(x - n) by the polynomial through its values at 6 Chebyshev nodes
-// (relative error below 2^-21, ex2.approx's is 2^-22), n into the exponent. Below 2^-126: about 2^-126
+// (relative error below 2^-21, ex2.approx's is 2^-22), times 2^n. Below 2^-126 0, as ex2.approx.ftz gives it (a masked score's
+// weight, whatever V holds there), and a NaN stays one: hence the maximum that keeps it, and a product for 2^n where an addition
+// to the exponent's bits would make numbers of both
+__device__ __forceinline__ float pm_max_nan(float x, float y) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+    return m;
+}
 __device__ __forceinline__ float2 pm_exp2(float2 x) {
-    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+    x = make_float2(pm_max_nan(x.x, -127.0f), pm_max_nan(x.y, -127.0f));
     const float2 b = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f)),   // 1.5 * 2^23: n in the low bits
                  n = __fadd2_rn(b, make_float2(-12582912.0f, -12582912.0f)), f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
     float2 e = __ffma2_rn(f, make_float2(0.0013390863f, 0.0013390863f), make_float2(0.009676032f, 0.009676032f));
@@ -128,8 +135,8 @@ __device__ __forceinline__ float2 pm_exp2(float2 x) {
     e = __ffma2_rn(f, e, make_float2(0.24022107f, 0.24022107f));
     e = __ffma2_rn(f, e, make_float2(0.6931472f, 0.6931472f));
     e = __ffma2_rn(f, e, make_float2(1.0f, 1.0f));
-    return make_float2(__int_as_float(__float_as_int(e.x) + (__float_as_int(b.x) << 23)),
-                       __int_as_float(__float_as_int(e.y) + (__float_as_int(b.y) << 23)));
+    return __fmul2_rn(e, make_float2(__int_as_float((__float_as_int(b.x) << 23) + 0x3f800000),    // n = -127: 0
+                                     __int_as_float((__float_as_int(b.y) << 23) + 0x3f800000)));
 }
 
 template <typename T, int D>

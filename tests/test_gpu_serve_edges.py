@@ -2,7 +2,8 @@
 them, against their restatement in 64 bits (tests/serve_plain.py)."""
 import pytest
 
-from test_gpu_serve_ops import attn_case, run_attn
+import nunchi_b200 as nb
+from test_gpu_serve_ops import attn_case, run_attn, torch
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +28,38 @@ def test_attn_scale_zero_and_negative(rows, dt, d, scale):
     c["prefix"][33] = -1
     run_attn(c, scale=scale, status_want=1)
     run_attn(attn_case(rows, 2, 4, d, dt, 16, 1408, lengths(rows), seed=rows), scale=scale)
+
+
+# ------------------------------------------------------------------------------------------ NaN and infinite scores
+@pytest.mark.parametrize("dt,d", [("f16", 64), ("bf16", 64), ("f16", 128)])
+@pytest.mark.parametrize("rows", ROWS)
+def test_attn_a_visible_key_that_is_not_a_number_shows(rows, dt, d):
+    """A NaN in K, or an infinite score, at a position that a row sees makes the row NaN, wherever in a tile it lies; below the
+    rows' windows it changes nothing."""
+    c = attn_case(rows, 2, 4, d, dt, 16, 1400, [3] * rows, seed=d)
+    c["q"].abs_().add_(0.1)                                     # so that an infinite K is an infinite score
+    out, lse = torch.zeros_like(c["q"]), torch.zeros(c["q"].shape[:2], device="cuda")
+    work = nb.prefix_attn_work(c["q"], c["k"], 1400, c["table"])
+    for bad in (float("nan"), float("inf")):
+        for pos in [*range(128, 160), 0, 1399]:
+            page, at = int(c["prefix"][pos // 16]), pos % 16
+            was = c["k"][page, :, at].clone()
+            c["k"][page, :, at] = bad
+            call = lambda window: nb.prefix_attn(c["q"], c["k"], c["v"], c["prefix"], 1400, c["table"], c["length"], out=out,  # noqa: E731
+                                                 lse=lse, work=work, window=window)
+            call(0)
+            assert out.isnan().all() and lse.isnan().all(), (bad, pos)
+            if pos in (134, 153):
+                run_attn(c, window=1100)
+            c["k"][page, :, at] = was
+    run_attn(c)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_attn_a_position_below_a_row_s_window_weighs_nothing(rows):
+    """Very large values in V at positions that one row sees and the others' windows have passed."""
+    own = [0] + [30] * (rows - 1)
+    c = attn_case(rows, 2, 4, 64, "bf16", 16, 1500, own, seed=rows, spread=4.0)
+    for pos in range(1302, 1318):                               # row 0 sees from 1300 on, the others from 1330
+        c["v"][int(c["prefix"][pos // 16]), :, pos % 16] = 1e37   # row 0's sum of 16 stays finite
+    run_attn(c, window=200)
