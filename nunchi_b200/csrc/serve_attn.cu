@@ -93,7 +93,8 @@ __device__ __forceinline__ void put_out(const imi_cuda_prefix_attn_args &a, long
     else put4((__nv_bfloat16 *) a.out + at, v);
 }
 
-// the positions of conversation i that its query sees: the prompt's from `plo`, its own from `olo` to `len`
+// the positions of conversation i that its query sees: the prompt's from `plo`, its own from `olo` to `len`. A row that is not in
+// use (len negative) sees nothing, so that under a window it does not hold down what the rows beside it are read from
 struct Seen {
     int len, plo, olo;
 };
@@ -105,7 +106,8 @@ __device__ __forceinline__ Seen seen_of(const PaArgs &p, int i) {
         if (a.status) atomicMax(a.status, IMI_DEV_TABLE);
         len = cap;
     }
-    const int low = a.window > 0 && len >= 0 ? max(0, a.prefix_len + len - a.window) : 0;
+    if (len < 0) return { len, a.prefix_len, 0 };
+    const int low = a.window > 0 ? max(0, a.prefix_len + len - a.window) : 0;
     return { len, min(low, a.prefix_len), max(0, low - a.prefix_len) };
 }
 

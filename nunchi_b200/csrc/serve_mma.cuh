@@ -245,8 +245,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
             if (tid == 0) low_of = INT32_MAX;
             __syncthreads();
             if (warp >= 4) {
-                lo = fr >= 0 ? seen_of(p, fr / p.g).plo : 0;
-                const int least = __reduce_min_sync(~0u, fr >= 0 ? lo : INT32_MAX);
+                const Seen v = fr >= 0 ? seen_of(p, fr / p.g) : Seen{ -1, 0, 0 };
+                lo = v.len < 0 ? 0 : v.plo;                    // a row not in use, whose piece nobody reads, masks no tile
+                const int least = __reduce_min_sync(~0u, v.len < 0 ? INT32_MAX : lo);
                 if (lane == 0) atomicMin(&low_of, least);
             }
             __syncthreads();

@@ -63,3 +63,33 @@ def test_attn_a_position_below_a_row_s_window_weighs_nothing(rows):
     for pos in range(1302, 1318):                               # row 0 sees from 1300 on, the others from 1330
         c["v"][int(c["prefix"][pos // 16]), :, pos % 16] = 1e37   # row 0's sum of 16 stays finite
     run_attn(c, window=200)
+
+
+# ---------------------------------------------------------------------------- windows, unused rows, what nobody sees
+def poison(c, low):
+    """NaN in K and V at the prompt's positions below `low`."""
+    for x in (c["k"], c["v"]):
+        for p in range(0, low, 16):
+            x[int(c["prefix"][p // 16]), :, :min(16, low - p)] = float("nan")
+
+
+WINDOWS = [(3000, 10), (3000, 130), (3000, 500), (3000, 2990), (2944, 100), (2944, 1024), (140, 60), (3000, 1)]
+
+
+@pytest.mark.parametrize("dt,d", [("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("prefix,window", WINDOWS)
+def test_attn_unused_rows_see_nothing(rows, dt, d, prefix, window):
+    """Rows that are not in use do not make the others read, under a window, what lies in front of all windows."""
+    own = lengths(rows, unused={1, rows - 1})
+    c = attn_case(rows, 2, 4, d, dt, 16, prefix, own, seed=window)
+    poison(c, (prefix + min(x for x in own if x >= 0) - window) // 128 * 128)
+    run_attn(c, window=window)
+
+
+def test_attn_no_row_in_use():
+    for rows in ROWS:
+        c = attn_case(rows, 2, 4, 64, "f16", 16, 1500, [5] * rows)
+        c["length"].fill_(-1)
+        run_attn(c)
+        run_attn(c, window=100)
