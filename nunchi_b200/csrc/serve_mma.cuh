@@ -11,7 +11,8 @@
 // thread run in the order of issue).
 //   warp 0       K and V rows from their pages by tensor copies of up to 128 rows x 128 bytes into rings of tiles (128-byte
 //                swizzle; the rows of a page that does not exist are read beyond the tensor's end, as zeros)
-//   warp 1       zeroes V's rows beyond the prompt's end in its last tile: what a page holds there may be anything
+//   warp 1       zeroes V's rows that nobody sees, beyond the prompt's end in its last tile and below the lowest window in a unit's
+//                first: what a page holds there may be anything
 //   warp 3       issues the products
 //   warps 4..7   softmax of stream 0, warps 8..11 of stream 1, with the registers that the others give up: a thread holds its
 //                row's 128 scores
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     uint8_t *sm = sm_raw + ((1024 - (smem_u32(sm_raw) & 1023)) & 1023);
     int *ids = (int *) (sm + L::IDS);
     uint64_t *k_full = (uint64_t *) (sm + L::BAR), *k_free = k_full + NK, *v_full = k_free + NK, *v_free = v_full + NV,
-             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *v_raw = o_full + 2, *q_full = v_raw + 1, *fin = q_full + 1,
+             *s_full = v_free + NV, *s_read = s_full + 2, *p_full = s_read + 2, *o_full = p_full + 2, *v_raw = o_full + 2, *q_full = v_raw + 2, *fin = q_full + 1,
              *turn_of = fin + 1;                               // [stream][warp]: the warp may begin its exponentials
     __shared__ uint32_t tmem_at;
     __shared__ int stop;
@@ -165,7 +166,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         for (int i = 0; i < NV; i++) { mbar_init(&v_full[i], 1); mbar_init(&v_free[i], 1); }
         for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&s_read[i], 128); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); }
         for (int i = 0; i < 8; i++) mbar_init(&turn_of[i], 1);
-        mbar_init(v_raw, 1);
+        mbar_init(&v_raw[0], 1);
+        mbar_init(&v_raw[1], 1);
         mbar_init(q_full, 256);
         mbar_init(fin, 1);
         stop = 0;
@@ -197,6 +199,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
     int at = (int) blockIdx.x * p.per;
     struct Unit {
         int kvh, row0, piece, page0, t0, t1, n0, n1;           // position tiles [t0, t1), of them the streams'
+        int low;                                               // the lowest position that a row of the unit sees
     };
     // the next unit's part, after the CTA is done with the one before: false where there is none. The page numbers are there
     // for warps 0..3 when it returns; the queries when q_full says so (the copies need not wait for them)
@@ -251,7 +254,8 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                 if (lane == 0) atomicMin(&low_of, least);
             }
             __syncthreads();
-            w.t0 = max(w.t0, min(w.t1, __shfl_sync(~0u, low_of, 0) / PM_N));
+            w.low = __shfl_sync(~0u, low_of, 0);
+            w.t0 = max(w.t0, min(w.t1, w.low / PM_N));
         } else if (warp < 4) {
             asm volatile("bar.sync 1, 128;" ::: "memory");     // the page numbers
         }
@@ -261,6 +265,10 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         return true;
     };
     Unit w = {};
+    // tiles of which nobody sees all V rows go past warp 1: the prompt's last by v_raw[1], a unit's first by v_raw[0]. At most one
+    // of each in a part, so neither barrier is ever two phases ahead of its waiter
+    auto at_end = [&](int t) { return (t + 1) * PM_N > a.prefix_len; };
+    auto at_low = [&](int t) { return t * PM_N < w.low && !at_end(t); };
     // the page of a position (a multiple of 16, or in its group of 16) of the part
     auto id_at = [&](int pos) { return ids[(pos >> p.shift) - w.page0]; };
 
@@ -291,7 +299,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                     nk++;
                     ok = __all_sync(~0u, wait(&v_free[vs], ((nv / NV) & 1) ^ 1));
                     if (!ok) break;
-                    load(v_map, t, sm + L::V + vs * L::TILE, (t + 1) * PM_N > a.prefix_len ? v_raw : &v_full[vs]);
+                    load(v_map, t, sm + L::V + vs * L::TILE, at_end(t) ? &v_raw[1] : at_low(t) ? &v_raw[0] : &v_full[vs]);
                     nv++;
                 }
                 if (!ok) {                                     // copies in flight land before the memory goes (bounded)
@@ -300,21 +308,24 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                 }
             }
         } else if (warp == 1) {
-            // ---------------- the prompt's end ----------------
-            int nv = 0, nr = 0;
+            // ---------------- V rows that nobody sees ----------------
+            int nv = 0, nr[2] = { 0, 0 };
             while (next(w)) {
-                if (w.t1 > w.t0 && w.t1 * PM_N > a.prefix_len) {
-                    const int vs = (nv + w.t1 - 1 - w.t0) % NV, rows = a.prefix_len - (w.t1 - 1) * PM_N;
-                    if (__all_sync(~0u, wait(v_raw, nr & 1))) {
+                auto clear = [&](int t, int end) {             // tile t: its rows below w.low, and from the prompt's end on
+                    const int vs = (nv + t - w.t0) % NV, lo = min(PM_N, max(0, w.low - t * PM_N)), hi = min(PM_N, a.prefix_len - t * PM_N);
+                    if (__all_sync(~0u, wait(&v_raw[end], nr[end] & 1))) {
                         uint8_t *v = sm + L::V + vs * L::TILE;
                         for (int half = 0; half < D / 64; half++)
-                            for (int x = rows * 8 + lane; x < PM_N * 8; x += 32) *(uint4 *) (v + half * (PM_N * 128) + x * 16) = make_uint4(0, 0, 0, 0);
+                            for (int x = lane; x < PM_N * 8; x += 32)
+                                if (x < lo * 8 || x >= hi * 8) *(uint4 *) (v + half * (PM_N * 128) + x * 16) = make_uint4(0, 0, 0, 0);
                         fence_proxy_async();
                         __syncwarp();
                         if (lane == 0) pm_arrive(&v_full[vs]);
                     }
-                    nr++;
-                }
+                    nr[end]++;
+                };
+                if (w.t1 > w.t0 && at_low(w.t0)) clear(w.t0, 0);
+                if (w.t1 > w.t0 && at_end(w.t1 - 1)) clear(w.t1 - 1, 1);
                 nv += w.t1 - w.t0;
             }
         } else if (warp == 2) {

@@ -93,3 +93,25 @@ def test_attn_no_row_in_use():
         c["length"].fill_(-1)
         run_attn(c)
         run_attn(c, window=100)
+
+
+@pytest.mark.parametrize("dt,d", [("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("prefix,window", WINDOWS)
+def test_attn_what_no_window_includes_may_be_anything(rows, dt, d, prefix, window):
+    own = lengths(rows)
+    c = attn_case(rows, 2, 4, d, dt, 16, prefix, own, seed=window)
+    low = prefix + min(own) - window
+    assert low > 0
+    poison(c, low)
+    run_attn(c, window=window)
+
+
+@pytest.mark.parametrize("window", [300, 3000, 9000, 19990])
+def test_attn_windows_on_a_long_prompt_in_many_parts(window):
+    """Parts of a prompt that begin below, in and behind the tile in which the lowest window begins, several to a CTA."""
+    for rows, kv in ((70, 3), (130, 1), (9, 5)):
+        own = lengths(rows, unused={0, 2})
+        c = attn_case(rows, kv, 4, 64, "f16", 16, 20000, own, seed=rows)
+        poison(c, 20000 + min(x for x in own if x >= 0) - window)
+        run_attn(c, window=window)
