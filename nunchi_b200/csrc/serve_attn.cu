@@ -23,6 +23,8 @@ namespace {
 constexpr int PA_ROWS = 4096;             // conversations at most
 constexpr int PA_WARPS = 4;               // warps of a piece's CTA
 constexpr int PA_STEP = 16;               // positions of a warp's step (a page holds whole steps)
+constexpr int PA_POSITIONS = 1 << 30;     // of the prompt and a table row together at most: a position and a piece's length behind it,
+                                          // or a whole tile, still fit 32 bits, as do the steps of all rows' tables (pa_shape_ok)
 constexpr int PA_MIN_STEPS = 2 * PA_WARPS;   // steps of a piece of the prompt at least
 constexpr int PO_MIN_STEPS = 4;           // of an own piece, which is one warp's
 constexpr int PO_ITEM_COST = 4, PO_ROUNDS = 3;   // own_plan
@@ -499,7 +501,7 @@ __device__ int own_plan(const PaArgs &p, int *off, int *tmp) {
     const long long warps = (long long) gridDim.x * PA_WARPS, work = (long long) sum * a.n_head_kv, rows = (long long) live * a.n_head_kv;
     // one round: at most work / chunk + rows items
     const int one = rows < warps ? (int) min((long long) max(1, most), (work + warps - rows - 1) / (warps - rows)) : INT32_MAX;
-    int chunk = max(PO_MIN_STEPS, (int) ((work + PO_ROUNDS * warps - 1) / (PO_ROUNDS * warps)));
+    int chunk = max(PO_MIN_STEPS, (int) min((long long) PA_POSITIONS / PA_STEP, (work + PO_ROUNDS * warps - 1) / (PO_ROUNDS * warps)));
     const long long rounds = (work / chunk + rows + warps - 1) / warps;
     if (one < INT32_MAX && one + PO_ITEM_COST <= rounds * (chunk + PO_ITEM_COST)) chunk = max(PO_MIN_STEPS, one);
     int cnt = 0;
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_pa_own(const __grid_constant_
         f.load_q(r < p.g ? q + r * D : nullptr, r + 8 < p.g ? q + (r + 8) * D : nullptr);
         const long long head = (long long) kvh * a.page * D;
         const Seen v = seen_of(p, row);
-        const int s0 = v.olo / PA_STEP + piece * chunk, lo = max(v.olo, s0 * PA_STEP), hi = min(v.len, (s0 + chunk) * PA_STEP);
+        const int s0 = v.olo / PA_STEP + piece * chunk, lo = max(v.olo, s0 * PA_STEP), hi = (int) min((long long) v.len, (s0 + (long long) chunk) * PA_STEP);
         f.run_ring(p, shb + warp * PO_STAGES * Pass<T, D, R8>::STAGE, a.table + row * a.table_stride, (const T *) a.k_pages + head,
                    (const T *) a.v_pages + head, ps, lo, hi);
         f.finish();
@@ -799,7 +801,7 @@ PaPlan pa_plan(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len
 bool pa_shape_ok(int rows, int n_head, int n_head_kv, int head_dim, int prefix_len, int width, int page) {
     return rows >= 0 && rows <= PA_ROWS && n_head_kv >= 1 && n_head >= n_head_kv && n_head <= 1024 && n_head % n_head_kv == 0 &&
            n_head / n_head_kv <= 16 && (head_dim == 64 || head_dim == 128) && prefix_len >= 0 && width >= 0 && page_ok(page) &&
-           (int64_t) width * page + prefix_len + page <= INT32_MAX;
+           (int64_t) width * page + prefix_len + page <= PA_POSITIONS && (int64_t) width * page / PA_STEP * rows <= INT32_MAX;
 }
 
 // the pages of K (or V) as rows of head_dim values, copied in boxes of up to 128 rows x 64 values with the 128-byte swizzle
@@ -916,7 +918,8 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
     if (a->out_type < IMI_F32 || a->out_type > IMI_BF16) return set_error(IMI_E_ARG, "prefix_attn: bad out_type");
     if (!pa_shape_ok(a->rows, a->n_head, a->n_head_kv, a->head_dim, a->prefix_len, a->width, a->page))
         return set_error(IMI_E_ARG, "prefix_attn: unsupported shape (rows up to " + std::to_string(PA_ROWS) +
-                                        ", head_dim 64 or 128, up to 16 heads per kv head, page a power of two in 16..256)");
+                                        ", head_dim 64 or 128, up to 16 heads per kv head, page a power of two in 16..256, prompt and table "
+                                        "row below 2^30 positions, all rows' tables below 2^35)");
     if (a->n_pages < 0 || a->window < 0) return set_error(IMI_E_ARG, "prefix_attn: negative n_pages or window");
     if (!std::isfinite(a->scale)) return set_error(IMI_E_ARG, "prefix_attn: scale is not finite");
     if (a->rows == 0) return IMI_OK;
