@@ -35,7 +35,8 @@ __device__ __forceinline__ int row_of(const int *first, int n, int j) {
 // the largest. Every CTA scans all lengths itself (8 n bytes from L2, at most 32 KB): no CTA waits for another, and
 // the table entries, slots and positions are then shared out evenly. What may alias an input (length, n_free_out) is
 // written by the CTA that is the last to have read its inputs; the count of those that have is asked for before the tables
-// and slots are written, and its answer used after that.
+// and slots are written, and its answer used after that. A CTA has read all of them by the scan's barrier; fences in front of
+// its count and behind the last one's order those reads before the writes.
 // Measured, one call behind the other: 64 decode steps 4.6 us, 384 prompts of 1,000,000 tokens at most (8 MB written) 10.9.
 __global__ void __launch_bounds__(MAP_THREADS) k_page_map(const __grid_constant__ MapArgs m) {
     extern __shared__ int sh[];
@@ -43,10 +44,10 @@ __global__ void __launch_bounds__(MAP_THREADS) k_page_map(const __grid_constant_
     const int n = a.n, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int *held = sh, *start = sh + n, *first = start + n + 1;
     __shared__ long long ws[2][MAP_THREADS / 32];
-    __shared__ int werr[MAP_THREADS / 32], last;
+    __shared__ int werr[MAP_THREADS / 32], last, free_now;
     pdl_wait();
     pdl_trigger();
-    const int n_free = *a.n_free;
+    if (tid == 0) free_now = *a.n_free;
     // each thread: `per` consecutive requests, then a scan of the threads' sums
     const int per = (n + MAP_THREADS - 1) / MAP_THREADS, i0 = min(n, tid * per), i1 = min(n, i0 + per);
     long long sa = 0, sn = 0;
@@ -72,6 +73,7 @@ __global__ void __launch_bounds__(MAP_THREADS) k_page_map(const __grid_constant_
     err = __reduce_max_sync(~0u, err);
     if (lane == 31) { ws[0][warp] = xa; ws[1][warp] = xn; werr[warp] = err; }
     __syncthreads();
+    const int n_free = free_now;
     long long ba = 0, bn = 0, ta = 0, tn = 0;
     err = 0;
 #pragma unroll
@@ -96,7 +98,10 @@ __global__ void __launch_bounds__(MAP_THREADS) k_page_map(const __grid_constant_
     int read = 0;   // thread 0: CTAs that had read their inputs before this one (whose threads all have, since the scan)
     if (tid == 0) {
         start[n] = rows;
-        if (gridDim.x > 1) read = atomicAdd(a.status + 1, 1);
+        if (gridDim.x > 1) {
+            __threadfence();
+            read = atomicAdd(a.status + 1, 1);
+        }
     }
     __syncthreads();
     bool bad = false;
@@ -131,7 +136,10 @@ __global__ void __launch_bounds__(MAP_THREADS) k_page_map(const __grid_constant_
     }
     if (bad) atomicMax(a.status, IMI_DEV_PAGE);
     if (gridDim.x > 1) {
-        if (tid == 0) last = read == (int) gridDim.x - 1;
+        if (tid == 0) {
+            last = read == (int) gridDim.x - 1;
+            if (last) __threadfence();
+        }
         __syncthreads();
         if (!last) return;
     }

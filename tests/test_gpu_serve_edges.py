@@ -1,9 +1,10 @@
 """The serving operators on calls at the edge of what the header allows (include/imi_cuda.h), each way of the attention among
 them, against their restatement in 64 bits (tests/serve_plain.py)."""
+import numpy as np
 import pytest
 
 import nunchi_b200 as nb
-from test_gpu_serve_ops import attn_case, run_attn, torch
+from test_gpu_serve_ops import I32, attn_case, dev, run_attn, torch
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +116,33 @@ def test_attn_windows_on_a_long_prompt_in_many_parts(window):
         c = attn_case(rows, kv, 4, 64, "f16", 16, 20000, own, seed=rows)
         poison(c, 20000 + min(x for x in own if x >= 0) - window)
         run_attn(c, window=window)
+
+
+# -------------------------------------------------------------------------------------------------------- page_map
+@pytest.mark.parametrize("n,cap,steps", [(384, 610000, 60), (4096, 40000, 25), (1, 2100, 200)])
+def test_page_map_in_place_step_after_step(n, cap, steps):
+    """Lengths and the free count in place, over many CTAs, one step behind the other without a wait: every step takes its
+    pages from where the one before left the list."""
+    rng = np.random.default_rng(n)
+    page, n_pages = 16, 16000 if n > 1 else 300
+    add = rng.integers(0, 2 if n > 1000 else 9, n)
+    width = -(-int(add.max()) * steps // page) + 1
+    order = rng.permutation(n_pages)
+    held, nf, free, a = dev(np.zeros(n), I32), dev([n_pages], I32), dev(order, I32), dev(add, I32)
+    table = torch.full((n, width), -1, dtype=I32, device="cuda")
+    start, slots, pos, status = (torch.zeros(k, dtype=I32, device="cuda") for k in (n + 1, cap, cap, 2))
+    for _ in range(steps):
+        nb.page_map(held, a, table, free, nf, page=page, n_pages=n_pages, start=start, length=held, slots=slots, pos=pos, n_free_out=nf,
+                    status=status)
+    want, left = np.full((n, width), -1), n_pages
+    for k in range(steps):
+        for i in range(n):
+            for c in range(-(-add[i] * k // page), -(-add[i] * (k + 1) // page)):
+                left -= 1
+                want[i, c] = order[left]
+    assert status.tolist() == [0, 0] and int(nf) == left
+    assert np.array_equal(held.cpu().numpy(), add * steps) and np.array_equal(table.cpu().numpy(), want)
+    p = np.concatenate([np.arange(x * (steps - 1), x * steps) for x in add])
+    i = np.repeat(np.arange(n), add)
+    assert np.array_equal(pos.cpu().numpy()[:p.size], p) and (slots.cpu().numpy()[p.size:] == -1).all()
+    assert np.array_equal(slots.cpu().numpy()[:p.size], want[i, p // page] * page + p % page)
