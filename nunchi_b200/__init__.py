@@ -403,9 +403,9 @@ def _types():
     global _F32, _F16, _BF16, _I32, _stream_of
     import torch
     _F32, _F16, _BF16, _I32 = torch.float32, torch.float16, torch.bfloat16, torch.int32
-    _TYPE.update({_F32: 0, _F16: 1, _BF16: 2})
     # the current stream's handle; the call that gives it without a Stream object where this torch has one
     _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    _TYPE.update({_F32: 0, _F16: 1, _BF16: 2})   # last: another thread that finds it filled does not come here
 
 
 def _bad(msg):
