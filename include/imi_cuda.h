@@ -94,7 +94,7 @@ imi_cuda_status imi_cuda_greedy(imi_cuda_state *const *s, int n, const int32_t *
 /* Sampling from conversations' latest word scores (imi picks greedily only): the words imi_cuda_sample (below) names for the
  * uniform numbers u[n], with per-conversation settings (arrays of n, host; NULL: temperature 1, the filters off). ids,
  * logprob and kept (each may be NULL) receive them. A word becomes its conversation's last pick: what imi_cuda_get_argmax
- * returns as id, and what a later imi_cuda_greedy or imi_cuda_sampled without tokens reads first. */
+ * returns, with its score, and what a later imi_cuda_greedy or imi_cuda_sampled without tokens reads first. */
 imi_cuda_status imi_cuda_sample_states(imi_cuda_state *const *s, int n, const float *u, const float *temperature,
                                        const int32_t *top_k, const float *top_p, const float *min_p, int32_t *ids, float *logprob,
                                        int32_t *kept);
@@ -128,7 +128,9 @@ imi_cuda_status imi_cuda_state_load(imi_cuda_state *s, const void *buf, size_t s
 /* The latest outputs of a conversation (imi_seoul::hidden / ::logits, seoul.h:51): host copies. */
 imi_cuda_status imi_cuda_get_hidden(const imi_cuda_state *s, float *out /* n_embd */);
 imi_cuda_status imi_cuda_get_logits(const imi_cuda_state *s, float *out /* n_vocab */);
-/* The greedy pick of the latest step with logits: first maximum, lowest id on ties (imi/core/hear.cpp:67-68). */
+/* The greedy pick of the latest step with logits: first maximum, lowest id on ties (imi/core/hear.cpp:67-68); or the word
+ * sampled since (imi_cuda_sample_states, imi_cuda_sampled). value (may be NULL): its score (0 behind imi_cuda_state_load,
+ * whose image does not hold it). */
 imi_cuda_status imi_cuda_get_argmax(const imi_cuda_state *s, int32_t *id, float *value);
 
 /* ---- the model file's keys and tensor headers (host only; imi_file, imi/model.h:17-36) ----

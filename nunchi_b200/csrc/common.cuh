@@ -31,9 +31,9 @@ constexpr int MV_SMEM_BUDGET = 220 * 1024; // shared memory of one table-read CT
 // Per-conversation scalars that live on the device (the rest of imi_seoul_state is device buffers).
 struct SessDev {
     int pos;                   // positions read so far (imi_seoul::pos)
-    int next_token;            // greedy pick of the latest step with logits
+    int next_token;            // greedy pick of the latest step with logits, or the word sampled since
     unsigned long long amax;   // running argmax key of the step in flight (0 between steps)
-    float amax_val;
+    float amax_val;            // its score
     int pad;
 };
 

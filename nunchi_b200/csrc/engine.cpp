@@ -1970,15 +1970,15 @@ size_t image_bytes(const imi_cuda_engine *e, int pos) {
 
 namespace {
 // one call's sampling data for up to ncmax conversations and SMP_STEPS steps, as it lies in host and device memory: scores'
-// addresses, picks' addresses, settings, then u[step][conversation], ids, logprobs, kept counts
+// addresses, records' addresses, settings, then u[step][conversation], ids, logprobs, kept counts
 constexpr int SMP_STEPS = 64;
 struct SampleBlock {
-    size_t rows, picks, temperature, top_k, top_p, min_p, u, ids, logprob, kept, in_bytes, bytes;
+    size_t rows, states, temperature, top_k, top_p, min_p, u, ids, logprob, kept, in_bytes, bytes;
     explicit SampleBlock(int nc) {
         size_t o = 0;
         auto take = [&](size_t n) { const size_t r = o; o = (o + n + 15) / 16 * 16; return r; };
         rows = take((size_t) nc * 8);
-        picks = take((size_t) nc * 8);
+        states = take((size_t) nc * 8);
         temperature = take((size_t) nc * 4);
         top_k = take((size_t) nc * 4);
         top_p = take((size_t) nc * 4);
@@ -2004,7 +2004,7 @@ imi_cuda_status sample_begin(imi_cuda_state *const *s, int n, int steps, const f
     uint8_t *h = e->smp_h;
     for (int c = 0; c < n; c++) {
         ((const void **) (h + b.rows))[c] = s[c]->logits;
-        ((int32_t **) (h + b.picks))[c] = &s[c]->s->next_token;
+        ((SessDev **) (h + b.states))[c] = s[c]->s;
         ((float *) (h + b.temperature))[c] = temperature ? temperature[c] : 1.0f;
         ((int32_t *) (h + b.top_k))[c] = top_k ? top_k[c] : 0;
         ((float *) (h + b.top_p))[c] = top_p ? top_p[c] : 1.0f;
@@ -2030,7 +2030,7 @@ imi_cuda_status sample_step(imi_cuda_engine *e, int n, int k) {
     a.ids = (int32_t *) (d + b.ids) + (size_t) k * n;
     a.logprob = (float *) (d + b.logprob) + (size_t) k * n;
     a.kept = (int32_t *) (d + b.kept) + (size_t) k * n;
-    CK(launch_sample(e->device, a, (const void *const *) (d + b.rows), (int32_t *const *) (d + b.picks), e->stream));
+    CK(launch_sample(e->device, a, (const void *const *) (d + b.rows), (SessDev *const *) (d + b.states), e->stream));
     e->gen++;   // the conversations' records have changed
     return IMI_OK;
 }

@@ -10,11 +10,13 @@
 #include <string>
 
 namespace imi {
+struct SessDev;   // common.cuh: a conversation's scalars on the device
+
 imi_cuda_status set_error(imi_cuda_status st, const std::string &msg);   // engine.cpp: the text of imi_cuda_error()
 
 // serve_sample.cu: sampling of checked arguments with `device` current; rows (or null): device pointers of the rows' scores,
-// picks (or null): where the words go besides a.ids
-cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void *const *rows, int32_t *const *picks, cudaStream_t st);
+// states (or null): the conversations whose last pick, with its score, the words become
+cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void *const *rows, SessDev *const *states, cudaStream_t st);
 
 // makes `device` current while it lives; ok() false: there is no such device
 class OnDevice {

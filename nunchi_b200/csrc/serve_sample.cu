@@ -56,7 +56,7 @@ struct SampleArgs {
     imi_cuda_sample_args a;
     int seg, slice;   // words per warp (a multiple of SM_TILE) and per CTA (SM_NW * seg)
     const void *const *rows;   // the rows' scores where they do not lie `stride` apart (the engine's conversations)
-    int32_t *const *picks;     // and where each row's word goes besides ids (not if there is none)
+    SessDev *const *states;    // and the conversations whose last pick each row's word becomes (not if there is none)
 };
 
 // scores as unsigned keys in the same order; NaN is -infinity, whose key no kept word has; the zeros are one
@@ -386,7 +386,10 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     uint32_t floor = max(__reduce_min_sync(~0u, lane < C ? s.all_floor[lane] : ~0u), KEY_NONE + 1);
     auto emit = [&](int id, float lp, int kept) {
         a.ids[row] = id;
-        if (p.picks && id >= 0) *p.picks[row] = id;
+        if (p.states && id >= 0) {
+            p.states[row]->next_token = id;
+            p.states[row]->amax_val = score_at(x, id);
+        }
         if (a.logprob) a.logprob[row] = lp;
         if (a.kept) a.kept[row] = kept;
     };
@@ -1036,7 +1039,7 @@ size_t sample_smem(int slice) { return (sizeof(SampleShared) + 15) / 16 * 16 + (
 }  // namespace
 
 // the launch of checked arguments (the engine's sampling calls it too)
-cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void *const *rows, int32_t *const *picks, cudaStream_t st) {
+cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void *const *rows, SessDev *const *states, cudaStream_t st) {
     const void *fn = a.type == IMI_F32   ? (const void *) k_sample<float>
                      : a.type == IMI_F16 ? (const void *) k_sample<__half>
                                           : (const void *) k_sample<__nv_bfloat16>;
@@ -1048,7 +1051,7 @@ cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void 
     // and cost where the short way does (32 rows of 32,000 by top-k: 8.1 us with 4, 15.4 with 8; 64 of 8,000: 7.1 with 2, 8.9 with 4)
     int C = 1;
     while (C < SM_MAX_CLUSTER && ((a.vocab + C - 1) / C > SM_SLICE || (a.n * C < SM_FEW(C) && a.vocab > C * SM_NW * SM_TILE))) C *= 2;
-    SampleArgs p = { a, 0, 0, rows, picks };
+    SampleArgs p = { a, 0, 0, rows, states };
     p.seg = ((a.vocab + C * SM_NW - 1) / (C * SM_NW) + SM_TILE - 1) / SM_TILE * SM_TILE;
     p.slice = p.seg * SM_NW;
     void *args[] = { &p };
