@@ -14,6 +14,28 @@ struct SessDev;   // common.cuh: a conversation's scalars on the device
 
 imi_cuda_status set_error(imi_cuda_status st, const std::string &msg);   // engine.cpp: the text of imi_cuda_error()
 
+// How sampling cuts n rows of vocab words: `ctas` per row (a cluster), `share` words for each of them but the last, held in SM_NW
+// parts of `seg` (a multiple of SM_TILE). CTAs per row: as many as hold the row, more while the call has few (SM_FEW) and a CTA
+// keeps a tile per warp. More CTAs help the passes over the row (one row of 97,496 by nucleus: 22 us with 8, 25.9 with 4; 16 of
+// 32,000: 15.4 with 4, 38 with 1), and cost where the short way does (32 rows of 32,000 by top-k: 8.1 us with 4, 15.4 with 8; 64 of
+// 8,000: 7.1 with 2, 8.9 with 4). The words are shared out evenly, by fours (the loads' width): CTAs filled to their last part one
+// after the other leave some cluster's last ones with few words or none, whose threads' maxima then bound nothing, and the row
+// misses its short list (one row of 50,257 by top-k 50: 23.9 us so, 7.4 shared out)
+constexpr int SM_NW = 16;                // warps of a CTA
+constexpr int SM_TILE = 128;             // words of a warp's load: four per lane
+constexpr int SM_MAX_CLUSTER = 8;
+constexpr int SM_SLICE = 32768;          // words a CTA holds at most
+constexpr int SM_FEW(int c) { return c < 4 ? 96 : 48; }   // CTAs of a call, of c per row, below which its rows get twice as many
+struct SampleSplit {
+    int ctas, seg, share;
+};
+inline SampleSplit sample_split(int n, int vocab) {
+    int c = 1;
+    while (c < SM_MAX_CLUSTER && ((vocab + c - 1) / c > SM_SLICE || (n * c < SM_FEW(c) && vocab > c * SM_NW * SM_TILE))) c *= 2;
+    const int share = ((vocab + c - 1) / c + 3) / 4 * 4;
+    return { c, ((share + SM_NW - 1) / SM_NW + SM_TILE - 1) / SM_TILE * SM_TILE, share };
+}
+
 // serve_sample.cu: sampling of checked arguments with `device` current; rows (or null): device pointers of the rows' scores,
 // states (or null): the conversations whose last pick, with its score, the words become
 cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void *const *rows, SessDev *const *states, cudaStream_t st);

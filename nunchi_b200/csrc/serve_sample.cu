@@ -32,7 +32,7 @@ namespace cg = cooperative_groups;
 namespace imi {
 namespace {
 
-constexpr int SM_NT = 512, SM_NW = SM_NT / 32;
+constexpr int SM_NT = 32 * SM_NW;
 constexpr int SM_BINS = 2 * SM_NT;       // two bins per thread in the scans
 constexpr int SM_LIST = 768;             // words of a list at most
 constexpr int SM_AIM = 384;              // words listed for top-p alone, about
@@ -42,10 +42,6 @@ constexpr int SM_STEPS = 256;            // steps in which the threads' maxima a
 // the 32-bit mass's relative error at most: of a word's exponent (up to 45) 2^-23 twice, in powers of 2, its exp2 2^-22, the
 // sum of up to 64 words of a thread 2^-18; the threads' sums are added in 64 bits
 constexpr double SM_MASS_ERR = 45 * 0.7 * 2.4e-7 + 2.4e-7 + 3.9e-6;
-constexpr int SM_TILE = 128;             // words of a warp's load: four per lane
-constexpr int SM_MAX_CLUSTER = 8;
-constexpr int SM_SLICE = 32768;          // words a CTA holds at most
-constexpr int SM_FEW(int c) { return c < 4 ? 96 : 48; }   // CTAs of a call, of c per row, below which its rows get twice as many
 constexpr double SM_ONE = 17592186044416.0;   // 2^44
 static_assert((long long) SM_SLICE * SM_MAX_CLUSTER >= IMI_CUDA_SAMPLE_VOCAB, "a row fits a cluster");
 static_assert((long long) IMI_CUDA_SAMPLE_VOCAB <= 1 << 18, "the weights' sum fits 62 bits");
@@ -54,7 +50,7 @@ typedef unsigned long long u64;
 
 struct SampleArgs {
     imi_cuda_sample_args a;
-    int seg, slice;   // words per warp (a multiple of SM_TILE) and per CTA (SM_NW * seg)
+    int seg, share;            // sample_split
     const void *const *rows;   // the rows' scores where they do not lie `stride` apart (the engine's conversations)
     SessDev *const *states;    // and the conversations whose last pick each row's word becomes (not if there is none)
 };
@@ -280,7 +276,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int) cl.num_blocks(), rank = (int) cl.block_rank();
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int base = rank * p.slice;                       // this CTA's first word
+    const int base = rank * p.share, end = min(a.vocab, base + p.share);   // this CTA's words
     if (tid == 0) { s.mx = 0; s.mn = ~0u; s.nvalid = 0; s.idmin = ~0u; s.n_list = s.n_all = 0; s.floor = s.lmin = ~0u; }
     if (tid < SM_STEPS) s.steps[tid] = 0;
     __syncthreads();
@@ -308,7 +304,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
         mx = max(max(mx, max(k.x, k.y)), max(k.z, k.w));
         *(uint4 *) (mine + o) = k;
     };
-    const int inside = a.vocab - (base + warp * p.seg);     // words of the row in this warp's part
+    const int inside = end - (base + warp * p.seg);         // words of the row in this warp's part
     const int whole = vec ? max(0, min(p.seg, inside / SM_TILE * SM_TILE)) : 0;
     int o = 0;
     constexpr int BATCH = sizeof(S) == 4 ? 4 : 6;           // tiles' loads in flight
@@ -332,7 +328,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
             for (int e = 0; e < 4; e++) f[e] = score_at((const S *) &v, e);
         } else
 #pragma unroll
-            for (int e = 0; e < 4; e++) f[e] = first + o + e < a.vocab ? score_at(x, first + o + e) : -INFINITY;
+            for (int e = 0; e < 4; e++) f[e] = first + o + e < end ? score_at(x, first + o + e) : -INFINITY;
         put(o, f);
     }
     // the value that the r-th largest of the threads' maxima reaches: the maxima ranked in 256 steps, all steps down to the
@@ -1046,16 +1042,10 @@ cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void 
     static SmemLimit lim;
     cudaError_t r = lim.raise(device, { (const void *) k_sample<float>, (const void *) k_sample<__half>, (const void *) k_sample<__nv_bfloat16> },
                               (int) sample_smem(SM_SLICE));
-    // CTAs per row: as many as hold the row, more while the call has few (SM_FEW) and a CTA keeps a tile per warp. More CTAs help
-    // the passes over the row (one row of 97,496 by nucleus: 22 us with 8, 25.9 with 4; 16 of 32,000: 15.4 with 4, 38 with 1),
-    // and cost where the short way does (32 rows of 32,000 by top-k: 8.1 us with 4, 15.4 with 8; 64 of 8,000: 7.1 with 2, 8.9 with 4)
-    int C = 1;
-    while (C < SM_MAX_CLUSTER && ((a.vocab + C - 1) / C > SM_SLICE || (a.n * C < SM_FEW(C) && a.vocab > C * SM_NW * SM_TILE))) C *= 2;
-    SampleArgs p = { a, 0, 0, rows, states };
-    p.seg = ((a.vocab + C * SM_NW - 1) / (C * SM_NW) + SM_TILE - 1) / SM_TILE * SM_TILE;
-    p.slice = p.seg * SM_NW;
+    const SampleSplit cut = sample_split(a.n, a.vocab);
+    SampleArgs p = { a, cut.seg, cut.share, rows, states };
     void *args[] = { &p };
-    if (r == cudaSuccess) r = launch_pdl(fn, dim3(a.n * C), SM_NT, sample_smem(p.slice), st, args, C);
+    if (r == cudaSuccess) r = launch_pdl(fn, dim3(a.n * cut.ctas), SM_NT, sample_smem(cut.seg * SM_NW), st, args, cut.ctas);
     return r;
 }
 }  // namespace imi

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import nunchi_b200 as nb
-from test_gpu_serve_ops import I32, attn_case, dev, run_attn, torch
+from test_gpu_serve_ops import FILTERS, I32, attn_case, dev, run_attn, run_sample, scores, torch
 
 pytestmark = pytest.mark.gpu
 
@@ -146,3 +146,23 @@ def test_page_map_in_place_step_after_step(n, cap, steps):
     i = np.repeat(np.arange(n), add)
     assert np.array_equal(pos.cpu().numpy()[:p.size], p) and (slots.cpu().numpy()[p.size:] == -1).all()
     assert np.array_equal(slots.cpu().numpy()[:p.size], want[i, p // page] * page + p % page)
+
+
+# ---------------------------------------------------------------------------------------------------------- sample
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 3, 13, 50])
+@pytest.mark.parametrize("vocab", [2049, 4097, 8195, 16385, 24000, 50257, 57345, 65537, 100277, 131071])
+def test_sample_rows_that_clusters_share_unevenly(vocab, n, dt):
+    """Rows just above what a number of CTAs' parts hold, and others that do not divide: the same words at every cluster size; the
+    last word of the row, and the words at the CTAs' ends, are drawn too."""
+    x = scores(n, vocab, dt, vocab + n)
+    rng = np.random.default_rng(vocab)
+    for f in (1, 2, 4, 7, 8, 9, 11):
+        run_sample(x, rng.random(n), **FILTERS[f])
+    y = torch.full((n, vocab), -float("inf"), device="cuda")
+    ends = [e for c in (1, 2, 4, 8) for r in range(1, c + 1) for e in (r * -(-vocab // c // 4) * 4, r * -(-vocab // c)) for e in (e - 1, e, e + 1)]
+    ends = sorted({e for e in ends + [0, vocab - 1] if 0 <= e < vocab})
+    y[:, ends] = torch.linspace(0, 1, len(ends), device="cuda")
+    for u in (0.0, 0.37, 0.9999999):
+        run_sample(y, u)
+        run_sample(y, u, k=max(1, len(ends) - 3), p=0.9)
