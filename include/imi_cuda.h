@@ -344,10 +344,10 @@ imi_cuda_status imi_cuda_page_write(int device, const imi_cuda_page_write_args *
  * length may hold anything, NaN included; a NaN or infinity in V at a prompt position that some conversation's window
  * includes may reach the others' outputs too.
  * type: IMI_F16 or IMI_BF16, of q and the pages; products, softmax and sums are held in 32 bits, the probabilities
- * rounded to `type` for their product with V. out_type: any imi_cuda_type. head_dim 64 or 128; n_head / n_head_kv at
- * most 16; rows at most 4096; page a power of two, 16..256; the prompt and a table row together at most 2^30 - page
- * positions, all table rows below 2^35; q and pages 16-byte aligned, q's and out's rows
- * q_stride / out_stride elements apart (multiples of 8), heads head_dim apart. A length beyond its table row
+ * rounded to `type` for their product with V. scale * log2(e) is finite. out_type: any imi_cuda_type. head_dim 64 or
+ * 128; n_head / n_head_kv at most 16; rows at most 4096; page a power of two, 16..256; the prompt and a table row together
+ * at most 2^30 - page positions, all table rows below 2^35; q and pages 16-byte aligned, q's and out's rows q_stride /
+ * out_stride elements apart (multiples of 8), heads head_dim apart. A length beyond its table row
  * (IMI_DEV_TABLE) counts as the row's positions; a page number outside the pool (IMI_DEV_PAGE) hides its positions.
  * work: imi_cuda_prefix_attn_work(...) bytes, 16-byte aligned, nothing expected in it; calls that may overlap need one
  * each. lse and status optional. */

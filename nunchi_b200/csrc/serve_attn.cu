@@ -433,7 +433,7 @@ __device__ __forceinline__ float4 scaled(float4 s, float l) {
     const float f = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);   // l NaN stays NaN
     return make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
 }
-constexpr float LN2 = 0.693147180559945309f;
+constexpr float LN2 = 0.693147180559945309f, LOG2E = 1.44269504088896340736f;
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2; }
 
 // ---- few positions: one CTA per (conversation, kv head) takes all of them, its warps step by step in turn ----
@@ -921,7 +921,7 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
                                         ", head_dim 64 or 128, up to 16 heads per kv head, page a power of two in 16..256, prompt and table "
                                         "row below 2^30 positions, all rows' tables below 2^35)");
     if (a->n_pages < 0 || a->window < 0) return set_error(IMI_E_ARG, "prefix_attn: negative n_pages or window");
-    if (!std::isfinite(a->scale)) return set_error(IMI_E_ARG, "prefix_attn: scale is not finite");
+    if (!std::isfinite(a->scale * LOG2E)) return set_error(IMI_E_ARG, "prefix_attn: scale is not finite, or not in powers of two");
     if (a->rows == 0) return IMI_OK;
     if (((int64_t) a->n_pages * a->n_head_kv + 1) * a->page > INT32_MAX) return set_error(IMI_E_ARG, "prefix_attn: too many pages");
     if ((int64_t) a->rows * a->n_head / PM_ROWS * ((int64_t) a->prefix_len / PM_N + 1) > INT32_MAX / 4)
@@ -948,7 +948,7 @@ extern "C" imi_cuda_status imi_cuda_prefix_attn(int device, const imi_cuda_prefi
     p.a = *a;
     p.shift = log2i(a->page);
     p.g = a->n_head / a->n_head_kv;
-    p.sl2 = a->scale * 1.44269504088896340736f;
+    p.sl2 = a->scale * LOG2E;
     p.pre_splits = pl.splits;
     p.pre_len = pl.len;
     p.mma = pl.mma;

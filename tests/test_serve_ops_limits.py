@@ -27,3 +27,12 @@ def test_prefix_attn_takes_sizes_below_the_limits(rows, prefix, width, page):
     st, msg = call("prefix_attn", nb._PREFIX_ATTN, a)
     assert "unsupported shape" not in msg
     assert nb.lib().imi_cuda_prefix_attn_work(rows, 32, 8, 64, prefix, width, page) > 0
+
+
+def test_prefix_attn_refuses_a_scale_that_overflows_in_powers_of_two():
+    """The kernels work in powers of two: what is finite has to stay so times log2(e) = 1.4427."""
+    for scale in (3e38, -2.4e38):
+        st, msg = call("prefix_attn", nb._PREFIX_ATTN, ATTN, scale=scale)
+        assert st == 1 and "scale" in msg
+    for scale in (2.3e38, -2.3e38, 0.0, 1e-45):
+        assert "scale" not in call("prefix_attn", nb._PREFIX_ATTN, ATTN, scale=scale)[1]
