@@ -56,6 +56,10 @@ template <> struct Half2<__half> {
         const __half2 h = __floats2half2_rn(a, b);
         return *(const uint32_t *) &h;
     }
+    static __device__ __forceinline__ uint32_t times_zero(uint32_t x) {   // what is not finite becomes NaN
+        const __half2 h = __hmul2(*(const __half2 *) &x, __floats2half2_rn(0.0f, 0.0f));
+        return *(const uint32_t *) &h;
+    }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -65,6 +69,10 @@ template <> struct Half2<__half> {
 template <> struct Half2<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *(const uint32_t *) &h;
+    }
+    static __device__ __forceinline__ uint32_t times_zero(uint32_t x) {   // what is not finite becomes NaN
+        const __nv_bfloat162 h = __hmul2(*(const __nv_bfloat162 *) &x, __floats2bfloat162_rn(0.0f, 0.0f));
         return *(const uint32_t *) &h;
     }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

@@ -193,8 +193,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
         return false;
     };
     const int qrows = a.rows * p.g;
-    const float sl2 = fabsf(p.sl2);                            // a negative scale turns q around
-    const bool turn = p.sl2 < 0.0f;
+    // a negative scale turns q around; a scale of 0, which must not meet a mask's -infinity, is multiplied into it
+    const float sl2 = p.sl2 == 0.0f ? 1.0f : fabsf(p.sl2);
+    const bool turn = p.sl2 < 0.0f, flat = p.sl2 == 0.0f;
     const int line = p.rtiles * a.n_head_kv * p.span, end = min(line, ((int) blockIdx.x + 1) * p.per);
     int at = (int) blockIdx.x * p.per;
     struct Unit {
@@ -238,6 +239,9 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
                     if (turn) { v[c].x ^= 0x80008000u; v[c].y ^= 0x80008000u; v[c].z ^= 0x80008000u; v[c].w ^= 0x80008000u; }
+                    if (flat)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) (&v[c].x)[e] = Half2<T>::times_zero((&v[c].x)[e]);
                     *(uint4 *) (dst + (c / 8) * (PM_M * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[c];
                 }
             }
@@ -430,21 +434,17 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                     pm_fence_before();
                     pm_arrive(&s_read[st]);
                 }
-                // masked behind the scale: a scale of 0 must not meet the mask's infinity. sc: what the scores still take
-                float sc = sl2;
-                if (masked) {
+                if (masked)
 #pragma unroll
                     for (int x = 0; x < PM_N; x++)
-                        v[x] = x < from || x >= to || (groups >> (x / 16) & 1) ? -INFINITY : v[x] * sl2;
-                    sc = 1.0f;
-                }
+                        if (x < from || x >= to || (groups >> (x / 16) & 1)) v[x] = -INFINITY;
                 float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
                 for (int x = 0; x < PM_N; x += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++) t4[e] = fmaxf(t4[e], fmaxf(v[x + e], v[x + e + 4]));
                 float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                top = top == -INFINITY ? top : top * sc;
+                top = top == -INFINITY ? top : top * sl2;
                 const bool raise = top > m + PM_RISE || (m == -INFINITY && top > m);
                 const bool any = __any_sync(~0u, raise);
                 // the product of the tile before reads P and adds to O: done before either is written
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(PM_THREADS, 1) k_pa_mma(const __grid_constant_
                     if (!ok) break;
                 }
                 const float u = m == -INFINITY ? 0.0f : -m;
-                const float2 s2 = make_float2(sc, sc), u2 = make_float2(u, u);
+                const float2 s2 = make_float2(sl2, sl2), u2 = make_float2(u, u);
                 float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
