@@ -349,6 +349,8 @@ imi_cuda_status imi_cuda_page_write(int device, const imi_cuda_page_write_args *
  * at most 2^30 - page positions, all table rows below 2^35; q and pages 16-byte aligned, q's and out's rows q_stride /
  * out_stride elements apart (multiples of 8), heads head_dim apart. A length beyond its table row
  * (IMI_DEV_TABLE) counts as the row's positions; a page number outside the pool (IMI_DEV_PAGE) hides its positions.
+ * The call is planned from width, not from the lengths: a width near the longest own length serves it best (table_stride
+ * may be larger; a workspace for a larger width fits).
  * work: imi_cuda_prefix_attn_work(...) bytes, 16-byte aligned, nothing expected in it; calls that may overlap need one
  * each. lse and status optional. */
 typedef struct {

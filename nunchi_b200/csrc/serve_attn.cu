@@ -7,6 +7,8 @@
 // piece gives (m, l, sum) and pieces join by rescaling to the largest m. The shared prompt is cut into pieces that
 // serve all conversations at once (rows of many conversations against one read of K and V); each conversation's own
 // positions into pieces of equal length; k_join adds them up.
+// Scores, maxima, sums and O are held in 32 bits. The weights 2^(s - m) are rounded to the pages' type for their product with V,
+// which the matrix instructions take in one type: half a step of it relative to each weight, and l is summed before that rounding.
 #include "common.cuh"
 #include "serve.h"
 

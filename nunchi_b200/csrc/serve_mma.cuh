@@ -18,7 +18,7 @@
 //                row's 128 scores
 // K is [position][dimension], the B operand with K = dimension contiguous; V is the B operand with N = dimension contiguous.
 // Bound by the exponentials: 16 per clock and SM, 2,048 clocks for two streams' tile; the products of head_dim 64 take half that.
-// Measured: 1.53 us for two streams' tile (1.07 at that rate); 256 conversations of 32 heads on 16,384 positions 65 us in all.
+// Measured: 1.64 us for two streams' tile (1.07 at that rate); 256 conversations of 32 heads on 16,384 positions 66 us in all.
 #pragma once
 
 constexpr int PM_M = 128, PM_N = 128, PM_ROWS = 2 * PM_M;
