@@ -5,6 +5,8 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <initializer_list>
 #include <mutex>
 #include <string>
@@ -25,15 +27,25 @@ constexpr int SM_NW = 16;                // warps of a CTA
 constexpr int SM_TILE = 128;             // words of a warp's load: four per lane
 constexpr int SM_MAX_CLUSTER = 8;
 constexpr int SM_SLICE = 32768;          // words a CTA holds at most
+constexpr int SM_LIST = 768;             // words of a list at most
+constexpr int SM_AIM(int c) { return c == 1 ? 600 : c == 2 ? 480 : 425; }   // words listed for top-p alone, about
 constexpr int SM_FEW(int c) { return c < 4 ? 96 : 48; }   // CTAs of a call, of c per row, below which its rows get twice as many
+// rank: for top-p alone, which of a CTA's threads' maxima bounds the list. Of L threads with q words each, a share f of the words is
+// above the (1 - (1 - f)^q) L-th largest of their maxima; f is set for SM_AIM words of the row, L and q are the last CTA's. The more
+// CTAs, the more their lowest bound lists beside that: about 500 words with 2 to 8; one CTA leaves 4 standard deviations to SM_LIST. (A fixed rank
+// of 384 over the CTAs asked one CTA for more maxima than it had, or for so low a one that the list overflowed: 100 rows of 5,000 by
+// nucleus 0.9 22.1 us so, 14.8 by this.) A row that fits the list whole is listed whole: a rank beyond all threads
 struct SampleSplit {
-    int ctas, seg, share;
+    int ctas, seg, share, rank;
 };
 inline SampleSplit sample_split(int n, int vocab) {
     int c = 1;
     while (c < SM_MAX_CLUSTER && ((vocab + c - 1) / c > SM_SLICE || (n * c < SM_FEW(c) && vocab > c * SM_NW * SM_TILE))) c *= 2;
     const int share = ((vocab + c - 1) / c + 3) / 4 * 4;
-    return { c, ((share + SM_NW - 1) / SM_NW + SM_TILE - 1) / SM_TILE * SM_TILE, share };
+    const int seg = ((share + SM_NW - 1) / SM_NW + SM_TILE - 1) / SM_TILE * SM_TILE, last = vocab - (c - 1) * share;
+    const int lanes = last / seg * 32 + std::min(32, (last % seg + 3) / 4);
+    const double above = 1.0 - std::pow(1.0 - std::min(1.0, (double) SM_AIM(c) / vocab), (double) last / lanes);
+    return { c, seg, share, vocab <= SM_LIST ? 32 * SM_NW : std::max(1, (int) (above * lanes)) };
 }
 
 // serve_sample.cu: sampling of checked arguments with `device` current; rows (or null): device pointers of the rows' scores,

@@ -11,7 +11,7 @@
 // read from HBM once, and every later pass is over shared memory.
 //   The list: while loading, every thread keeps its own words' maximum. The r-th largest of a CTA's thread maxima is a value
 // that r of its words reach, so the smallest of these over the cluster, with r = ceil(k / CTAs), is one that k words reach;
-// for top-p alone r is set for about 400 words, for min-p alone the value follows from the maximum. The words above it are
+// for top-p alone r is set for about 500 words, for min-p alone the value follows from the maximum. The words above it are
 // listed, and one CTA applies the filters to the list. What top-p needs of the other words is their mass: it is summed
 // in 32 bits, and only where the nucleus's end depends on the error of that sum, or lies below the list, in full.
 //   A nucleus, or a top-k, that goes on below the list: a histogram over 1,024 steps of score, of masses (or counts), is
@@ -34,8 +34,6 @@ namespace {
 
 constexpr int SM_NT = 32 * SM_NW;
 constexpr int SM_BINS = 2 * SM_NT;       // two bins per thread in the scans
-constexpr int SM_LIST = 768;             // words of a list at most
-constexpr int SM_AIM = 384;              // words listed for top-p alone, about
 constexpr int SM_SHORT = SM_NT / 4;      // words of a list that are all compared with one another
 constexpr int SM_PILES = 256;            // piles that a search in a longer list throws its words into
 constexpr int SM_STEPS = 256;            // steps in which the threads' maxima are ranked
@@ -50,7 +48,7 @@ typedef unsigned long long u64;
 
 struct SampleArgs {
     imi_cuda_sample_args a;
-    int seg, share;            // sample_split
+    int seg, share, rank;      // sample_split
     const void *const *rows;   // the rows' scores where they do not lie `stride` apart (the engine's conversations)
     SessDev *const *states;    // and the conversations whose last pick each row's word becomes (not if there is none)
 };
@@ -334,7 +332,7 @@ __global__ void __launch_bounds__(SM_NT, 2) k_sample(const __grid_constant__ Sam
     // the value that the r-th largest of the threads' maxima reaches: the maxima ranked in 256 steps, all steps down to the
     // one of the r-th taken whole
     const bool by_k = use_k && top_k <= SM_LIST, by_p = !use_k && use_p, by_m = !use_k && !use_p && use_m;
-    const int r_th = by_k ? (top_k + C - 1) / C : by_p ? SM_AIM / C : 0;
+    const int r_th = by_k ? (top_k + C - 1) / C : by_p ? p.rank : 0;
     const bool lists = !greedy && r_th <= SM_NT && (by_k || by_p || by_m);
     const uint32_t lmx = mx, wmax = __reduce_max_sync(~0u, mx);
     if (lane == 0) atomicMax(&s.mx, wmax);
@@ -1043,7 +1041,7 @@ cudaError_t launch_sample(int device, const imi_cuda_sample_args &a, const void 
     cudaError_t r = lim.raise(device, { (const void *) k_sample<float>, (const void *) k_sample<__half>, (const void *) k_sample<__nv_bfloat16> },
                               (int) sample_smem(SM_SLICE));
     const SampleSplit cut = sample_split(a.n, a.vocab);
-    SampleArgs p = { a, cut.seg, cut.share, rows, states };
+    SampleArgs p = { a, cut.seg, cut.share, cut.rank, rows, states };
     void *args[] = { &p };
     if (r == cudaSuccess) r = launch_pdl(fn, dim3(a.n * cut.ctas), SM_NT, sample_smem(cut.seg * SM_NW), st, args, cut.ctas);
     return r;

@@ -10,7 +10,7 @@ int main(int argc, char **argv) {
     const int n = atoi(argv[1]), lo = atoi(argv[2]), hi = atoi(argv[3]), step = atoi(argv[4]);
     for (int v = lo; v <= hi; v += step) {
         const imi::SampleSplit s = imi::sample_split(n, v);
-        printf("%d %d %d %d\n", v, s.ctas, s.seg, s.share);
+        printf("%d %d %d %d %d\n", v, s.ctas, s.seg, s.share, s.rank);
     }
     return 0;
 }

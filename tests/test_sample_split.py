@@ -30,7 +30,7 @@ def split(tmp_path_factory):
 @pytest.mark.parametrize("n", [1, 5, 11, 12, 24, 40, 64, 96, 65535])
 @pytest.mark.parametrize("lo,hi,step", [(1, 20000, 1), (16001, VOCAB, 37), (VOCAB - 100, VOCAB, 1)])
 def test_every_cta_has_its_share(split, n, lo, hi, step):
-    v, ctas, seg, share = split(n, lo, hi, step)
+    v, ctas, seg, share, _ = split(n, lo, hi, step)
     last = v - (ctas - 1) * share
     assert (last > 0).all() and (last <= share).all()                # all words, and no CTA without
     assert (share - last < 4 * ctas).all()                           # as many as the others, to a load each
@@ -41,3 +41,28 @@ def test_every_cta_has_its_share(split, n, lo, hi, step):
     # words each) are more than a nucleus's list asks of a CTA, about 384 / c
     m = ctas > 1
     assert (last[m] > 1024 - 4 * ctas[m]).all() and (last[m] // 4 >= 384 // ctas[m]).all()
+
+
+@pytest.mark.parametrize("n", [1, 12, 24, 48, 96])
+def test_a_nucleus_s_list_is_bounded_by_threads_that_have_words(split, n):
+    """The maximum that bounds the list is one that the last CTA has, and of words in any order about 500 are above it, well within
+    the list's 768: over 200 random rows of some sizes, by the layout's own threads."""
+    v, ctas, seg, share, rank = split(n, 769, 20000, 13)
+    last = v - (ctas - 1) * share
+    lanes = last // seg * 32 + np.minimum(32, -(-(last % seg) // 4))
+    assert (rank >= 1).all() and (rank < lanes).all()
+    rng = np.random.default_rng(n)
+    for i in rng.choice(v.size, 8, replace=False):
+        listed = []
+        for _ in range(200):
+            x, floor = rng.random(v[i]), 1.0
+            for r in range(ctas[i]):
+                part = x[r * share[i]:(r + 1) * share[i]]
+                at = np.arange(part.size)
+                top = np.zeros(16 * 32)
+                np.maximum.at(top, at // seg[i] * 32 + at % seg[i] % TILE // 4, part)
+                floor = min(floor, np.sort(top)[-rank[i]])
+            listed.append((x >= floor).sum())
+        # the r-th maximum's place varies by about sqrt(r): the lowest of up to 8 CTAs' lists a third more than one's
+        assert 300 < np.mean(listed) < 640 and np.max(listed) <= 768, (v[i], np.mean(listed), np.max(listed))
+    assert (split(n, 1, 768, 1)[4] == 512).all()
