@@ -32,9 +32,9 @@ constexpr int SM_AIM(int c) { return c == 1 ? 600 : c == 2 ? 480 : 425; }   // w
 constexpr int SM_FEW(int c) { return c < 4 ? 96 : 48; }   // CTAs of a call, of c per row, below which its rows get twice as many
 // rank: for top-p alone, which of a CTA's threads' maxima bounds the list. Of L threads with q words each, a share f of the words is
 // above the (1 - (1 - f)^q) L-th largest of their maxima; f is set for SM_AIM words of the row, L and q are the last CTA's. The more
-// CTAs, the more their lowest bound lists beside that: about 500 words with 2 to 8; one CTA leaves 4 standard deviations to SM_LIST. (A fixed rank
-// of 384 over the CTAs asked one CTA for more maxima than it had, or for so low a one that the list overflowed: 100 rows of 5,000 by
-// nucleus 0.9 22.1 us so, 14.8 by this.) A row that fits the list whole is listed whole: a rank beyond all threads
+// CTAs, the more their lowest bound lists beside that: about 500 words with 2 to 8; one CTA leaves 4 standard deviations to SM_LIST.
+// (A fixed rank of 384 over the CTAs asked one CTA for more maxima than it had, or for so low a one that the list overflowed: 100
+// rows of 5,000 by nucleus 0.9 22.1 us so, 14.8 by this.) A row that fits the list whole is listed whole: a rank beyond all threads
 struct SampleSplit {
     int ctas, seg, share, rank;
 };
