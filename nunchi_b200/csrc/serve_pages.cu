@@ -37,7 +37,7 @@ __device__ __forceinline__ int row_of(const int *first, int n, int j) {
 // written by the CTA that is the last to have read its inputs; the count of those that have is asked for before the tables
 // and slots are written, and its answer used after that. A CTA has read all of them by the scan's barrier; fences in front of
 // its count and behind the last one's order those reads before the writes.
-// Measured, one call behind the other: 64 decode steps 5.0 us, 384 prompts of 1,000,000 tokens at most (8 MB written) 10.2.
+// Measured, one call behind the other: 64 decode steps 5.0 us, 384 prompts of 1,000,000 tokens at most (8 MB written) 10.2 to 11.4.
 __global__ void __launch_bounds__(MAP_THREADS) k_page_map(const __grid_constant__ MapArgs m) {
     extern __shared__ int sh[];
     const imi_cuda_page_map_args &a = m.a;
